@@ -394,6 +394,94 @@ int m3_sample_tokens(const M3SampleArgs *args, void *stream);
 int m3_gated_act_bf16(const void *x, int64_t x_row_stride, void *out, int64_t out_row_stride, int64_t rows,
                       int32_t k, void *stream);
 
+/* ---------------------------------------------------------------------------------
+ * The vocabulary end of the language model.  No counterparts in the reference, which leaves
+ * these to XLA (embed[tokens], log_softmax, its gradient).  Rows are addressed by two levels
+ * of element strides, row r at (r / rows_inner) * outer + (r % rows_inner) * inner, so that
+ * logits[:, :-1] and tokens[:, 1:] need no copy; the vocabulary axis is contiguous.  All
+ * arithmetic is fp32.  Results are the same every call (no floating-point atomics).
+ * ------------------------------------------------------------------------------- */
+#define M3_MAX_TOP 128
+
+/* Per row x of logits, y = x / temperature: logprob = y[target] - lse(y) (target < 0: 0,
+ * target >= vocab: NaN), entropy of softmax(y), lse(y), and the `top` largest entries in
+ * descending order (equal logits: the lower index first; NaN above everything) with their
+ * log probabilities.  -inf logits have probability 0.  A row whose largest logit is not
+ * finite (every logit -inf, or one +inf or NaN) has no distribution: its floats are NaN. */
+typedef struct M3ScoreArgs {
+  int32_t rows_outer, rows_inner, vocab, top;    /* top <= min(vocab, M3_MAX_TOP) */
+  int32_t logits_dtype;                          /* M3_DTYPE_* */
+  float temperature;                             /* > 0 */
+  const void *logits;     int64_t ld_outer, ld_inner;
+  const int64_t *targets; int64_t t_outer, t_inner;  /* NULL: no logprob */
+  float *logprob, *entropy, *lse;                /* (rows) dense; logprob NULL iff targets NULL */
+  float *top_logprob;                            /* (rows, top) dense; NULL iff top == 0 */
+  int64_t *top_ids;
+} M3ScoreArgs;
+
+int m3_token_logprobs(const M3ScoreArgs *args, void *stream);
+
+/* Distillation from a teacher's k top logits, optionally mixed with hard labels:
+ *   p = softmax of the row's teacher logits / T over the entries with id >= 0
+ *   KL = sum_j p_j (ln p_j - ln softmax(x / T)[id_j]),   CE = -ln softmax(x)[label]
+ *   row loss = w [ (1 - hard_weight) T^2 KL + hard_weight CE ]
+ * and its gradient
+ *   g w [ (1 - hard_weight) T (softmax(x / T) - p) + hard_weight (softmax(x) - onehot(label)) ]
+ * times grad_scale and, for M3_REDUCE_MEAN, over sum(w); g is `upstream` (element r *
+ * upstream_stride; NULL = 1).  An id that occurs twice counts with both probabilities.
+ * label < 0: no CE term; no id >= 0: no KL term; a row with neither or with w == 0 has loss 0
+ * and gradient 0 whatever its logits are.  An id or label >= vocab makes the row NaN. */
+enum { M3_REDUCE_NONE = 0, M3_REDUCE_SUM = 1, M3_REDUCE_MEAN = 2 };
+
+typedef struct M3DistillArgs {
+  int32_t rows_outer, rows_inner, vocab, k;      /* 1 <= k <= M3_MAX_TOP */
+  int32_t logits_dtype, reduction;
+  float temperature, hard_weight, grad_scale;    /* T > 0, 0 <= hard_weight <= 1 */
+  const void *logits;     int64_t ld_outer, ld_inner;
+  const int64_t *ids;                            /* (rows, k) dense */
+  const float *teacher;                          /* (rows, k) dense */
+  const int64_t *labels;                         /* (rows); NULL iff hard_weight == 0 */
+  const float *weights;                          /* (rows); NULL = 1 */
+  const float *upstream;  int64_t upstream_stride;
+  float *row_loss;                               /* (rows): the rows' losses */
+  float *loss;                                   /* sum or mean; NULL iff M3_REDUCE_NONE */
+  float *weight_sum;                             /* one float of scratch for a mean with weights */
+  void *grad;             int64_t g_outer, g_inner;  /* logits' dtype; may be the logits; NULL = loss only */
+} M3DistillArgs;
+
+int m3_distill(const M3DistillArgs *args, void *stream);
+
+/* out[r] = scale * table[token r], rounded once; token < 0 (padding): zeros; token >= vocab: NaN. */
+typedef struct M3EmbedArgs {
+  int32_t rows_outer, rows_inner, vocab, dim;
+  int32_t table_dtype, out_dtype;
+  float scale;
+  int32_t reserved;
+  const int64_t *tokens;  int64_t t_outer, t_inner;
+  const void *table;      int64_t table_ld;
+  void *out;              int64_t out_ld;
+} M3EmbedArgs;
+
+int m3_embed(const M3EmbedArgs *args, void *stream);
+
+/* Gradient of m3_embed with respect to the table: grad[v] = scale * (sum of dy[r] over the rows
+ * with token v, r ascending, fp32), one rounding; tokens outside [0, vocab) have none.  accumulate
+ * == 0 writes every row of grad (zeros where a token does not occur); 1 adds to the rows that
+ * occur.  Workspace of m3_embed_bwd_workspace_size(rows, dim) bytes, 256-byte aligned. */
+typedef struct M3EmbedBwdArgs {
+  int32_t rows_outer, rows_inner, vocab, dim;
+  int32_t dy_dtype, grad_dtype;
+  float scale;
+  int32_t accumulate;
+  const int64_t *tokens;  int64_t t_outer, t_inner;
+  const void *dy;         int64_t dy_outer, dy_inner;
+  void *grad;             int64_t grad_ld;
+  void *workspace;        size_t workspace_bytes;
+} M3EmbedBwdArgs;
+
+size_t m3_embed_bwd_workspace_size(int64_t rows, int32_t dim);
+int m3_embed_bwd(const M3EmbedBwdArgs *args, void *stream);
+
 /* Last error message of this thread ("" if none). */
 const char *m3_last_error(void);
 

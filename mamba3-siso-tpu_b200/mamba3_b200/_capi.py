@@ -143,11 +143,55 @@ class M3GemmArgs(ctypes.Structure):
     ]
 
 
+class M3ScoreArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows_outer", _i32), ("rows_inner", _i32), ("vocab", _i32), ("top", _i32), ("logits_dtype", _i32),
+        ("temperature", _f32), ("logits", _vp), ("ld_outer", _i64), ("ld_inner", _i64),
+        ("targets", _vp), ("t_outer", _i64), ("t_inner", _i64),
+        ("logprob", _vp), ("entropy", _vp), ("lse", _vp), ("top_logprob", _vp), ("top_ids", _vp),
+    ]
+
+
+class M3DistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows_outer", _i32), ("rows_inner", _i32), ("vocab", _i32), ("k", _i32), ("logits_dtype", _i32),
+        ("reduction", _i32), ("temperature", _f32), ("hard_weight", _f32), ("grad_scale", _f32),
+        ("logits", _vp), ("ld_outer", _i64), ("ld_inner", _i64),
+        ("ids", _vp), ("teacher", _vp), ("labels", _vp), ("weights", _vp), ("upstream", _vp),
+        ("upstream_stride", _i64), ("row_loss", _vp), ("loss", _vp), ("weight_sum", _vp),
+        ("grad", _vp), ("g_outer", _i64), ("g_inner", _i64),
+    ]
+
+
+class M3EmbedArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows_outer", _i32), ("rows_inner", _i32), ("vocab", _i32), ("dim", _i32), ("table_dtype", _i32),
+        ("out_dtype", _i32), ("scale", _f32), ("reserved", _i32),
+        ("tokens", _vp), ("t_outer", _i64), ("t_inner", _i64), ("table", _vp), ("table_ld", _i64),
+        ("out", _vp), ("out_ld", _i64),
+    ]
+
+
+class M3EmbedBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows_outer", _i32), ("rows_inner", _i32), ("vocab", _i32), ("dim", _i32), ("dy_dtype", _i32),
+        ("grad_dtype", _i32), ("scale", _f32), ("accumulate", _i32),
+        ("tokens", _vp), ("t_outer", _i64), ("t_inner", _i64), ("dy", _vp), ("dy_outer", _i64), ("dy_inner", _i64),
+        ("grad", _vp), ("grad_ld", _i64), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+M3_MAX_TOP = 128
+M3_REDUCE_NONE = 0
+M3_REDUCE_SUM = 1
+M3_REDUCE_MEAN = 2
+
 EXPORTS = ("m3_siso_fwd", "m3_siso_fwd_workspace_size", "m3_siso_bwd", "m3_siso_bwd_workspace_size", "m3_siso_decode",
            "m3_last_error", "m3_version", "m3_siso_bwd_noalloc", "m3_siso_bwd_noalloc_scratch_bytes",
            "m3_device_error", "m3_copy2d_async", "m3_rms_norm", "m3_rms_norm_bwd", "m3_sample_tokens", "m3_gemv_bf16",
            "m3_gemv_scratch_floats", "m3_siso_fwd_saves_states", "m3_gated_act_bf16", "m3_siso_split_prep",
-           "m3_siso_split_carry", "m3_gemm_bf16")
+           "m3_siso_split_carry", "m3_gemm_bf16", "m3_token_logprobs", "m3_distill", "m3_embed", "m3_embed_bwd",
+           "m3_embed_bwd_workspace_size")
 
 _lib = None
 
@@ -201,6 +245,16 @@ def lib():
         L.m3_rms_norm_bwd.argtypes = [_vp, ctypes.c_int64, _vp, _vp, _vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp,
                                       ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _vp]
         L.m3_rms_norm_bwd.restype = ctypes.c_int
+        L.m3_token_logprobs.argtypes = [ctypes.POINTER(M3ScoreArgs), _vp]
+        L.m3_token_logprobs.restype = ctypes.c_int
+        L.m3_distill.argtypes = [ctypes.POINTER(M3DistillArgs), _vp]
+        L.m3_distill.restype = ctypes.c_int
+        L.m3_embed.argtypes = [ctypes.POINTER(M3EmbedArgs), _vp]
+        L.m3_embed.restype = ctypes.c_int
+        L.m3_embed_bwd.argtypes = [ctypes.POINTER(M3EmbedBwdArgs), _vp]
+        L.m3_embed_bwd.restype = ctypes.c_int
+        L.m3_embed_bwd_workspace_size.argtypes = [_i64, _i32]
+        L.m3_embed_bwd_workspace_size.restype = ctypes.c_size_t
         _lib = L
     return _lib
 

@@ -95,3 +95,45 @@ def st_bhlp(t) -> C.M3Strides:
 
 def st_blh(t) -> C.M3Strides:
     return C.M3Strides(t.stride(0), t.stride(2), t.stride(1))
+
+
+def rows2(t, nd):
+    """Element strides of the leading ``nd`` axes of ``t`` seen as two: (all but the last,
+    the last).  None if the outer ones do not collapse into one stride."""
+    if nd == 0:
+        return 0, 0
+    outer = [(s, st) for s, st in zip(t.shape[:nd - 1], t.stride()) if s != 1]
+    for (_, st0), (s1, st1) in zip(outer, outer[1:]):
+        if st0 != s1 * st1:
+            return None
+    return (outer[-1][1] if outer else 0), t.stride(nd - 1)
+
+
+def row_input(t, nd):
+    """``t`` with its trailing axis (if any, beyond the ``nd`` leading ones) contiguous and its
+    leading axes addressable by two strides, copied only where it is not, and those strides."""
+    st = rows2(t, nd) if t.dim() == nd or t.stride(-1) == 1 or t.shape[-1] == 1 else None
+    if st is None:
+        t = t.contiguous()
+        st = rows2(t, nd)
+    return t, st
+
+
+def row_counts(lead):
+    """(outer, inner) row counts of a leading shape, as `rows2` splits it."""
+    inner = lead[-1] if lead else 1
+    outer = 1
+    for s in lead[:-1]:
+        outer *= s
+    if outer * inner >= 1 << 31:
+        raise ValueError(f"{outer * inner} rows: at most 2^31 - 1 are supported")
+    return (outer, inner) if inner else (0, 1)
+
+
+def call(fn, args, device):
+    """One library call on the current stream of ``device``; raises on a non-zero status."""
+    if device.index is not None and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            C.check(fn(args, stream_handle(device)))
+    else:
+        C.check(fn(args, stream_handle(device)))

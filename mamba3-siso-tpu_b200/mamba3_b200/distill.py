@@ -1,0 +1,164 @@
+"""Distillation from a teacher's top logits, with hard labels mixed in (``m3_distill``).
+
+Per row x of student logits, with p the softmax of the teacher's k logits over T:
+
+    loss = w [ (1 - hard_weight) T^2 KL(p || softmax(x / T)) + hard_weight CE(x, label) ]
+
+`distill_loss` is an autograd function; `distill_loss_and_grad` gives the loss and the gradient
+with respect to the logits together, from one read of them (`train.make_distill_step`).  The
+teacher's lists are `scoring.token_logprobs`' ``top_ids`` and ``top_logprob``.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _capi as C
+from . import _tensors as T
+
+_REDUCE = {"none": C.M3_REDUCE_NONE, "sum": C.M3_REDUCE_SUM, "mean": C.M3_REDUCE_MEAN}
+
+
+def _check(logits, ids, teacher, labels, weights, temperature, hard_weight, reduction):
+    """Argument checks; returns the side inputs as the kernel reads them (dense int64 / f32)."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be (..., vocab), got {tuple(logits.shape)}")
+    T.require_cuda(logits, ids, teacher, labels, weights)
+    T.io_dtype(logits.dtype)
+    lead = logits.shape[:-1]
+    if ids.dim() != len(lead) + 1 or ids.shape[:-1] != lead or not 1 <= ids.shape[-1] <= C.M3_MAX_TOP:
+        raise ValueError(f"teacher_ids must be {tuple(lead)} + (k,), 1 <= k <= {C.M3_MAX_TOP}, got {tuple(ids.shape)}")
+    if teacher.shape != ids.shape:
+        raise ValueError(f"teacher_logits must have the shape of teacher_ids, got {tuple(teacher.shape)}")
+    if not temperature > 0 or not 0 <= hard_weight <= 1:
+        raise ValueError("need temperature > 0 and 0 <= hard_weight <= 1")
+    if reduction not in _REDUCE:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCE)}, got {reduction!r}")
+    if (labels is not None) != (hard_weight > 0):
+        raise ValueError("labels go with hard_weight > 0")
+    for name, t in (("labels", labels), ("weights", weights)):
+        if t is not None and t.shape != lead:
+            raise ValueError(f"{name} must be {tuple(lead)}, got {tuple(t.shape)}")
+    for name, t in (("teacher_ids", ids), ("labels", labels)):
+        if t is not None and t.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"{name} must be int64 or int32, got {t.dtype}")
+    for name, t in (("teacher_logits", teacher), ("weights", weights)):
+        if t is not None and not t.dtype.is_floating_point:
+            raise ValueError(f"{name} must be floating point, got {t.dtype}")
+    for t in (ids, teacher, labels, weights):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"every tensor must be on {logits.device}, got one on {t.device}")
+
+    def dense(t, dtype):
+        return None if t is None else t.detach().to(dtype).contiguous()
+
+    return dense(ids, torch.int64), dense(teacher, torch.float32), dense(labels, torch.int64), dense(
+        weights, torch.float32)
+
+
+def _run(logits, ids, teacher, labels, weights, temperature, hard_weight, reduction, grad=None, upstream=None,
+         grad_scale=1.0):
+    """One m3_distill call on checked inputs: the reduced loss, or the rows' losses."""
+    lead, dev = logits.shape[:-1], logits.device
+    nd = len(lead)
+    a = C.M3DistillArgs()
+    a.rows_outer, a.rows_inner = T.row_counts(lead)
+    a.vocab, a.k = logits.shape[-1], ids.shape[-1]
+    a.logits_dtype, a.reduction = T.io_dtype(logits.dtype), _REDUCE[reduction]
+    a.temperature, a.hard_weight, a.grad_scale = temperature, hard_weight, grad_scale
+    logits, (a.ld_outer, a.ld_inner) = T.row_input(logits, nd)
+    a.logits, a.ids, a.teacher = T.ptr(logits), T.ptr(ids), T.ptr(teacher)
+    a.labels, a.weights = T.ptr(labels), T.ptr(weights)
+    row_loss = torch.empty(lead, dtype=torch.float32, device=dev)
+    a.row_loss = T.ptr(row_loss)
+    loss = scratch = None
+    if reduction != "none":
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        a.loss = T.ptr(loss)
+        if reduction == "mean" and weights is not None:
+            scratch = torch.empty(1, dtype=torch.float32, device=dev)
+            a.weight_sum = T.ptr(scratch)
+    if grad is not None:
+        a.grad = T.ptr(grad)
+        a.g_outer, a.g_inner = T.rows2(grad, nd)
+    if upstream is not None:
+        a.upstream, a.upstream_stride = T.ptr(upstream), int(upstream.dim() > 0 and upstream.numel() > 1)
+    T.call(C.lib().m3_distill, a, dev)
+    return row_loss if loss is None else loss
+
+
+class _DistillFn(torch.autograd.Function):
+    """The forward reads the logits once; the backward reads them once more and writes their
+    gradient, the softmax recomputed in the same pass (nothing but the inputs is saved)."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, labels, weights, temperature, hard_weight, reduction):
+        ctx.save_for_backward(logits, ids, teacher, labels, weights)
+        ctx.opts = (temperature, hard_weight, reduction)
+        return _run(logits, ids, teacher, labels, weights, temperature, hard_weight, reduction)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        logits = ctx.saved_tensors[0]
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _run(*ctx.saved_tensors, *ctx.opts, grad=grad, upstream=dloss.float().contiguous())
+        return (grad,) + (None,) * 7
+
+
+def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                 temperature: float = 1.0, labels: Optional[torch.Tensor] = None, hard_weight: float = 0.0,
+                 weights: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
+    """The loss of ``logits (..., V)`` (bf16 or f32) against ``teacher_ids`` / ``teacher_logits``
+    ``(..., k)``, k <= 128; differentiable in ``logits`` alone.
+
+    A negative id is an absent entry, a negative label an absent label; the teacher's logits
+    may be shifted by any constant (log probabilities do).  ``weights (...)`` weigh the rows; a
+    row of weight 0, or with neither entries nor label, contributes exactly 0 to the loss and
+    the gradient whatever its logits are.  An id or label at or past V makes its row NaN.
+    ``reduction``: "mean" over the weights' sum (or the row count), "sum", or "none" for the
+    rows' losses."""
+    side = _check(logits, teacher_ids, teacher_logits, labels, weights, temperature, hard_weight, reduction)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillFn.apply(logits, *side, float(temperature), float(hard_weight), reduction)
+    return _run(logits.detach(), *side, temperature, hard_weight, reduction)
+
+
+@torch.no_grad()
+def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+                          temperature: float = 1.0, labels: Optional[torch.Tensor] = None, hard_weight: float = 0.0,
+                          weights: Optional[torch.Tensor] = None, reduction: str = "mean", grad_scale: float = 1.0,
+                          out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`distill_loss` ("mean" or "sum") and ``grad_scale`` times its gradient with respect to the
+    logits, in the logits' dtype, from one read of them.  ``out`` takes the gradient; it may be
+    ``logits`` itself, which are then overwritten."""
+    if reduction == "none":
+        raise ValueError("reduction must be 'mean' or 'sum'")
+    side = _check(logits, teacher_ids, teacher_logits, labels, weights, temperature, hard_weight, reduction)
+    nd = logits.dim() - 1
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype} on {logits.device}")
+    elif not _writable_rows(out, nd):
+        raise ValueError("out must have a contiguous vocabulary axis and rows that do not overlap")
+    loss = _run(logits, *side, temperature, hard_weight, reduction, grad=out, grad_scale=grad_scale)
+    return loss, out
+
+
+def _writable_rows(t, nd) -> bool:
+    if t.numel() == 0:
+        return True
+    st = T.rows2(t, nd)
+    if st is None or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        return False
+    outer, inner = T.row_counts(t.shape[:-1])
+    span = t.shape[-1]
+    for count, stride in sorted(((inner, st[1]), (outer, st[0])), key=lambda cs: cs[1]):
+        if count > 1:
+            if stride < span:
+                return False
+            span = stride * (count - 1) + span
+    return True

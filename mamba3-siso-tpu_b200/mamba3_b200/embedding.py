@@ -1,0 +1,100 @@
+"""Embedding lookup with scaling (``m3_embed``) and its gradient by sorted tokens (``m3_embed_bwd``).
+
+`embed_tokens` is ``(scale * table[tokens]).to(dtype)`` with one rounding and no intermediate
+copy; its gradient sums each token's rows in the order of their positions, in fp32, so that it
+is the same every run.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _capi as C
+from . import _tensors as T
+
+
+def _check_tokens(tokens, ref):
+    T.require_cuda(tokens, ref)
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"tokens must be int64 or int32, got {tokens.dtype}")
+    if tokens.device != ref.device:
+        raise ValueError(f"tokens must be on {ref.device}, got {tokens.device}")
+
+
+def _lookup(table, tokens, scale, dtype):
+    lead = tokens.shape
+    a = C.M3EmbedArgs()
+    a.rows_outer, a.rows_inner = T.row_counts(lead)
+    a.vocab, a.dim = table.shape
+    a.table_dtype, a.out_dtype, a.scale = T.io_dtype(table.dtype), T.io_dtype(dtype), scale
+    tokens, (a.t_outer, a.t_inner) = T.row_input(tokens.to(torch.int64), len(lead))
+    if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
+        table = table.contiguous()
+    out = torch.empty(*lead, a.dim, dtype=dtype, device=table.device)
+    a.tokens, a.table, a.table_ld, a.out, a.out_ld = T.ptr(tokens), T.ptr(table), table.stride(0), T.ptr(out), a.dim
+    T.call(C.lib().m3_embed, a, table.device)
+    return out
+
+
+class _EmbedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, tokens, scale, dtype):
+        ctx.save_for_backward(tokens)
+        ctx.vocab, ctx.scale, ctx.dtype = table.shape[0], scale, table.dtype
+        return _lookup(table, tokens, scale, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        tokens, = ctx.saved_tensors
+        return embedding_grad(dy, tokens, ctx.vocab, scale=ctx.scale, dtype=ctx.dtype), None, None, None
+
+
+def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
+                 dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``table (V, D)`` bf16 or f32, ``tokens (...)`` int -> ``(..., D)`` in ``dtype`` (the table's
+    by default).  A negative token is padding: a zero row without gradient; one at or past V
+    gives a NaN row.  Differentiable in ``table`` (a dense gradient in its dtype)."""
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"table must be (vocab, dim), got {tuple(table.shape)}")
+    _check_tokens(tokens, table)
+    dtype = table.dtype if dtype is None else dtype
+    T.io_dtype(table.dtype), T.io_dtype(dtype)
+    if torch.is_grad_enabled() and table.requires_grad:
+        return _EmbedFn.apply(table, tokens, float(scale), dtype)
+    return _lookup(table.detach(), tokens, scale, dtype)
+
+
+@torch.no_grad()
+def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: float = 1.0,
+                   dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of `embed_tokens` with respect to its table: ``dy (..., D)`` -> ``(vocab, D)``
+    in ``dtype``.  With ``out`` it is added to that ``(vocab, D)`` tensor instead (only the rows
+    of tokens that occur are touched; each sum is rounded once), e.g. the gradient a tied head
+    has left there."""
+    if dy.dim() != tokens.dim() + 1 or dy.shape[:-1] != tokens.shape or dy.shape[-1] < 1:
+        raise ValueError(f"dy must be {tuple(tokens.shape)} + (dim,), got {tuple(dy.shape)}")
+    if vocab < 1:
+        raise ValueError(f"vocab must be >= 1, got {vocab}")
+    _check_tokens(tokens, dy)
+    lead, dim, dev = tokens.shape, dy.shape[-1], dy.device
+    add = out is not None
+    if not add:
+        out = torch.empty(vocab, dim, dtype=dtype, device=dev)
+    elif out.shape != (vocab, dim) or out.device != dev or (dim > 1 and out.stride(1) != 1) or out.stride(0) < dim:
+        raise ValueError(f"out must be ({vocab}, {dim}) on {dev} with contiguous rows")
+    a = C.M3EmbedBwdArgs()
+    a.rows_outer, a.rows_inner = T.row_counts(lead)
+    a.vocab, a.dim, a.dy_dtype, a.grad_dtype = vocab, dim, T.io_dtype(dy.dtype), T.io_dtype(out.dtype)
+    a.scale, a.accumulate = scale, int(add)
+    nd = len(lead)
+    tokens, (a.t_outer, a.t_inner) = T.row_input(tokens.to(torch.int64), nd)
+    dy, (a.dy_outer, a.dy_inner) = T.row_input(dy, nd)
+    lib = C.lib()
+    ws = torch.empty(lib.m3_embed_bwd_workspace_size(a.rows_outer * a.rows_inner, dim), dtype=torch.uint8, device=dev)
+    a.tokens, a.dy, a.grad, a.grad_ld = T.ptr(tokens), T.ptr(dy), T.ptr(out), out.stride(0)
+    a.workspace, a.workspace_bytes = T.ptr(ws), ws.numel()
+    T.call(lib.m3_embed_bwd, a, dev)
+    return out

@@ -95,12 +95,14 @@ def init_lm(cfg: LMConfig, key=0, dtype=torch.float32, device="cuda") -> LMParam
 
 def lm_forward(params: LMParams, tokens: torch.Tensor, cfg: LMConfig, interpret=False, device_kind=None,
                states: Optional[List[SISOState]] = None, compute_dtype: Optional[torch.dtype] = None,
-               return_hidden: bool = False, logits: str = "all"):
+               return_hidden: bool = False, logits: str = "all", embeds: Optional[torch.Tensor] = None):
     """``model.py:194-232``: ``(B, L)`` tokens -> ``(B, L, vocab)`` logits (and the
     per-layer carry when ``states`` is given).  ``logits="last"`` computes the head for
     the final position only (``(B, vocab)``), ``"none"`` skips it (prefill for decode).
+    ``embeds`` are the tokens' embeddings ``(B, L, d_model)`` already looked up (e.g. by
+    `embedding.embed_tokens`); ``tokens`` are then not read.
     ``interpret`` / ``device_kind`` keep the reference's argument order; no effect here."""
-    x = params.embed[tokens]
+    x = params.embed[tokens] if embeds is None else embeds
     if compute_dtype is not None:
         x = x.to(compute_dtype)
     eps = cfg.siso.norm_eps

@@ -4,6 +4,7 @@
 process group it is data parallel: each rank runs its batch shard and the gradients are
 averaged with NCCL all-reduces issued bucket by bucket as the backward produces them
 (the counterpart of ``jax.lax.pmean`` inside ``shard_map``, ``train.py:427-451``).
+`make_distill_step` is the same step against a teacher's top logits, which `score` gives.
 `generate` is chunked prefill through the scan kernels, then one decode-kernel step per
 token with the sampling filters applied on the device.
 """
@@ -18,7 +19,10 @@ import torch.nn.functional as F
 
 from . import _capi as C
 from . import _tensors as T
+from . import distill as D
+from . import embedding as E
 from . import model as M
+from . import scoring as S
 from .sampling import TokenSampler
 
 
@@ -86,15 +90,9 @@ class GradBucketer:
         self.flats = [None] * len(self.buckets)
 
 
-def make_step(cfg: M.LMConfig, params: M.LMParams, lr: float = 1e-3, betas=(0.9, 0.95), eps: float = 1e-8,
-              weight_decay: float = 0.0, clip: Optional[float] = 1.0, compute_dtype=torch.bfloat16,
-              distributed: Optional[bool] = None):
-    """Build ``step(xs, ys) -> loss`` for fp32 master ``params`` (trained in place).
-
-    Forward and backward run in ``compute_dtype`` (bf16: the scan kernels take bf16
-    operands with fp32 state); the optimizer is torch's fused AdamW on the fp32 masters,
-    after a global-norm clip like ``optax.clip_by_global_norm`` (``train.py:799-805``).
-    """
+def _optimizer(params: M.LMParams, lr, betas, eps, weight_decay, clip, distributed):
+    """AdamW over the fp32 masters, and ``finish(loss)``: what every step does after its
+    backward (gradient averaging over the process group, clipping, the update)."""
     import torch.distributed as dist
 
     plist = param_list(params)
@@ -106,11 +104,7 @@ def make_step(cfg: M.LMConfig, params: M.LMParams, lr: float = 1e-3, betas=(0.9,
     opt = torch.optim.AdamW(plist, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                             fused=plist[0].is_cuda)
 
-    def step(xs: torch.Tensor, ys: torch.Tensor) -> torch.Tensor:
-        opt.zero_grad(set_to_none=False)
-        logits = M.lm_forward(params, xs, cfg, compute_dtype=compute_dtype)
-        loss = F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), ys.reshape(-1))
-        loss.backward()
+    def finish(loss: torch.Tensor) -> torch.Tensor:
         if bucketer is not None:
             bucketer.finish()
             loss = loss.detach().clone()
@@ -121,9 +115,70 @@ def make_step(cfg: M.LMConfig, params: M.LMParams, lr: float = 1e-3, betas=(0.9,
         opt.step()
         return loss.detach()
 
+    return opt, plist, finish
+
+
+def make_step(cfg: M.LMConfig, params: M.LMParams, lr: float = 1e-3, betas=(0.9, 0.95), eps: float = 1e-8,
+              weight_decay: float = 0.0, clip: Optional[float] = 1.0, compute_dtype=torch.bfloat16,
+              distributed: Optional[bool] = None):
+    """Build ``step(xs, ys) -> loss`` for fp32 master ``params`` (trained in place).
+
+    Forward and backward run in ``compute_dtype`` (bf16: the scan kernels take bf16
+    operands with fp32 state); the optimizer is torch's fused AdamW on the fp32 masters,
+    after a global-norm clip like ``optax.clip_by_global_norm`` (``train.py:799-805``).
+    """
+    opt, plist, finish = _optimizer(params, lr, betas, eps, weight_decay, clip, distributed)
+
+    def step(xs: torch.Tensor, ys: torch.Tensor) -> torch.Tensor:
+        opt.zero_grad(set_to_none=False)
+        logits = M.lm_forward(params, xs, cfg, compute_dtype=compute_dtype)
+        loss = F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), ys.reshape(-1))
+        loss.backward()
+        return finish(loss)
+
     step.optimizer = opt
     step.params = plist
     return step
+
+
+def make_distill_step(cfg: M.LMConfig, params: M.LMParams, temperature: float = 1.0, hard_weight: float = 0.0,
+                      lr: float = 1e-3, betas=(0.9, 0.95), eps: float = 1e-8, weight_decay: float = 0.0,
+                      clip: Optional[float] = 1.0, compute_dtype=torch.bfloat16, distributed: Optional[bool] = None):
+    """Build ``step(xs, teacher_ids, teacher_logits, ys=None, weights=None) -> loss``: `make_step`
+    with `distill.distill_loss` in place of the cross entropy.  ``teacher_ids`` and
+    ``teacher_logits (B, L, k)`` are a teacher's top alternatives for the token after each of
+    ``xs (B, L)`` (`score`'s ``top_ids`` and ``top_logprob``); ``ys`` are the hard labels that go
+    with ``hard_weight > 0``, ``weights (B, L)`` the positions' weights.  Tokens < 0 are padding.
+
+    The lookup and its gradient are `embedding.embed_tokens`; the loss and the gradient of the
+    logits come from one kernel that overwrites the logits with their gradient.  Weights are
+    normalised within a rank's shard, whose means are then averaged."""
+    opt, plist, finish = _optimizer(params, lr, betas, eps, weight_decay, clip, distributed)
+
+    def step(xs: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+             ys: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+        opt.zero_grad(set_to_none=False)
+        x = E.embed_tokens(params.embed, xs, dtype=compute_dtype)
+        logits = M.lm_forward(params, xs, cfg, embeds=x)
+        d = logits.detach()
+        loss, dlogits = D.distill_loss_and_grad(d, teacher_ids, teacher_logits, temperature=temperature, labels=ys,
+                                                hard_weight=hard_weight, weights=weights, out=d)
+        logits.backward(dlogits)
+        return finish(loss)
+
+    step.optimizer = opt
+    step.params = plist
+    return step
+
+
+@torch.no_grad()
+def score(params: M.LMParams, cfg: M.LMConfig, xs: torch.Tensor, ys: Optional[torch.Tensor] = None, top: int = 0,
+          temperature: float = 1.0, compute_dtype=None) -> S.TokenLogprobs:
+    """How likely the model finds ``ys (B, L)`` after ``xs (B, L)`` (L a multiple of the chunk):
+    `scoring.token_logprobs` of its logits, with the ``top`` alternatives of every position.
+    ``ys`` are the next tokens (< 0: none); without them only entropy and alternatives."""
+    x = E.embed_tokens(params.embed, xs, dtype=compute_dtype)
+    return S.token_logprobs(M.lm_forward(params, xs, cfg, embeds=x), ys, top=top, temperature=temperature)
 
 
 def _seed_from(key, device) -> int:
