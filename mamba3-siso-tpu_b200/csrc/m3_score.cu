@@ -1,7 +1,14 @@
 // Log probabilities of given tokens, entropy and top alternatives of logits rows.
 //   y = x / T, m = max y, Z = sum e^(y - m):  lse = m + ln Z,  entropy = ln Z - sum e d / Z, d = y - m
-// One CTA per row: a pass for the maximum, one for the sums, then one pass per alternative (the
-// largest entry below the previous one in the order (logit, lower index)).
+// One read of the logits: a row (or a cluster's share of it) stays in registers as 16-byte
+// vectors.  Each warp sums against its own maximum, so that the (max, sum, sum e d) triples of
+// all warps meet at one barrier, through distributed shared memory where a row has several CTAs.
+//
+// Alternatives: every warp gives the r-th largest of its lanes' maxima, r = ceil(top / warps); the
+// smallest of these has at least `top` lane maxima at or above it, so every alternative is at or
+// above it as well.  Only vectors that reach this bound are looked into (about twice `top` on
+// rows without order), the candidates are ranked by counting, and the CTAs' sorted lists are merged.
+// Rows that defeat the bound (many equal logits, NaN) take an exact selection by bits.
 #include "m3_internal.h"
 #include "m3_vocab.cuh"
 
@@ -10,11 +17,13 @@ namespace {
 
 using namespace vocab;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kNV = 8;          // vectors a thread holds
+constexpr int kMaxCluster = 8;  // CTAs per row (portable size)
+constexpr int kVecCap = 256, kCandCap = 1024;
 
 struct Params {
   int64_t rows;
-  int vocab, top;
+  int vocab, top, cluster;
   float inv_t;
   Rows lrow, trow;
   const void* logits;
@@ -23,64 +32,455 @@ struct Params {
   int64_t* top_ids;
 };
 
-template <typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, F f, V* sm) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sm[0];
-  for (int w = 1; w < kWarps; ++w) v = f(v, sm[w]);
-  return v;
-}
+// Sums against a maximum, in log2 units: s = sum 2^d, u = sum 2^d d, d = (x - m) log2(e) / T.
+struct Part {
+  float m, s, u;
+};
+
+__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) score_kernel(const Params p) {
-  __shared__ float fs[kWarps];
-  __shared__ uint64_t ws[kWarps];
-  const int64_t row = blockIdx.x;
-  const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
+__device__ __forceinline__ void add_vec(const uint4& v, float m, float c, float2& s, float2& u) {
+  float2 f[kVec<T> / 2];
+  unpack<T>(v, f);
+#pragma unroll
+  for (int j = 0; j < kVec<T> / 2; ++j) {
+    const float2 d = mul2(add2(f[j], f2s(-m)), f2s(c));
+    const float2 e = f2(ex2(d.x), ex2(d.y));
+    s = add2(s, e);
+    u = fma2(e, f2(fmaxf(d.x, -1e4f), fmaxf(d.y, -1e4f)), u);  // 2^d is 0 there: 0 * -inf is 0
+  }
+}
+
+// Joins the parts held by the lanes of a warp (lanes without one: m = -inf, s = u = 0).
+__device__ __forceinline__ Part join(Part p, float c) {
+  const float m = warp_max(p.m);
+  // a warp of masked entries may lie further below than fp32 reaches: 2^d is 0, s d has to stay finite
+  const float d = fmaxf((p.m - m) * c, -1e4f);
+  const float e = p.m == -INFINITY ? 0.f : ex2(d);
+  Part r;
+  r.m = m;
+  r.s = warp_sum(p.s * e);
+  r.u = warp_sum((p.u + p.s * d) * e);
+  // a part with NaN has s = NaN under any maximum
+  return r;
+}
+
+struct Row {
+  float m, ln_z, inv_t;
+  __device__ __forceinline__ float logprob(float x) const { return (x - m) * inv_t - ln_z; }
+};
+
+__device__ __forceinline__ Row finish(const Params& p, const Part& r, int64_t row, bool write) {
+  const float l2 = r.m == -INFINITY ? NAN : log2f(r.s);
+  Row w{r.m, l2 * kLn2, p.inv_t};
+  if (write) {
+    p.lse[row] = fmaf(r.m, p.inv_t, w.ln_z);
+    p.entropy[row] = (l2 - r.u / r.s) * kLn2;
+  }
+  return w;
+}
+
+__device__ __forceinline__ void write_target(const Params& p, const Row& w, int64_t row, int64_t t, float xt) {
+  p.logprob[row] = t < 0 ? 0.f : t >= p.vocab ? NAN : w.logprob(xt);
+}
+
+// ---- one CTA or one cluster per row -------------------------------------------------------
+template <int NW, bool TOP>
+struct Smem {
+  Part part[NW];
+  Part parts[kMaxCluster];
+};
+template <int NW>
+struct Smem<NW, true> {
+  Part part[NW];
+  Part parts[kMaxCluster];
+  float bound[NW];
+  int n_vec, n_cand;
+  int vec_at[kVecCap];
+  uint4 vec[kVecCap];
+  uint64_t cand[kCandCap];
+  uint64_t list[kMaxCluster][M3_MAX_TOP];  // every CTA's alternatives, descending, 0 past the end
+  int before[M3_MAX_TOP];                  // entries of the row above this CTA's i-th
+  int count[NW];
+};
+
+// The `need` first of the entries [lo, hi) in the order of rank_word, unsorted, by selection on the
+// bits of the key and then of the index.  All threads of the CTA.
+template <typename T, int TB, typename S>
+__device__ __noinline__ void exact_top(const T* x, int lo, int hi, int need, S& s) {
+  constexpr int NW = TB / 32;
+  const int tid = threadIdx.x;
+  auto count = [&](auto pred) {
+    int n = 0;
+    for (int i = lo + tid; i < hi; i += TB) n += pred(key_of(ld(x + i)), i) ? 1 : 0;
+    n = __reduce_add_sync(0xffffffffu, n);
+    __syncthreads();
+    if ((tid & 31) == 0) s.count[tid >> 5] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < NW; ++w) n += s.count[w];
+    return n;
+  };
+  uint32_t key = 0;  // the need-th largest key
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t t = key | (1u << b);
+    if (count([&](uint32_t k, int) { return k >= t; }) >= need) key = t;
+  }
+  const int ties = need - count([&](uint32_t k, int) { return k > key; });
+  int last = 0;  // the index of the last tie taken
+  for (int b = 31 - __clz(hi); b >= 0; --b) {
+    const int t = last | (1 << b);
+    if (count([&](uint32_t k, int i) { return k == key && i < t; }) < ties) last = t;
+  }
+  if (tid == 0) s.n_cand = 0;
+  __syncthreads();
+  for (int i = lo + tid; i < hi; i += TB) {
+    const float v = ld(x + i);
+    const uint32_t k = key_of(v);
+    if (k > key || (k == key && i <= last)) s.cand[atomicAdd(&s.n_cand, 1)] = rank_word(v, i);
+  }
+  __syncthreads();
+}
+
+template <typename T, int TB, bool RES, bool TOP>
+__global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
+  constexpr int E = kVec<T>, NW = TB / 32;
+  __shared__ Smem<NW, TOP> s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int cl = p.cluster, rank = cl > 1 ? cluster_rank() : 0;
+  const int64_t row = blockIdx.x / cl;
   const int V = p.vocab;
-  auto sum = [](float a, float b) { return a + b; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < V; i += kThreads) m = fmaxf(m, ld(x + i));
-  m = block_reduce(m, [](float a, float b) { return fmaxf(a, b); }, fs);
-  // log2 units; a row without a finite maximum makes every term NaN
+  const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
+  const int shift = row_shift(x), nvec = (shift + V + E - 1) / E, per = (nvec + cl - 1) / cl;
+  const int v0 = rank * per, v1 = min(nvec, v0 + per);
   const float c = p.inv_t * kLog2e;
-  float s = 0.f, u = 0.f;
-  for (int i = threadIdx.x; i < V; i += kThreads) {
-    const float d = (ld(x + i) - m) * c;
-    const float e = ex2(d);
-    s += e;
-    u = fmaf(e, fmaxf(d, -1e4f), u);  // e = 0 below -150: 0 * -inf is 0
+  if (cl > 1) cluster_arrive();  // peers have started before anyone writes to their shared memory
+
+  uint4 d[kNV];
+  Part a{-INFINITY, 0.f, 0.f};
+  float mine = -INFINITY;  // this lane's maximum
+  auto load = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < kNV; ++j) {
+      const int q = base + j * TB + tid;
+      d[j] = q < v1 ? load_vec(x, q * E - shift, V) : neg_inf_vec<T>();
+    }
+  };
+  for (int base = v0; base < v1; base += kNV * TB) {
+    load(base);
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+      if (base + j * TB < v1) m = fmaxf(m, vec_max<T>(d[j]));
+    mine = fmaxf(mine, m);
+    m = fmaxf(a.m, warp_max(m));
+    const float ref = finite_or_0(m);
+    float2 s2 = f2s(0.f), u2 = f2s(0.f);
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+      if (base + j * TB < v1) add_vec<T>(d[j], ref, c, s2, u2);
+    if (!RES && a.m != -INFINITY) {  // what came before, against the new maximum
+      const float dm = fmaxf((a.m - m) * c, -1e4f), e = ex2(dm);
+      s2.x += a.s * e;
+      u2.x += (a.u + a.s * dm) * e;
+    }
+    a = Part{m, s2.x + s2.y, u2.x + u2.y};
+    if (RES) break;
   }
-  s = block_reduce(s, sum, fs);
-  u = block_reduce(u, sum, fs);
-  const float l2 = log2f(s);
-  const float lse = m * p.inv_t + l2 * kLn2;
-  if (threadIdx.x == 0) {
-    p.lse[row] = lse;
-    p.entropy[row] = (l2 - u / s) * kLn2;
-    if (p.targets) {
-      const int64_t t = p.targets[p.trow.at(row)];
-      p.logprob[row] = t < 0 ? 0.f : t >= V ? NAN : (ld(x + t) - m) * p.inv_t - l2 * kLn2;
+  int64_t t = -1;
+  float xt = 0.f;
+  if (p.targets && rank == 0 && tid == 0) {
+    t = p.targets[p.trow.at(row)];
+    if (t >= 0 && t < V) xt = ld(x + t);
+  }
+  a.s = warp_sum(a.s);
+  a.u = warp_sum(a.u);
+  if (lane == 0) s.part[warp] = a;
+  if constexpr (TOP) {
+    const int r = (p.top + NW - 1) / NW;
+    float v = mine, bound = -INFINITY;
+    for (int i = 0; i < r; ++i) {
+      bound = warp_max(v);
+      const unsigned at = __ballot_sync(0xffffffffu, v == bound);
+      if (lane == __ffs(at) - 1) v = -INFINITY;
+    }
+    if (lane == 0) s.bound[warp] = bound;
+    if (tid == 0) s.n_vec = s.n_cand = 0;
+  }
+  __syncthreads();
+  a = join(lane < NW ? s.part[lane] : Part{-INFINITY, 0.f, 0.f}, c);
+
+  if constexpr (TOP) {
+    const int k = p.top, lo = max(0, v0 * E - shift), hi = min(V, v1 * E - shift);
+    float bound = lane < NW ? s.bound[lane] : INFINITY;
+    bound = -warp_max(-bound);
+    auto scan = [&](int base) {
+#pragma unroll
+      for (int j = 0; j < kNV; ++j)
+        if (base + j * TB < v1 && vec_max<T>(d[j]) >= bound) {
+          const int at = atomicAdd(&s.n_vec, 1);
+          if (at < kVecCap) {
+            s.vec[at] = d[j];
+            s.vec_at[at] = base + j * TB + tid;
+          }
+        }
+    };
+    if (RES) {
+      scan(v0);
+    } else {
+      for (int base = v0; base < v1; base += kNV * TB) {
+        load(base);
+        scan(base);
+      }
+    }
+    __syncthreads();
+    const int nv = s.n_vec;
+    if (nv <= kVecCap)
+      for (int i = tid; i < nv * E; i += TB) {
+        const float xv = ld(reinterpret_cast<const T*>(s.vec) + i);
+        const int idx = s.vec_at[i / E] * E - shift + i % E;
+        if (xv >= bound && idx >= 0 && idx < V) {
+          const int at = atomicAdd(&s.n_cand, 1);
+          if (at < kCandCap) s.cand[at] = rank_word(xv, idx);
+        }
+      }
+    __syncthreads();
+    // the sum is NaN iff the share holds NaN or +inf, which the comparisons above do not order
+    if (nv > kVecCap || s.n_cand > kCandCap || a.s != a.s) exact_top<T, TB>(x, lo, hi, min(k, hi - lo), s);
+    const int n = s.n_cand;
+    uint64_t* list = s.list[rank];
+    for (int i = tid; i < n; i += TB) {
+      const uint64_t w = s.cand[i];
+      int above = 0;
+      for (int j = 0; j < n; ++j) above += s.cand[j] > w ? 1 : 0;
+      if (above < k) list[above] = w;
+    }
+    for (int i = max(n, 0) + tid; i < k; i += TB) list[i] = 0;
+    for (int i = tid; i < k; i += TB) s.before[i] = i;
+    __syncthreads();
+  }
+
+  if (cl > 1) {
+    __syncwarp();
+    cluster_wait();
+    if (tid < cl) *peer(&s.parts[rank], tid) = a;
+    if constexpr (TOP)
+      for (int i = tid; i < p.top * cl; i += TB) {
+        const int r = i / p.top, j = i - r * p.top;
+        if (r != rank) *peer(&s.list[rank][j], r) = s.list[rank][j];
+      }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    a = join(lane < cl ? s.parts[lane] : Part{-INFINITY, 0.f, 0.f}, c);
+  }
+  const Row w = finish(p, a, row, rank == 0 && tid == 0);
+  if (p.targets && rank == 0 && tid == 0) write_target(p, w, row, t, xt);
+
+  if constexpr (TOP) {
+    const int k = p.top;
+    if (cl > 1) {  // entries of the other lists above each of this one's
+      for (int i = tid; i < k * cl; i += TB) {
+        const int r = i / k, j = i - r * k;
+        const uint64_t e = s.list[rank][j];
+        if (r == rank || e == 0) continue;
+        int lo = 0, hi = k;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (s.list[r][mid] > e)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        atomicAdd(&s.before[j], lo);
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < k; i += TB) {
+      const uint64_t e = s.list[rank][i];
+      const int at = s.before[i];
+      if (e != 0 && at < k) {
+        p.top_ids[row * k + at] = rank_index(e);
+        p.top_logprob[row * k + at] = w.logprob(key_value((uint32_t)(e >> 32)));
+      }
     }
   }
-  uint64_t prev = ~0ull;
-  for (int j = 0; j < p.top; ++j) {
-    uint64_t best = 0;
-    for (int i = threadIdx.x; i < V; i += kThreads) {
-      const uint64_t w = rank_word(ld(x + i), i);
-      if ((w < prev || j == 0) && w > best) best = w;  // (NaN, 0) has the top word
-    }
-    best = block_reduce(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; }, ws);
-    if (threadIdx.x == 0) {
-      p.top_ids[row * p.top + j] = rank_index(best);
-      p.top_logprob[row * p.top + j] = (key_value((uint32_t)(best >> 32)) - m) * p.inv_t - l2 * kLn2;
-    }
-    prev = best;
+}
+
+// ---- one warp per row ---------------------------------------------------------------------
+// The (logit, lower index) order as one word: 32 bits for bf16 rows of at most 512 entries.
+template <typename T>
+struct Word;
+template <>
+struct Word<__nv_bfloat16> {
+  using type = uint32_t;
+  static __device__ __forceinline__ type make(float x, int i) { return (key_of(x) & 0xFFFF0000u) | (0xFFFFu - i); }
+  static __device__ __forceinline__ float value(type w) { return key_value(w >= 0xFFFF0000u ? ~0u : (w & 0x80000000u) ? w & 0xFFFF0000u : w | 0xFFFFu); }
+  static __device__ __forceinline__ int index(type w) { return 0xFFFF - (int)(w & 0xFFFFu); }
+  static __device__ __forceinline__ type max(type w) { return __reduce_max_sync(0xffffffffu, w); }
+};
+template <>
+struct Word<float> {
+  using type = uint64_t;
+  static __device__ __forceinline__ type make(float x, int i) { return rank_word(x, i); }
+  static __device__ __forceinline__ float value(type w) { return key_value((uint32_t)(w >> 32)); }
+  static __device__ __forceinline__ int index(type w) { return rank_index(w); }
+  static __device__ __forceinline__ type max(type w) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(w >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(w >> 32) == hi ? (uint32_t)w : 0u);
+    return ((uint64_t)hi << 32) | lo;
   }
+};
+
+// Descending, by Batcher's odd-even merge exchange (Knuth, TAOCP vol. 3, 5.2.2, algorithm M).
+template <int N, typename W>
+__device__ __forceinline__ void sort_desc(W (&w)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const W a = w[i + j], b = w[i + j + k];
+            w[i + j] = a > b ? a : b;
+            w[i + j + k] = a > b ? b : a;
+          }
+}
+
+constexpr int kWarpThreads = 256, kWarpRows = kWarpThreads / 32;
+
+template <typename T, int NV, bool TOP>
+__global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p) {
+  constexpr int E = kVec<T>;
+  const int lane = threadIdx.x & 31, V = p.vocab;
+  const int64_t step = (int64_t)gridDim.x * kWarpRows;
+  const float c = p.inv_t * kLog2e;
+  int64_t row = (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5);
+  const T* x = nullptr;
+  uint4 d[NV];
+  auto load = [&](int64_t r) {
+    x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(r);
+    const int shift = row_shift(x);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int lo = (j * 32 + lane) * E - shift;
+      d[j] = lo < V ? load_vec(x, lo, V) : neg_inf_vec<T>();
+    }
+  };
+  if (row < p.rows) load(row);
+  while (row < p.rows) {
+    const T* xr = x;
+    const int shift = row_shift(xr);
+    int64_t t = -1;
+    if (p.targets && lane == 0) t = p.targets[p.trow.at(row)];
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) m = fmaxf(m, vec_max<T>(d[j]));
+    m = warp_max(m);
+    const float ref = finite_or_0(m);
+    float2 s2 = f2s(0.f), u2 = f2s(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) add_vec<T>(d[j], ref, c, s2, u2);
+    typename Word<T>::type wd[TOP ? NV * E : 1];
+    if constexpr (TOP) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float2 f[E / 2];
+        unpack<T>(d[j], f);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const int idx = (j * 32 + lane) * E - shift + i;
+          wd[j * E + i] = idx >= 0 && idx < V ? Word<T>::make(i & 1 ? f[i / 2].y : f[i / 2].x, idx) : 0;
+        }
+      }
+    }
+    const int64_t next = row + step;
+    if (next < p.rows) load(next);  // on its way while this row is finished
+    float xt = 0.f;
+    if (t >= 0 && t < V) xt = ld(xr + t);
+    const Part a{m, warp_sum(s2.x + s2.y), warp_sum(u2.x + u2.y)};
+    const Row w = finish(p, a, row, lane == 0);
+    if (p.targets && lane == 0) write_target(p, w, row, t, xt);
+    if constexpr (TOP) {
+      sort_desc(wd);
+      typename Word<T>::type keep = 0;
+      for (int j = 0; j < p.top; ++j) {
+        const auto best = Word<T>::max(wd[0]);
+        if (wd[0] == best) {
+#pragma unroll
+          for (int i = 0; i + 1 < NV * E; ++i) wd[i] = wd[i + 1];
+          wd[NV * E - 1] = 0;
+        }
+        if (lane == (j & 31)) keep = best;
+        if ((j & 31) == 31 || j == p.top - 1) {
+          const int i = (j & ~31) + lane;
+          if (i <= j) {
+            p.top_ids[row * p.top + i] = Word<T>::index(keep);
+            p.top_logprob[row * p.top + i] = w.logprob(Word<T>::value(keep));
+          }
+        }
+      }
+    }
+    row = next;
+  }
+}
+
+int sm_count() {
+  int dev = 0, c = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
+  return c;
+}
+
+template <typename T, int TB, bool RES, bool TOP>
+int launch_cta(const Params& p, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.rows * p.cluster), 1, 1);
+  cfg.blockDim = dim3(TB, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = p.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, score_kernel<T, TB, RES, TOP>, p);
+  return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_token_logprobs: ") + cudaGetErrorString(e));
+}
+
+template <typename T, int NV, bool TOP>
+int launch_warp(const Params& p, cudaStream_t s) {
+  const int64_t want = (p.rows + kWarpRows - 1) / kWarpRows, most = (int64_t)sm_count() * 8;
+  score_warp_kernel<T, NV, TOP><<<(unsigned)(want < most ? want : most), kWarpThreads, 0, s>>>(p);
+  return check_launch("m3_token_logprobs");
+}
+
+// A row goes to a warp while its vectors fit the lanes' registers (with alternatives: while a lane
+// can keep its 8 or 16 entries sorted), else to the fewest threads that hold it, else to a cluster.
+template <typename T, bool TOP>
+int launch(Params p, int nvec, cudaStream_t s) {
+  if (nvec <= 32) return launch_warp<T, 1, TOP>(p, s);
+  if (nvec <= 64) return launch_warp<T, 2, TOP>(p, s);
+  if constexpr (!TOP) {
+    if (nvec <= 128) return launch_warp<T, 4, TOP>(p, s);
+    if (nvec <= 256) return launch_warp<T, 8, TOP>(p, s);
+  }
+  int cl = 1;
+  while (cl < kMaxCluster && (nvec > cl * kNV * 512)) cl *= 2;
+  // few rows: more CTAs per row until they cover the SMs
+  const int sms = sm_count();
+  while (cl < kMaxCluster && p.rows * cl * 2 <= sms && nvec / (cl * 2) >= 128) cl *= 2;
+  p.cluster = cl;
+  if (p.rows * cl > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_token_logprobs: too many rows");
+  const int per = (nvec + cl - 1) / cl;
+  if (per > kNV * 512) return launch_cta<T, 512, false, TOP>(p, s);
+  if (per > kNV * 256 || p.rows * cl < sms) return launch_cta<T, 512, true, TOP>(p, s);
+  if (per > kNV * 128) return launch_cta<T, 256, true, TOP>(p, s);
+  return launch_cta<T, 128, true, TOP>(p, s);
 }
 
 }  // namespace
@@ -91,8 +491,9 @@ using namespace m3;
 extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
   if (!args) return set_error(M3_ERR_ARG, "m3_token_logprobs: args is NULL");
   const M3ScoreArgs& a = *args;
-  if (a.rows_outer < 0 || a.rows_inner < 0 || a.vocab <= 0 || a.top < 0 || a.top > M3_MAX_TOP || a.top > a.vocab)
-    return set_error(M3_ERR_SHAPE, "m3_token_logprobs: need rows >= 0, vocab > 0 and 0 <= top <= min(vocab, 128)");
+  if (a.rows_outer < 0 || a.rows_inner < 0 || a.vocab <= 0 || a.vocab > kMaxVocab || a.top < 0 ||
+      a.top > M3_MAX_TOP || a.top > a.vocab)
+    return set_error(M3_ERR_SHAPE, "m3_token_logprobs: need rows >= 0, 0 < vocab <= 2^30 and 0 <= top <= min(vocab, 128)");
   if (a.logits_dtype != M3_DTYPE_F32 && a.logits_dtype != M3_DTYPE_BF16)
     return set_error(M3_ERR_UNSUPPORTED, "m3_token_logprobs: logits must be f32 or bf16");
   if (!(a.temperature > 0.f)) return set_error(M3_ERR_ARG, "m3_token_logprobs: temperature must be > 0");
@@ -100,11 +501,13 @@ extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
   if (rows == 0) return M3_OK;
   if (!a.logits || !a.entropy || !a.lse || (a.targets && !a.logprob) || (a.top > 0 && (!a.top_logprob || !a.top_ids)))
     return set_error(M3_ERR_ARG, "m3_token_logprobs: NULL pointer");
-  if (rows > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_token_logprobs: more than 2^31 - 1 rows");
+  const bool bf = a.logits_dtype == M3_DTYPE_BF16;
+  if (((uintptr_t)a.logits) % (bf ? 2 : 4)) return set_error(M3_ERR_ARG, "m3_token_logprobs: logits are not aligned to their type");
   Params p;
   p.rows = rows;
   p.vocab = a.vocab;
   p.top = a.top;
+  p.cluster = 1;
   p.inv_t = 1.f / a.temperature;
   p.lrow = Rows{a.rows_inner, a.ld_outer, a.ld_inner};
   p.trow = Rows{a.rows_inner, a.t_outer, a.t_inner};
@@ -116,9 +519,7 @@ extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
   p.top_logprob = a.top_logprob;
   p.top_ids = a.top_ids;
   cudaStream_t s = (cudaStream_t)stream;
-  if (a.logits_dtype == M3_DTYPE_BF16)
-    score_kernel<__nv_bfloat16><<<(unsigned)rows, kThreads, 0, s>>>(p);
-  else
-    score_kernel<float><<<(unsigned)rows, kThreads, 0, s>>>(p);
-  return check_launch("m3_token_logprobs");
+  const int nvec = most_vectors(a.logits, a.vocab, bf ? 2 : 4, a.ld_outer, a.ld_inner);
+  if (bf) return a.top ? launch<__nv_bfloat16, true>(p, nvec, s) : launch<__nv_bfloat16, false>(p, nvec, s);
+  return a.top ? launch<float, true>(p, nvec, s) : launch<float, false>(p, nvec, s);
 }
