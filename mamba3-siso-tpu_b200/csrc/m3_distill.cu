@@ -2,10 +2,10 @@
 //   q = softmax(x / T), p = softmax(teacher / T) over the k given entries
 //   KL = sum_j p_j (ln p_j - ln q_{id_j}),   d(T^2 KL)/dx = T (q - p)
 // and with hard labels CE = lse(x) - x_label, dCE/dx = softmax(x) - onehot.
-// One read of the logits and one write of their gradient: a row (or a cluster's share of it) stays
-// in registers as 16-byte vectors between the sums and the gradient.  Each warp sums against its
-// own maximum; the parts of all warps (and CTAs, through distributed shared memory) meet at one
-// barrier.  One warp holds the teacher's entries, four to a lane.  The dense gradient k_s q is stored
+// One read of the logits from memory and one write of their gradient.  Each warp walks its share of a
+// row with a running maximum and sums against it; the parts of the row's warps meet at one barrier;
+// then the row is walked again, from L2 (so that the rows in flight have to fit there), and its
+// gradient written.  One warp holds the teacher's entries, four to a lane.  The dense gradient k_s q is stored
 // first; then each entry's place is stored again as k_s q - p, from the same fp32 values, so that
 // every element is rounded once.
 #include "m3_internal.h"
@@ -16,13 +16,12 @@ namespace {
 
 using namespace vocab;
 
-constexpr int kNV = 8;          // vectors a thread holds
+constexpr int kNV = 8;          // vectors a thread loads at a time
 constexpr int kMaxCluster = 8;  // CTAs per row (portable size)
 constexpr int kEnt = M3_MAX_TOP / 32;  // entries a lane holds
 
 struct Params {
-  int64_t rows;
-  int vocab, k, cluster;
+  int rows, vocab, k, cluster, log2_cluster;
   float temperature, inv_t, hard, scale;  // scale: grad_scale, over the row count for an unweighted mean
   Rows lrow, grow;
   const void* logits;
@@ -77,7 +76,7 @@ enum { kSoft = 1, kHard = 2, kBad = 4 };  // a row's terms; kBad: an id or label
 
 // `ids` are loaded as they are, absent and bad ones become -1.
 template <bool HARD>
-__device__ __forceinline__ int load_entries(const Params& p, int64_t row, float w, int64_t label, Entries& en) {
+__device__ __forceinline__ int load_entries(const Params& p, int row, float w, int64_t label, Entries& en) {
   const int lane = threadIdx.x & 31;
   bool any = false, bad = false;
 #pragma unroll
@@ -87,8 +86,8 @@ __device__ __forceinline__ int load_entries(const Params& p, int64_t row, float 
     if (32 * e < p.k) {
       const int j = lane + 32 * e;
       if (j < p.k) {
-        const int64_t id = p.ids[row * p.k + j];
-        const float t = p.teacher[row * p.k + j];
+        const int64_t id = p.ids[(int64_t)row * p.k + j];
+        const float t = p.teacher[(int64_t)row * p.k + j];
         bad |= id >= p.vocab;
         if (id >= 0 && id < p.vocab) {
           en.id[e] = (int)id;
@@ -170,7 +169,7 @@ struct Coef {
 };
 
 template <bool HARD>
-__device__ __forceinline__ Coef coefficients(const Params& p, const Part& a, int64_t row, int flags, float w) {
+__device__ __forceinline__ Coef coefficients(const Params& p, const Part& a, int row, int flags, float w) {
   float r = p.scale * w;
   if (p.weight_sum) r /= *p.weight_sum;
   if (p.upstream) r *= p.upstream[row * p.upstream_stride];
@@ -197,24 +196,20 @@ __device__ __forceinline__ uint4 grad_vec(const uint4& v, const Coef& k) {
     return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
 }
 
-// Elements [lo, lo + E) of a row; `vec`: that place is 16-byte aligned.
+// The E elements at g; `vec`: g is 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void store_vec(T* g, int lo, int n, const uint4& u, bool vec) {
-  constexpr int E = kVec<T>;
-  if (vec && lo >= 0 && lo + E <= n) {
-    *reinterpret_cast<uint4*>(g + lo) = u;
+__device__ __forceinline__ void store_vec(T* g, const uint4& u, bool vec, uint64_t policy) {
+  if (vec) {
+    store_stream(g, u, policy);
     return;
   }
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const int i = lo + j;
-    if (i >= 0 && i < n) {
-      if constexpr (sizeof(T) == 2)
-        *reinterpret_cast<uint16_t*>(g + i) = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
-      else
-        *reinterpret_cast<uint32_t*>(g + i) = w[j];
-    }
+  for (int j = 0; j < kVec<T>; ++j) {
+    if constexpr (sizeof(T) == 2)
+      reinterpret_cast<uint16_t*>(g)[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+    else
+      reinterpret_cast<uint32_t*>(g)[j] = w[j];
   }
 }
 
@@ -272,41 +267,33 @@ __device__ __forceinline__ void store_entries(const Params& p, T* g, int lo, int
 }
 
 // ---- one CTA or one cluster per row -------------------------------------------------------
-template <typename T, int TB, bool RES, bool GRAD>
+template <int TB, bool GRAD>
 struct Smem {
-  static constexpr int kSeen = GRAD && RES ? kNV * TB * kVec<T> / 32 : 1;
+  static constexpr int kSeen = GRAD ? 8 * TB : 4;  // a bit per element of a share of up to 256 TB
   Part part[TB / 32];
   Part parts[kMaxCluster];
   int flags;
   int ids[GRAD ? M3_MAX_TOP : 1];
   float amounts[GRAD ? M3_MAX_TOP : 1];
-  uint32_t seen[kSeen];
+  alignas(16) uint32_t seen[kSeen];  // cleared as 16-byte vectors
 };
 
-template <typename T, int TB, bool RES, bool HARD, bool GRAD>
+template <typename T, int TB, bool HARD, bool GRAD>
 __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) {
   constexpr int E = kVec<T>, NW = TB / 32;
-  using S = Smem<T, TB, RES, GRAD>;
+  using S = Smem<TB, GRAD>;
   __shared__ S s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cl = p.cluster, rank = cl > 1 ? cluster_rank() : 0;
-  const int64_t row = blockIdx.x / cl;
+  const int row = (int)blockIdx.x >> p.log2_cluster;
   const int V = p.vocab;
   const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
-  const int shift = row_shift(x), nvec = (shift + V + E - 1) / E, per = (nvec + cl - 1) / cl;
-  const int v0 = rank * per, v1 = min(nvec, v0 + per);
+  const Split sp = split_row(x, V);
+  const int per = (sp.full + cl - 1) >> p.log2_cluster, v0 = min(sp.full, rank * per), n = min(per, sp.full - v0);
+  const uint4* v = reinterpret_cast<const uint4*>(x + sp.head) + v0;
   const float c = p.inv_t * kLog2e;
-  if (cl > 1) cluster_arrive();  // peers have started before anyone writes to their shared memory
+  if (cl > 1) cluster_arrive_relaxed();  // peers have started before anyone writes to their shared memory
 
-  uint4 d[kNV];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int j = 0; j < kNV; ++j) {
-      const int q = base + j * TB + tid;
-      d[j] = q < v1 ? load_vec(x, q * E - shift, V) : neg_inf_vec<T>();
-    }
-  };
-  if (RES) load(v0);
   const float w = p.weights ? p.weights[row] : 1.f;
   const int64_t label = HARD ? p.labels[row] : -1;
   Entries en;
@@ -315,38 +302,47 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   if (warp == 0) {
     const int f = load_entries<HARD>(p, row, w, label, en);
     if (lane == 0) s.flags = f;
-    // read here: below, the gradient may overwrite the logits
-    if (holder) {
+    if (holder) {  // read here: below, the gradient may overwrite the logits
 #pragma unroll
       for (int e = 0; e < kEnt; ++e) en.x[e] = 32 * e < p.k && en.id[e] >= 0 ? ld(x + en.id[e]) : 0.f;
       if (HARD && label >= 0 && label < V) xl = ld(x + label);
     }
   }
-  if constexpr (GRAD && RES)
-    for (int i = tid; i < S::kSeen; i += TB) s.seen[i] = 0u;
+  if constexpr (GRAD)
+    for (int i = tid; i < S::kSeen / 4; i += TB) reinterpret_cast<uint4*>(s.seen)[i] = make_uint4(0u, 0u, 0u, 0u);
 
-  Part a{-INFINITY, 0.f, 0.f};
-  for (int base = v0; base < v1; base += kNV * TB) {
-    if (!RES) load(base);
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kNV; ++j)
-      if (base + j * TB < v1) m = fmaxf(m, vec_max<T>(d[j]));
-    m = fmaxf(a.m, warp_max(m));
-    const float ref = finite_or_0(m);
-    float2 s2 = f2s(0.f), t2 = f2s(0.f);
-#pragma unroll
-    for (int j = 0; j < kNV; ++j)
-      if (base + j * TB < v1) add_vec<T, HARD>(d[j], ref, c, s2, t2);
-    if (!RES && a.m != -INFINITY) {  // what came before, against the new maximum
-      s2.x += a.s * ex2((a.m - m) * c);
-      if (HARD) t2.x += a.s1 * ex2((a.m - m) * kLog2e);
+  float m = -INFINITY;  // the warp's maximum
+  float2 s2 = f2s(0.f), t2 = f2s(0.f);
+  auto raise = [&](float to) {  // the sums against a new maximum
+    if (to > m) {
+      if (m != -INFINITY) {
+        s2 = mul2(s2, f2s(ex2((m - to) * c)));
+        if (HARD) t2 = mul2(t2, f2s(ex2((m - to) * kLog2e)));
+      }
+      m = to;
     }
-    a = Part{m, s2.x + s2.y, t2.x + t2.y};
-    if (RES) break;
+  };
+  walk<T, kNV, TB>(v, n, tid, GRAD ? Keep::kYes : Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
+    float mt = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+      if (full.value || base + j * TB < n) mt = fmaxf(mt, vec_max<T>(d[j]));
+    raise(warp_max(mt));
+    const float ref = finite_or_0(m);
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+      if (full.value || base + j * TB < n) add_vec<T, HARD>(d[j], ref, c, s2, t2);
+  });
+  int edge = -1;  // this lane's element of the row's edges
+  float xe = -INFINITY;
+  if (warp == NW - 1) {
+    edge = edge_index(sp, lane, rank == 0, rank == cl - 1);
+    if (edge >= 0) xe = ld(x + edge);
+    raise(warp_max(xe));
+    s2.x += ex2((xe - finite_or_0(m)) * c);
+    if (HARD) t2.x += ex2((xe - finite_or_0(m)) * kLog2e);
   }
-  a.s = warp_sum(a.s);
-  if (HARD) a.s1 = warp_sum(a.s1);
+  Part a{m, warp_sum(s2.x + s2.y), HARD ? warp_sum(t2.x + t2.y) : 0.f};
   if (lane == 0) s.part[warp] = a;
   if (holder) teacher_softmax(p, en, pr, lp);
   __syncthreads();
@@ -368,24 +364,31 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   }
   if constexpr (GRAD) {
     T* g = reinterpret_cast<T*>(p.grad) + p.grow.at(row);
-    const bool vec = row_shift(g) == shift;
+    T* gv = g + sp.head + v0 * E;  // this share's vectors, aligned or not
+    const bool vec = row_shift(gv) == 0;
     const Coef k = coefficients<HARD>(p, a, row, flags, w);
-    for (int base = v0; base < v1; base += kNV * TB) {
-      if (!RES) load(base);
+    const uint64_t first = l2_policy(Keep::kNo);
+    if (flags) {
+      walk<T, kNV, TB>(v, n, tid, Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
 #pragma unroll
-      for (int j = 0; j < kNV; ++j) {
-        const int q = base + j * TB + tid;
-        if (base + j * TB < v1) {
-          const uint4 u = flags ? grad_vec<T, HARD>(d[j], k) : make_uint4(0u, 0u, 0u, 0u);
-          if (q < v1) store_vec<T>(g, q * E - shift, V, u, vec);
+        for (int j = 0; j < kNV; ++j) {
+          const int q = base + j * TB + tid;
+          if (full.value || base + j * TB < n) {
+            const uint4 u = grad_vec<T, HARD>(d[j], k);
+            if (full.value || q < n) store_vec<T>(gv + (int64_t)q * E, u, vec, first);
+          }
         }
-      }
-      if (RES) break;
+      });
+    } else {
+      for (int q = tid; q < n; q += TB) store_vec<T>(gv + (int64_t)q * E, make_uint4(0u, 0u, 0u, 0u), vec, first);
     }
+    if (edge >= 0) stg<T>(g + edge, flags ? k.at<HARD>(f2s(xe)).x : 0.f);
     __syncthreads();
-    if (warp == 0 && flags && !(flags & kBad))
-      store_entries<T, HARD>(p, g, max(0, v0 * E - shift), min(V, v1 * E - shift), k, en, pr, label, xl,
-                             RES ? s.seen : nullptr, s.ids, s.amounts);
+    if (warp == 0 && flags && !(flags & kBad)) {
+      const int lo = rank == 0 ? 0 : sp.head + v0 * E, hi = rank == cl - 1 ? V : sp.head + (v0 + n) * E;
+      store_entries<T, HARD>(p, g, lo, hi, k, en, pr, label, xl, hi - lo <= 32 * S::kSeen ? s.seen : nullptr, s.ids,
+                             s.amounts);
+    }
   }
 }
 
@@ -400,12 +403,12 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
   __shared__ int ids_of[kWarpRows][GRAD ? M3_MAX_TOP : 1];
   __shared__ float amounts_of[kWarpRows][GRAD ? M3_MAX_TOP : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, V = p.vocab;
-  const int64_t step = (int64_t)gridDim.x * kWarpRows;
+  const int step = gridDim.x * kWarpRows;
   const float c = p.inv_t * kLog2e;
-  int64_t row = (int64_t)blockIdx.x * kWarpRows + warp;
+  int row = blockIdx.x * kWarpRows + warp;
   uint4 d[NV];
   int shift = 0;
-  auto load = [&](int64_t r) {
+  auto load = [&](int r) {
     const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(r);
     shift = row_shift(x);
 #pragma unroll
@@ -455,10 +458,18 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
     if constexpr (GRAD) {
       T* g = reinterpret_cast<T*>(p.grad) + p.grow.at(row);
       const bool vec = row_shift(g) == at;
+      const uint64_t first = l2_policy(Keep::kNo);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int lo = (j * 32 + lane) * E - at;
-        if (lo < V) store_vec<T>(g, lo, V, u[j], vec);
+        if (lo >= 0 && lo + E <= V) {
+          store_vec<T>(g + lo, u[j], vec, first);
+        } else if (lo < V) {
+          const T* e = reinterpret_cast<const T*>(&u[j]);
+#pragma unroll
+          for (int i = 0; i < E; ++i)
+            if (lo + i >= 0 && lo + i < V) g[lo + i] = e[i];
+        }
       }
       __syncwarp();
       if (flags && !(flags & kBad))
@@ -475,7 +486,7 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
     sum_kernel(const float* __restrict__ v, int64_t n, const float* div_by, float scale, float* out) {
   __shared__ float sm[32], total[kSumCtas];
   const int tid = threadIdx.x, rank = cluster_rank();
-  cluster_arrive();
+  cluster_arrive_relaxed();
   float s = 0.f;
 #pragma unroll 4
   for (int64_t i = (int64_t)rank * kSumThreads + tid; i < n; i += kSumCtas * kSumThreads) s += v[i];
@@ -502,10 +513,10 @@ int sm_count() {
   return c;
 }
 
-template <typename T, int TB, bool RES, bool HARD, bool GRAD>
+template <typename T, int TB, bool HARD, bool GRAD>
 int launch_cta(const Params& p, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.rows * p.cluster), 1, 1);
+  cfg.gridDim = dim3((unsigned)p.rows * p.cluster, 1, 1);
   cfg.blockDim = dim3(TB, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -514,37 +525,37 @@ int launch_cta(const Params& p, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_kernel<T, TB, RES, HARD, GRAD>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_kernel<T, TB, HARD, GRAD>, p);
   return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_distill: ") + cudaGetErrorString(e));
 }
 
 template <typename T, int NV, bool HARD, bool GRAD>
 int launch_warp(const Params& p, cudaStream_t s) {
-  const int64_t want = (p.rows + kWarpRows - 1) / kWarpRows, most = (int64_t)sm_count() * 8;
+  const int want = (p.rows + kWarpRows - 1) / kWarpRows, most = sm_count() * 8;
   distill_warp_kernel<T, NV, HARD, GRAD><<<(unsigned)(want < most ? want : most), kWarpThreads, 0, s>>>(p);
   return check_launch("m3_distill");
 }
 
-// A row goes to a warp while its vectors fit the lanes' registers, else to the fewest threads that
-// hold it, else to a cluster.
+// A row goes to a warp while its vectors fit the lanes' registers, else to a CTA, and with few rows to
+// a cluster.
 template <typename T, bool HARD, bool GRAD>
 int launch(Params p, int nvec, cudaStream_t s) {
   if (nvec <= 32) return launch_warp<T, 1, HARD, GRAD>(p, s);
   if (nvec <= 64) return launch_warp<T, 2, HARD, GRAD>(p, s);
   if (nvec <= 128) return launch_warp<T, 4, HARD, GRAD>(p, s);
   if (nvec <= 256) return launch_warp<T, 8, HARD, GRAD>(p, s);
-  int cl = 1;
-  while (cl < kMaxCluster && nvec > cl * kNV * 512) cl *= 2;
-  // few rows: more CTAs per row until they cover the SMs
+  // few rows: several CTAs per row until they cover the SMs
   const int sms = sm_count();
-  while (cl < kMaxCluster && p.rows * cl * 2 <= sms && nvec / (cl * 2) >= 128) cl *= 2;
+  int cl = 1;
+  while (cl < kMaxCluster && (int64_t)p.rows * cl * 2 <= sms && nvec / (cl * 2) >= 128) cl *= 2;
   p.cluster = cl;
-  if (p.rows * cl > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_distill: too many rows");
-  const int per = (nvec + cl - 1) / cl;
-  if (per > kNV * 512) return launch_cta<T, 512, false, HARD, GRAD>(p, s);
-  if (per > kNV * 256 || p.rows * cl < sms) return launch_cta<T, 512, true, HARD, GRAD>(p, s);
-  if (per > kNV * 128) return launch_cta<T, 256, true, HARD, GRAD>(p, s);
-  return launch_cta<T, 128, true, HARD, GRAD>(p, s);
+  while ((1 << p.log2_cluster) < cl) ++p.log2_cluster;
+  if ((int64_t)p.rows * cl > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_distill: too many rows");
+  // a second walk finds its row in L2 only while the rows in flight (1024 / threads per SM) fit there
+  if (nvec <= kNV * 128 * cl) return launch_cta<T, 128, HARD, GRAD>(p, s);
+  const bool fits = (int64_t)nvec * 16 * 4 * sms <= (int64_t)64 << 20;
+  return (GRAD && !fits) || (int64_t)p.rows * cl <= 2 * sms ? launch_cta<T, 512, HARD, GRAD>(p, s)
+                                                             : launch_cta<T, 256, HARD, GRAD>(p, s);
 }
 
 template <typename T>
@@ -570,7 +581,7 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
   if (!(a.temperature > 0.f) || !(a.hard_weight >= 0.f && a.hard_weight <= 1.f))
     return set_error(M3_ERR_ARG, "m3_distill: need temperature > 0 and 0 <= hard_weight <= 1");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
-  if (rows > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_distill: more than 2^31 - 1 rows");
+  if (rows > kMaxRows) return set_error(M3_ERR_SHAPE, "m3_distill: more than 2^30 rows");
   if ((rows > 0 && (!a.logits || !a.ids || !a.teacher || !a.row_loss)) ||
       (a.hard_weight > 0.f && rows > 0 && !a.labels) || (a.reduction != M3_REDUCE_NONE && !a.loss))
     return set_error(M3_ERR_ARG, "m3_distill: NULL pointer");
@@ -584,8 +595,9 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
     return set_error(M3_ERR_ARG, "m3_distill: logits and grad must be aligned to their type");
   cudaStream_t s = (cudaStream_t)stream;
   Params p;
-  p.rows = rows;
+  p.rows = (int)rows;
   p.cluster = 1;
+  p.log2_cluster = 0;
   p.vocab = a.vocab;
   p.k = a.k;
   p.temperature = a.temperature;

@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const FwdParams p) {
   for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
     const int64_t r = i / p.dim;
     const int c = (int)(i - r * p.dim);
-    const int64_t t = p.tokens[p.trow.at(r)];
+    const int64_t t = p.tokens[p.trow.at((int)r)];
     float v = t < 0 ? 0.f : NAN;
     if (t >= 0 && t < p.vocab) v = ld(reinterpret_cast<const T*>(p.table) + t * p.table_ld + c) * p.scale;
     stg<O>(reinterpret_cast<O*>(p.out) + r * p.out_ld + c, v);
@@ -84,7 +84,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
         e = __ldcg(src + i);
         return true;
       }
-      const int64_t t = p.tokens[p.trow.at(i)];
+      const int64_t t = p.tokens[p.trow.at((int)i)];
       e = make_uint2((uint32_t)t, (uint32_t)i);
       return t >= 0 && t < p.vocab;
     };
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const SumParams p) {
   G* g = reinterpret_cast<G*>(p.grad) + v * p.grad_ld;
   for (int c = threadIdx.x; c < p.dim; c += kThreads) {
     float s = 0.f;
-    for (int i = i0; i < i1; ++i) s += ld(reinterpret_cast<const D*>(p.dy) + p.drow.at(p.sorted[i].y) + c);
+    for (int i = i0; i < i1; ++i) s += ld(reinterpret_cast<const D*>(p.dy) + p.drow.at((int)p.sorted[i].y) + c);
     s *= p.scale;
     stg<G>(g + c, p.accumulate ? ld(g + c) + s : s);
   }
@@ -209,7 +209,7 @@ extern "C" int m3_embed(const M3EmbedArgs* args, void* stream) {
   if (!dtype_ok(a.table_dtype) || !dtype_ok(a.out_dtype))
     return set_error(M3_ERR_UNSUPPORTED, "m3_embed: table and out must be f32 or bf16");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
-  if (rows > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_embed: more than 2^31 - 1 rows");
+  if (rows > vocab::kMaxRows) return set_error(M3_ERR_SHAPE, "m3_embed: more than 2^30 rows");
   if (rows == 0) return M3_OK;
   if (!a.tokens || !a.table || !a.out) return set_error(M3_ERR_ARG, "m3_embed: NULL pointer");
   if (a.table_ld < a.dim || a.out_ld < a.dim) return set_error(M3_ERR_SHAPE, "m3_embed: bad leading dimension");
@@ -226,7 +226,7 @@ extern "C" int m3_embed(const M3EmbedArgs* args, void* stream) {
 }
 
 extern "C" size_t m3_embed_bwd_workspace_size(int64_t rows, int32_t dim) {
-  if (rows < 0 || rows > 0x7FFFFFFF || dim <= 0) return 0;
+  if (rows < 0 || rows > vocab::kMaxRows || dim <= 0) return 0;
   return 2 * align256((size_t)rows * sizeof(uint2)) + 256;
 }
 
@@ -238,7 +238,7 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   if (!dtype_ok(a.dy_dtype) || !dtype_ok(a.grad_dtype))
     return set_error(M3_ERR_UNSUPPORTED, "m3_embed_bwd: dy and grad must be f32 or bf16");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
-  if (rows > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: more than 2^31 - 1 rows");
+  if (rows > vocab::kMaxRows) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: more than 2^30 rows");
   if (!a.grad || (rows > 0 && (!a.tokens || !a.dy))) return set_error(M3_ERR_ARG, "m3_embed_bwd: NULL pointer");
   if (a.grad_ld < a.dim) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: bad leading dimension");
   const size_t need = m3_embed_bwd_workspace_size(rows, a.dim);
@@ -254,7 +254,7 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   sp.vocab = a.vocab;
   sp.passes = (bits_all + kMaxBits - 1) / kMaxBits;
   sp.bits = (bits_all + sp.passes - 1) / sp.passes;
-  sp.trow = Rows{a.rows_inner > 0 ? a.rows_inner : 1, a.t_outer, a.t_inner};
+  sp.trow = Rows{a.rows_inner, a.t_outer, a.t_inner};
   sp.tokens = a.tokens;
   sp.count = (int*)ws;
   sp.buf[0] = (uint2*)(ws + 256);
@@ -270,7 +270,7 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   }
   sort_kernel<<<kSortCtas, kSortThreads, sizeof(SortSmem), s>>>(sp);
   const SumParams p{a.grad_ld, a.dim,    a.accumulate,
-                    a.scale,   Rows{a.rows_inner > 0 ? a.rows_inner : 1, a.dy_outer, a.dy_inner},
+                    a.scale,   Rows{a.rows_inner, a.dy_outer, a.dy_inner},
                     sp.buf[(sp.passes - 1) & 1], sp.count, a.dy, a.grad};
   const bool db = a.dy_dtype == M3_DTYPE_BF16, gb = a.grad_dtype == M3_DTYPE_BF16;
   auto* kern = db ? (gb ? sum_kernel<__nv_bfloat16, __nv_bfloat16> : sum_kernel<__nv_bfloat16, float>)

@@ -1,14 +1,14 @@
 // Log probabilities of given tokens, entropy and top alternatives of logits rows.
 //   y = x / T, m = max y, Z = sum e^(y - m):  lse = m + ln Z,  entropy = ln Z - sum e d / Z, d = y - m
-// One read of the logits: a row (or a cluster's share of it) stays in registers as 16-byte
-// vectors.  Each warp sums against its own maximum, so that the (max, sum, sum e d) triples of
-// all warps meet at one barrier, through distributed shared memory where a row has several CTAs.
+// One read of the logits: each warp walks its share of a row with a running maximum and sums
+// against it, and the (max, sum, sum e d) triples of the row's warps meet at one barrier.
 //
-// Alternatives: every warp gives the r-th largest of its lanes' maxima, r = ceil(top / warps); the
-// smallest of these has at least `top` lane maxima at or above it, so every alternative is at or
-// above it as well.  Only vectors that reach this bound are looked into (about twice `top` on
-// rows without order), the candidates are ranked by counting, and the CTAs' sorted lists are merged.
-// Rows that defeat the bound (many equal logits, NaN) take an exact selection by bits.
+// Alternatives: every warp keeps the r-th largest of its lanes' maxima so far, r = ceil(top / warps);
+// the smallest of these over the warps has at least `top` elements at or above it, so every
+// alternative is at or above it as well, and it only rises.  Vectors that reach it when they pass are
+// put aside (on rows without order about 2 top ln(tiles) of them), their elements that reach the
+// final bound are ranked by counting, and the CTAs' sorted lists are merged.  Rows that defeat the
+// bound (many equal logits, rising rows, NaN) take an exact selection by bits.
 #include "m3_internal.h"
 #include "m3_vocab.cuh"
 
@@ -17,13 +17,12 @@ namespace {
 
 using namespace vocab;
 
-constexpr int kNV = 8;          // vectors a thread holds
+constexpr int kNV = 8;          // vectors a thread loads at a time
 constexpr int kMaxCluster = 8;  // CTAs per row (portable size)
-constexpr int kVecCap = 256, kCandCap = 1024;
+constexpr int kVecCap = 512, kCandCap = 512;
 
 struct Params {
-  int64_t rows;
-  int vocab, top, cluster;
+  int rows, vocab, top, cluster, log2_cluster;
   float inv_t;
   Rows lrow, trow;
   const void* logits;
@@ -71,7 +70,7 @@ struct Row {
   __device__ __forceinline__ float logprob(float x) const { return (x - m) * inv_t - ln_z; }
 };
 
-__device__ __forceinline__ Row finish(const Params& p, const Part& r, int64_t row, bool write) {
+__device__ __forceinline__ Row finish(const Params& p, const Part& r, int row, bool write) {
   const float l2 = r.m == -INFINITY ? NAN : log2f(r.s);
   Row w{r.m, l2 * kLn2, p.inv_t};
   if (write) {
@@ -81,7 +80,7 @@ __device__ __forceinline__ Row finish(const Params& p, const Part& r, int64_t ro
   return w;
 }
 
-__device__ __forceinline__ void write_target(const Params& p, const Row& w, int64_t row, int64_t t, float xt) {
+__device__ __forceinline__ void write_target(const Params& p, const Row& w, int row, int64_t t, float xt) {
   p.logprob[row] = t < 0 ? 0.f : t >= p.vocab ? NAN : w.logprob(xt);
 }
 
@@ -143,120 +142,135 @@ __device__ __noinline__ void exact_top(const T* x, int lo, int hi, int need, S& 
   __syncthreads();
 }
 
-template <typename T, int TB, bool RES, bool TOP>
+template <typename T, int TB, bool TOP>
 __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
   constexpr int E = kVec<T>, NW = TB / 32;
   __shared__ Smem<NW, TOP> s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cl = p.cluster, rank = cl > 1 ? cluster_rank() : 0;
-  const int64_t row = blockIdx.x / cl;
+  const int row = (int)blockIdx.x >> p.log2_cluster;
   const int V = p.vocab;
   const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
-  const int shift = row_shift(x), nvec = (shift + V + E - 1) / E, per = (nvec + cl - 1) / cl;
-  const int v0 = rank * per, v1 = min(nvec, v0 + per);
+  const Split sp = split_row(x, V);
+  const int per = (sp.full + cl - 1) >> p.log2_cluster, v0 = min(sp.full, rank * per), n = min(per, sp.full - v0);
+  const uint4* v = reinterpret_cast<const uint4*>(x + sp.head) + v0;
   const float c = p.inv_t * kLog2e;
-  if (cl > 1) cluster_arrive();  // peers have started before anyone writes to their shared memory
+  if (cl > 1) cluster_arrive_relaxed();  // peers have started before anyone writes to their shared memory
 
-  uint4 d[kNV];
-  Part a{-INFINITY, 0.f, 0.f};
-  float mine = -INFINITY;  // this lane's maximum
-  auto load = [&](int base) {
-#pragma unroll
-    for (int j = 0; j < kNV; ++j) {
-      const int q = base + j * TB + tid;
-      d[j] = q < v1 ? load_vec(x, q * E - shift, V) : neg_inf_vec<T>();
-    }
-  };
-  for (int base = v0; base < v1; base += kNV * TB) {
-    load(base);
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kNV; ++j)
-      if (base + j * TB < v1) m = fmaxf(m, vec_max<T>(d[j]));
-    mine = fmaxf(mine, m);
-    m = fmaxf(a.m, warp_max(m));
-    const float ref = finite_or_0(m);
-    float2 s2 = f2s(0.f), u2 = f2s(0.f);
-#pragma unroll
-    for (int j = 0; j < kNV; ++j)
-      if (base + j * TB < v1) add_vec<T>(d[j], ref, c, s2, u2);
-    if (!RES && a.m != -INFINITY) {  // what came before, against the new maximum
-      const float dm = fmaxf((a.m - m) * c, -1e4f), e = ex2(dm);
-      s2.x += a.s * e;
-      u2.x += (a.u + a.s * dm) * e;
-    }
-    a = Part{m, s2.x + s2.y, u2.x + u2.y};
-    if (RES) break;
-  }
   int64_t t = -1;
   float xt = 0.f;
   if (p.targets && rank == 0 && tid == 0) {
     t = p.targets[p.trow.at(row)];
     if (t >= 0 && t < V) xt = ld(x + t);
   }
-  a.s = warp_sum(a.s);
-  a.u = warp_sum(a.u);
-  if (lane == 0) s.part[warp] = a;
-  if constexpr (TOP) {
-    const int r = (p.top + NW - 1) / NW;
-    float v = mine, bound = -INFINITY;
-    for (int i = 0; i < r; ++i) {
-      bound = warp_max(v);
-      const unsigned at = __ballot_sync(0xffffffffu, v == bound);
-      if (lane == __ffs(at) - 1) v = -INFINITY;
+  float m = -INFINITY, mine = -INFINITY;  // the warp's maximum, this lane's
+  float2 s2 = f2s(0.f), u2 = f2s(0.f);
+  auto raise = [&](float to) {  // the sums against a new maximum
+    if (to > m) {
+      if (m != -INFINITY) {
+        const float dm = fmaxf((m - to) * c, -1e4f), e = ex2(dm);
+        u2 = mul2(fma2(s2, f2s(dm), u2), f2s(e));
+        s2 = mul2(s2, f2s(e));
+      }
+      m = to;
     }
-    if (lane == 0) s.bound[warp] = bound;
+  };
+  // warps all of whose lanes see a vector, and how many lane maxima each of them gives
+  const int wide = min(NW, n >> 5), r = wide ? (p.top + wide - 1) / wide : 33;
+  float bound = -INFINITY;  // of the row
+  if constexpr (TOP) {
+    if (lane == 0) s.bound[warp] = r <= 32 && warp >= wide ? INFINITY : -INFINITY;
     if (tid == 0) s.n_vec = s.n_cand = 0;
+    __syncthreads();
   }
+  auto raise_bound = [&]() {  // after a change of a lane's maximum
+    if constexpr (TOP) {
+      if (r > 32 || warp >= wide) return;
+      float left = mine, b = 0.f;
+      for (int i = 0; i < r; ++i) {
+        b = warp_max(left);
+        const unsigned at = __ballot_sync(0xffffffffu, left == b);
+        if (lane == __ffs(at) - 1) left = -INFINITY;
+      }
+      if (lane == 0) *(volatile float*)&s.bound[warp] = b;
+    }
+  };
+  walk<T, kNV, TB>(v, n, tid, Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
+    float mt = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+      if (full.value || base + j * TB < n) mt = fmaxf(mt, vec_max<T>(d[j]));
+    raise(warp_max(mt));
+    const float ref = finite_or_0(m);
+#pragma unroll
+    for (int j = 0; j < kNV; ++j)
+      if (full.value || base + j * TB < n) add_vec<T>(d[j], ref, c, s2, u2);
+    if constexpr (TOP) {
+      if (__any_sync(0xffffffffu, mt > mine)) {
+        mine = fmaxf(mine, mt);
+        raise_bound();
+      }
+      if (base == 0) __syncthreads();  // a first bound from every warp; later ones may be read late
+      __syncwarp();
+      bound = -warp_max(lane < NW ? -*(volatile float*)&s.bound[lane] : -INFINITY);
+      if (mt >= bound) {
+#pragma unroll
+        for (int j = 0; j < kNV; ++j) {
+          const int q = base + j * TB + tid;
+          if ((full.value || q < n) && vec_max<T>(d[j]) >= bound) {
+            const int at = atomicAdd(&s.n_vec, 1);
+            if (at < kVecCap) {
+              s.vec[at] = d[j];
+              s.vec_at[at] = q;
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+  });
+  if (warp == NW - 1) {  // the row's edges
+    const int i = edge_index(sp, lane, rank == 0, rank == cl - 1);
+    const float xe = i >= 0 ? ld(x + i) : -INFINITY;
+    raise(warp_max(xe));
+    const float d = (xe - finite_or_0(m)) * c, e = ex2(d);
+    s2.x += e;
+    u2.x = fmaf(e, fmaxf(d, -1e4f), u2.x);
+    if constexpr (TOP)
+      if (i >= 0) s.cand[atomicAdd(&s.n_cand, 1)] = rank_word(xe, i);
+  }
+  Part a{m, warp_sum(s2.x + s2.y), warp_sum(u2.x + u2.y)};
+  if (lane == 0) s.part[warp] = a;
   __syncthreads();
   a = join(lane < NW ? s.part[lane] : Part{-INFINITY, 0.f, 0.f}, c);
 
   if constexpr (TOP) {
-    const int k = p.top, lo = max(0, v0 * E - shift), hi = min(V, v1 * E - shift);
-    float bound = lane < NW ? s.bound[lane] : INFINITY;
-    bound = -warp_max(-bound);
-    auto scan = [&](int base) {
-#pragma unroll
-      for (int j = 0; j < kNV; ++j)
-        if (base + j * TB < v1 && vec_max<T>(d[j]) >= bound) {
-          const int at = atomicAdd(&s.n_vec, 1);
-          if (at < kVecCap) {
-            s.vec[at] = d[j];
-            s.vec_at[at] = base + j * TB + tid;
-          }
-        }
-    };
-    if (RES) {
-      scan(v0);
-    } else {
-      for (int base = v0; base < v1; base += kNV * TB) {
-        load(base);
-        scan(base);
-      }
-    }
-    __syncthreads();
+    const int k = p.top, first = sp.head + v0 * E;  // element 0 of this share's vectors
+    bound = -warp_max(lane < NW ? -s.bound[lane] : -INFINITY);
     const int nv = s.n_vec;
     if (nv <= kVecCap)
       for (int i = tid; i < nv * E; i += TB) {
         const float xv = ld(reinterpret_cast<const T*>(s.vec) + i);
-        const int idx = s.vec_at[i / E] * E - shift + i % E;
-        if (xv >= bound && idx >= 0 && idx < V) {
+        if (xv >= bound) {
           const int at = atomicAdd(&s.n_cand, 1);
-          if (at < kCandCap) s.cand[at] = rank_word(xv, idx);
+          if (at < kCandCap) s.cand[at] = rank_word(xv, first + s.vec_at[i / E] * E + i % E);
         }
       }
     __syncthreads();
     // the sum is NaN iff the share holds NaN or +inf, which the comparisons above do not order
-    if (nv > kVecCap || s.n_cand > kCandCap || a.s != a.s) exact_top<T, TB>(x, lo, hi, min(k, hi - lo), s);
-    const int n = s.n_cand;
+    if (nv > kVecCap || s.n_cand > kCandCap || a.s != a.s) {
+      const int lo = rank == 0 ? 0 : first, hi = rank == cl - 1 ? V : first + n * E;
+      exact_top<T, TB>(x, lo, hi, min(k, hi - lo), s);
+    }
+    const int nc = s.n_cand;
     uint64_t* list = s.list[rank];
-    for (int i = tid; i < n; i += TB) {
+    for (int i = tid; i < nc; i += TB) {
       const uint64_t w = s.cand[i];
       int above = 0;
-      for (int j = 0; j < n; ++j) above += s.cand[j] > w ? 1 : 0;
+      for (int j = 0; j < nc; ++j) above += s.cand[j] > w ? 1 : 0;
       if (above < k) list[above] = w;
     }
-    for (int i = max(n, 0) + tid; i < k; i += TB) list[i] = 0;
+    for (int i = nc + tid; i < k; i += TB) list[i] = 0;
     for (int i = tid; i < k; i += TB) s.before[i] = i;
     __syncthreads();
   }
@@ -301,8 +315,8 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
       const uint64_t e = s.list[rank][i];
       const int at = s.before[i];
       if (e != 0 && at < k) {
-        p.top_ids[row * k + at] = rank_index(e);
-        p.top_logprob[row * k + at] = w.logprob(key_value((uint32_t)(e >> 32)));
+        p.top_ids[(int64_t)row * k + at] = rank_index(e);
+        p.top_logprob[(int64_t)row * k + at] = w.logprob(key_value((uint32_t)(e >> 32)));
       }
     }
   }
@@ -357,12 +371,12 @@ template <typename T, int NV, bool TOP>
 __global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p) {
   constexpr int E = kVec<T>;
   const int lane = threadIdx.x & 31, V = p.vocab;
-  const int64_t step = (int64_t)gridDim.x * kWarpRows;
+  const int step = gridDim.x * kWarpRows;
   const float c = p.inv_t * kLog2e;
-  int64_t row = (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5);
+  int row = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
   const T* x = nullptr;
   uint4 d[NV];
-  auto load = [&](int64_t r) {
+  auto load = [&](int r) {
     x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(r);
     const int shift = row_shift(x);
 #pragma unroll
@@ -398,7 +412,7 @@ __global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p
         }
       }
     }
-    const int64_t next = row + step;
+    const int next = row + step;
     if (next < p.rows) load(next);  // on its way while this row is finished
     float xt = 0.f;
     if (t >= 0 && t < V) xt = ld(xr + t);
@@ -419,8 +433,8 @@ __global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p
         if ((j & 31) == 31 || j == p.top - 1) {
           const int i = (j & ~31) + lane;
           if (i <= j) {
-            p.top_ids[row * p.top + i] = Word<T>::index(keep);
-            p.top_logprob[row * p.top + i] = w.logprob(Word<T>::value(keep));
+            p.top_ids[(int64_t)row * p.top + i] = Word<T>::index(keep);
+            p.top_logprob[(int64_t)row * p.top + i] = w.logprob(Word<T>::value(keep));
           }
         }
       }
@@ -436,10 +450,10 @@ int sm_count() {
   return c;
 }
 
-template <typename T, int TB, bool RES, bool TOP>
+template <typename T, int TB, bool TOP>
 int launch_cta(const Params& p, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.rows * p.cluster), 1, 1);
+  cfg.gridDim = dim3((unsigned)p.rows * p.cluster, 1, 1);
   cfg.blockDim = dim3(TB, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -448,19 +462,19 @@ int launch_cta(const Params& p, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, score_kernel<T, TB, RES, TOP>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, score_kernel<T, TB, TOP>, p);
   return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_token_logprobs: ") + cudaGetErrorString(e));
 }
 
 template <typename T, int NV, bool TOP>
 int launch_warp(const Params& p, cudaStream_t s) {
-  const int64_t want = (p.rows + kWarpRows - 1) / kWarpRows, most = (int64_t)sm_count() * 8;
+  const int want = (p.rows + kWarpRows - 1) / kWarpRows, most = sm_count() * 8;
   score_warp_kernel<T, NV, TOP><<<(unsigned)(want < most ? want : most), kWarpThreads, 0, s>>>(p);
   return check_launch("m3_token_logprobs");
 }
 
 // A row goes to a warp while its vectors fit the lanes' registers (with alternatives: while a lane
-// can keep its 8 or 16 entries sorted), else to the fewest threads that hold it, else to a cluster.
+// can keep its 8 or 16 entries sorted), else to a CTA, and with few rows to a cluster.
 template <typename T, bool TOP>
 int launch(Params p, int nvec, cudaStream_t s) {
   if (nvec <= 32) return launch_warp<T, 1, TOP>(p, s);
@@ -469,18 +483,15 @@ int launch(Params p, int nvec, cudaStream_t s) {
     if (nvec <= 128) return launch_warp<T, 4, TOP>(p, s);
     if (nvec <= 256) return launch_warp<T, 8, TOP>(p, s);
   }
-  int cl = 1;
-  while (cl < kMaxCluster && (nvec > cl * kNV * 512)) cl *= 2;
-  // few rows: more CTAs per row until they cover the SMs
+  // few rows: several CTAs per row until they cover the SMs
   const int sms = sm_count();
-  while (cl < kMaxCluster && p.rows * cl * 2 <= sms && nvec / (cl * 2) >= 128) cl *= 2;
+  int cl = 1;
+  while (cl < kMaxCluster && (int64_t)p.rows * cl * 2 <= sms && nvec / (cl * 2) >= 128) cl *= 2;
   p.cluster = cl;
-  if (p.rows * cl > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_token_logprobs: too many rows");
-  const int per = (nvec + cl - 1) / cl;
-  if (per > kNV * 512) return launch_cta<T, 512, false, TOP>(p, s);
-  if (per > kNV * 256 || p.rows * cl < sms) return launch_cta<T, 512, true, TOP>(p, s);
-  if (per > kNV * 128) return launch_cta<T, 256, true, TOP>(p, s);
-  return launch_cta<T, 128, true, TOP>(p, s);
+  while ((1 << p.log2_cluster) < cl) ++p.log2_cluster;
+  if ((int64_t)p.rows * cl > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_token_logprobs: too many rows");
+  if (nvec <= kNV * 128 * cl) return launch_cta<T, 128, TOP>(p, s);
+  return (int64_t)p.rows * cl <= 2 * sms ? launch_cta<T, 512, TOP>(p, s) : launch_cta<T, 256, TOP>(p, s);
 }
 
 }  // namespace
@@ -504,10 +515,11 @@ extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
   const bool bf = a.logits_dtype == M3_DTYPE_BF16;
   if (((uintptr_t)a.logits) % (bf ? 2 : 4)) return set_error(M3_ERR_ARG, "m3_token_logprobs: logits are not aligned to their type");
   Params p;
-  p.rows = rows;
+  p.rows = (int)rows;
   p.vocab = a.vocab;
   p.top = a.top;
   p.cluster = 1;
+  p.log2_cluster = 0;
   p.inv_t = 1.f / a.temperature;
   p.lrow = Rows{a.rows_inner, a.ld_outer, a.ld_inner};
   p.trow = Rows{a.rows_inner, a.t_outer, a.t_inner};

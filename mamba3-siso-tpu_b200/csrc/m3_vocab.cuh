@@ -8,7 +8,7 @@ namespace m3 {
 namespace vocab {
 
 constexpr float kLn2 = 0.69314718055994530942f;
-constexpr int kMaxVocab = 1 << 30;  // element and vector indices are ints
+constexpr int kMaxVocab = 1 << 30, kMaxRows = 1 << 30;  // element, vector and row indices are ints
 
 // The most 16-byte vectors that a row of n elements can touch: its start's place in a vector is the
 // same for every row if both strides are whole vectors, else anything.
@@ -18,13 +18,32 @@ inline int most_vectors(const void* x, int n, int size, int64_t outer, int64_t i
   return (shift + n + e - 1) / e;
 }
 
-// Element offset of row r = (r / inner) * outer_stride + (r % inner) * inner_stride.
+// n / d for 0 <= n < 2^31, 1 <= d < 2^31, by one multiplication: with s = ceil(log2 d) and
+// m = ceil(2^(31 + s) / d) < 2^32, m d exceeds 2^(31 + s) by less than d <= 2^s,
+// so n m / 2^(31 + s) exceeds n / d by less than 1 / d.
+struct Divider {
+  uint32_t m;
+  int shift, d;
+  Divider() = default;
+  explicit Divider(int div) : d(div) {
+    int s = 0;
+    while (((int64_t)1 << s) < div) ++s;
+    shift = 31 + s;
+    m = (uint32_t)((((uint64_t)1 << shift) + div - 1) / div);
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)((uint64_t)(uint32_t)n * m >> shift); }
+};
+
+// Element offset of row r = (r / inner) * outer_stride + (r % inner) * inner_stride.  (A 64-bit
+// division by every thread cost as much as 20 logits each.)
 struct Rows {
-  int inner;
+  Divider inner;
   int64_t outer_stride, inner_stride;
-  __device__ __forceinline__ int64_t at(int64_t r) const {
-    const int64_t o = r / inner;
-    return o * outer_stride + (r - o * inner) * inner_stride;
+  Rows() = default;
+  Rows(int n, int64_t outer, int64_t in) : inner(n > 0 ? n : 1), outer_stride(outer), inner_stride(in) {}
+  __device__ __forceinline__ int64_t at(int r) const {
+    const int o = inner.div(r);
+    return o * outer_stride + (r - o * inner.d) * inner_stride;
   }
 };
 
@@ -45,32 +64,57 @@ __device__ __forceinline__ uint64_t rank_word(float x, int idx) {
 __device__ __forceinline__ int rank_index(uint64_t w) { return (int)~(uint32_t)w; }
 
 // ---- a row as 16-byte vectors ---------------------------------------------------------------
-// Vector q of a row that starts `shift` elements past a 16-byte boundary holds the elements
-// [q E - shift, q E - shift + E); those outside [0, n) read as -inf, which has probability 0.
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
 template <typename T>
-__device__ __forceinline__ int row_shift(const T* x) {
+__device__ __forceinline__ int row_shift(const T* x) {  // elements past a 16-byte boundary
   return (int)(((uintptr_t)x & 15u) / sizeof(T));
 }
 
 template <typename T>
-__device__ __forceinline__ uint4 neg_inf_vec() {
+__device__ __forceinline__ uint4 neg_inf_vec() {  // probability 0
   const uint32_t w = sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
   return make_uint4(w, w, w, w);
 }
 
+// Logits pass through L1 without a place there.  In L2 they either stay for a second walk of the row
+// or go first; a gradient goes first as well, so that it does not displace the rows in flight.
+enum class Keep { kNo, kYes };
+
+__device__ __forceinline__ uint64_t l2_policy(Keep keep) {
+  uint64_t p;
+  if (keep == Keep::kYes)
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  else
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint4 load_stream(const uint4* p, uint64_t policy) {
+  uint4 u;
+  asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "l"(p), "l"(policy));
+  return u;
+}
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+  uint4 u;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "l"(p));
+  return u;
+}
+__device__ __forceinline__ void store_stream(void* p, const uint4& u, uint64_t policy) {
+  asm volatile("st.global.L2::cache_hint.v4.u32 [%0], {%1,%2,%3,%4}, %5;" ::"l"(p), "r"(u.x), "r"(u.y), "r"(u.z),
+               "r"(u.w), "l"(policy)
+               : "memory");
+}
+
+// Vector of the elements [lo, lo + E) of a row, those outside [0, n) as -inf.
 template <typename T>
 __device__ __forceinline__ uint4 load_vec(const T* row, int lo, int n) {
   constexpr int E = kVec<T>;
-  uint4 u;
-  if (lo >= 0 && lo + E <= n) {  // read once: no place in L1
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                 : "l"(row + lo));
-    return u;
-  }
+  if (lo >= 0 && lo + E <= n) return load_once(reinterpret_cast<const uint4*>(row + lo));
   // the ragged ends of a row, element by element
   uint32_t w[4];
 #pragma unroll
@@ -86,6 +130,56 @@ __device__ __forceinline__ uint4 load_vec(const T* row, int lo, int n) {
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A row of n elements as `head` elements, `full` aligned vectors and `tail` elements.  The first CTA
+// of a row's cluster takes the head and the last one the tail: lanes 0.. and 16.. of one warp.
+struct Split {
+  int head, full, tail, n;
+};
+template <typename T>
+__device__ __forceinline__ Split split_row(const T* x, int n) {
+  constexpr int E = kVec<T>;
+  Split r;
+  r.n = n;
+  r.head = min(n, (E - row_shift(x)) & (E - 1));
+  r.full = (n - r.head) / E;
+  r.tail = n - r.head - r.full * E;
+  return r;
+}
+__device__ __forceinline__ int edge_index(const Split& r, int lane, bool first, bool last) {  // -1: none
+  if (first && lane < r.head) return lane;
+  return last && lane >= 16 && lane - 16 < r.tail ? r.n - r.tail + lane - 16 : -1;
+}
+
+// Walks n vectors by TB threads, NV a thread and tile: f(d, base, full) with d[j] = v[base + j TB +
+// thread], -inf past the end.  `full` tiles have no bounds to check, which halves the instructions of
+// the loop; in the last one, f skips the j with base + j TB >= n.
+template <bool B>
+struct Flag {
+  static constexpr bool value = B;
+};
+template <typename T, int NV, int TB, typename F>
+__device__ __forceinline__ void walk(const uint4* v, int n, int thread, Keep keep, F f) {
+  const uint64_t policy = l2_policy(keep);
+  int base = 0;
+  for (; base + NV * TB <= n; base += NV * TB) {
+    const uint4* q = v + base + thread;
+    uint4 d[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) d[j] = load_stream(q + j * TB, policy);
+    f(d, base, Flag<true>());
+  }
+  if (base < n) {
+    uint4 d[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int i = base + j * TB + thread;
+      d[j] = neg_inf_vec<T>();
+      if (i < n) d[j] = load_stream(v + i, policy);
+    }
+    f(d, base, Flag<false>());
+  }
 }
 
 // The vector's elements as pairs of floats.
@@ -126,6 +220,8 @@ __device__ __forceinline__ int cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return (int)r;
 }
+// Only that the peers have started: nothing written before it is waited for.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The address of this CTA's shared `p` in CTA `rank` of the cluster.

@@ -125,8 +125,8 @@ def row_counts(lead):
     outer = 1
     for s in lead[:-1]:
         outer *= s
-    if outer * inner >= 1 << 31:
-        raise ValueError(f"{outer * inner} rows: at most 2^31 - 1 are supported")
+    if outer * inner > 1 << 30:
+        raise ValueError(f"{outer * inner} rows: at most 2^30 are supported")
     return (outer, inner) if inner else (0, 1)
 
 
