@@ -1,8 +1,9 @@
 // Embedding lookup with scaling, and the table's gradient by sorted tokens.
 //   out[r] = scale * table[token r]              grad[v] = scale * sum of dy[r] over token r == v
 // The gradient's rows are summed in the order of r (fp32), so that it is the same every call:
-// (token, r) pairs are put in order by a stable radix sort (one 8-CTA cluster), then every
-// vocabulary row sums its own range of the sorted list.
+// (token, r) pairs are put in order by a stable radix sort (one 8-CTA cluster), the sorted list is cut
+// into chunks of equal length, each summed by one group of threads, and the pieces of tokens that
+// cross a cut are joined.  The cuts depend on the sizes alone, so the result is the same every call.
 #include <cooperative_groups.h>
 
 #include "m3_internal.h"
@@ -15,6 +16,16 @@ using vocab::Rows;
 
 constexpr int kThreads = 256;
 
+// The threads of a CTA as groups over a row's columns, N columns a thread: at most kThreads threads a
+// group, wider rows take several CTAs (blockIdx.y).
+struct Columns {
+  int width, groups;  // threads per group, groups per CTA
+  __device__ __forceinline__ int group() const { return (int)threadIdx.x / width; }
+  __device__ __forceinline__ int first(int n) const {
+    return ((int)threadIdx.x - group() * width + (int)blockIdx.y * width) * n;
+  }
+};
+
 // ---- lookup -------------------------------------------------------------------------------
 struct FwdParams {
   int64_t rows, table_ld, out_ld;
@@ -24,18 +35,74 @@ struct FwdParams {
   const int64_t* tokens;
   const void* table;
   void* out;
+  Columns cols;
 };
 
-template <typename T, typename O>
+// N consecutive elements as floats and back; p is aligned to min(16 bytes, N elements).
+template <int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
+  if constexpr (N == 8 && sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else if constexpr (N == 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const float2 a = bf2f(u.x), b = bf2f(u.y), c = bf2f(u.z), d = bf2f(u.w);
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = c.x, f[5] = c.y, f[6] = d.x, f[7] = d.y;
+  } else if constexpr (N == 2 && sizeof(T) == 4) {
+    const float2 a = *reinterpret_cast<const float2*>(p);
+    f[0] = a.x, f[1] = a.y;
+  } else if constexpr (N == 2) {
+    const float2 a = bf2f(*reinterpret_cast<const uint32_t*>(p));
+    f[0] = a.x, f[1] = a.y;
+  } else {
+    f[0] = ld(p);
+  }
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_n(T* p, const float (&f)[N]) {
+  if constexpr (N == 8 && sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else if constexpr (N == 8) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(f2bf(f2(f[0], f[1])), f2bf(f2(f[2], f[3])), f2bf(f2(f[4], f[5])), f2bf(f2(f[6], f[7])));
+  } else if constexpr (N == 2 && sizeof(T) == 4) {
+    *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
+  } else if constexpr (N == 2) {
+    *reinterpret_cast<uint32_t*>(p) = f2bf(f2(f[0], f[1]));
+  } else {
+    stg<T>(p, f[0]);
+  }
+}
+
+constexpr int kRows = 4;  // rows in flight
+
+template <typename T, typename O, int N>
 __global__ void __launch_bounds__(kThreads) embed_kernel(const FwdParams p) {
-  const int64_t total = p.rows * p.dim;
-  for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t r = i / p.dim;
-    const int c = (int)(i - r * p.dim);
-    const int64_t t = p.tokens[p.trow.at((int)r)];
-    float v = t < 0 ? 0.f : NAN;
-    if (t >= 0 && t < p.vocab) v = ld(reinterpret_cast<const T*>(p.table) + t * p.table_ld + c) * p.scale;
-    stg<O>(reinterpret_cast<O*>(p.out) + r * p.out_ld + c, v);
+  const int g = p.cols.group(), c = p.cols.first(N);
+  if (g >= p.cols.groups || c >= p.dim) return;
+  const T* table = reinterpret_cast<const T*>(p.table) + c;
+  O* out = reinterpret_cast<O*>(p.out) + c;
+  const int64_t step = (int64_t)gridDim.x * p.cols.groups;
+  for (int64_t r0 = (int64_t)blockIdx.x * p.cols.groups + g; r0 < p.rows; r0 += step * kRows) {
+    int64_t t[kRows];
+    float v[kRows][N];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) t[j] = r0 + j * step < p.rows ? p.tokens[p.trow.at((int)(r0 + j * step))] : -1;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const float none = t[j] < 0 ? 0.f : NAN;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[j][i] = none;
+      if (t[j] >= 0 && t[j] < p.vocab) load_n<N>(table + t[j] * p.table_ld, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+      if (r0 + j * step < p.rows) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[j][i] *= p.scale;
+        store_n<N>(out + (r0 + j * step) * p.out_ld, v[j]);
+      }
   }
 }
 
@@ -148,16 +215,35 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
 }
 
 // ---- row sums -----------------------------------------------------------------------------
+// Chunk k holds the sorted entries [k C, (k + 1) C).  A group walks its chunk and writes the rows of the
+// tokens that lie within it; of a token that goes on past an end it writes its piece to `parts`: slot 2 k
+// for one that began before the chunk, 2 k + 1 for one that begins in it.
 struct SumParams {
   int64_t grad_ld;
-  int dim, accumulate;
+  int dim, chunk, vocab, accumulate, sum_ctas;
   float scale;
   Rows drow;
   const uint2* sorted;
   const int* count;
   const void* dy;
   void* grad;
+  float* parts;  // (2 chunks, dim)
+  Columns cols;
 };
+
+template <int N, typename G>
+__device__ __forceinline__ void write_row(const SumParams& p, uint32_t token, int c, float (&s)[N]) {
+  G* g = reinterpret_cast<G*>(p.grad) + (int64_t)token * p.grad_ld + c;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] *= p.scale;
+  if (p.accumulate) {
+    float old[N];
+    load_n<N>(g, old);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] += old[i];
+  }
+  store_n<N>(g, s);
+}
 
 __device__ __forceinline__ int lower_bound(const uint2* a, int n, uint32_t key) {
   int lo = 0, hi = n;
@@ -171,18 +257,111 @@ __device__ __forceinline__ int lower_bound(const uint2* a, int n, uint32_t key) 
   return lo;
 }
 
-template <typename D, typename G>
+constexpr int kAhead = 8;  // entries in flight
+
+template <typename D, typename G, int N>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const SumParams p) {
-  const int v = blockIdx.x, n = *p.count;
-  const int i0 = lower_bound(p.sorted, n, (uint32_t)v), i1 = lower_bound(p.sorted, n, (uint32_t)v + 1u);
-  if (p.accumulate && i0 == i1) return;
-  G* g = reinterpret_cast<G*>(p.grad) + v * p.grad_ld;
-  for (int c = threadIdx.x; c < p.dim; c += kThreads) {
-    float s = 0.f;
-    for (int i = i0; i < i1; ++i) s += ld(reinterpret_cast<const D*>(p.dy) + p.drow.at((int)p.sorted[i].y) + c);
-    s *= p.scale;
-    stg<G>(g + c, p.accumulate ? ld(g + c) + s : s);
+  const int n = *p.count;
+  if ((int)blockIdx.x >= p.sum_ctas) {
+    // the rows of tokens that do not occur: a warp looks 32 of them up and clears those
+    const int lane = threadIdx.x & 31, warps = ((int)gridDim.x - p.sum_ctas) * (kThreads / 32);
+    int64_t v0 = (int64_t)(((int)blockIdx.x - p.sum_ctas) * (kThreads / 32) + (int)(threadIdx.x >> 5)) * 32;
+    const int span = p.cols.width * N, c0 = (int)blockIdx.y * span, c1 = min(p.dim, c0 + span);
+    float zero[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) zero[i] = 0.f;
+    for (; v0 < p.vocab; v0 += (int64_t)warps * 32) {
+      const int64_t v = v0 + lane;
+      bool absent = false;
+      if (v < p.vocab) {
+        const int i = lower_bound(p.sorted, n, (uint32_t)v);
+        absent = i == n || p.sorted[i].x != (uint32_t)v;
+      }
+      for (unsigned m = __ballot_sync(0xffffffffu, absent); m; m &= m - 1) {
+        G* g = reinterpret_cast<G*>(p.grad) + (v0 + __ffs(m) - 1) * p.grad_ld;
+        for (int c = c0 + lane * N; c < c1; c += 32 * N) store_n<N>(g + c, zero);
+      }
+    }
+    return;
   }
+  const int g = p.cols.group(), c = p.cols.first(N);
+  if (g >= p.cols.groups || c >= p.dim) return;
+  const int64_t k = (int64_t)blockIdx.x * p.cols.groups + g, b0 = k * p.chunk;
+  if (b0 >= n) return;
+  const int i0 = (int)b0, i1 = (int)min((int64_t)n, b0 + p.chunk);
+  const D* dy = reinterpret_cast<const D*>(p.dy) + c;
+  uint32_t token = p.sorted[i0].x;
+  bool began = i0 > 0 && p.sorted[i0 - 1].x == token;  // the current token's entries began before the chunk
+  float acc[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  for (int i = i0; i < i1; i += kAhead) {
+    uint2 e[kAhead];
+    float v[kAhead][N];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) e[j] = p.sorted[min(i + j, i1 - 1)];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i + j < i1) load_n<N>(dy + p.drow.at((int)e[j].y), v[j]);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i + j < i1) {
+        if (e[j].x != token) {
+          if (began)
+            store_n<N>(p.parts + 2 * k * p.dim + c, acc);
+          else
+            write_row<N, G>(p, token, c, acc);
+          token = e[j].x;
+          began = false;
+#pragma unroll
+          for (int q = 0; q < N; ++q) acc[q] = 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < N; ++q) acc[q] += v[j][q];
+      }
+  }
+  const bool goes_on = i1 < n && p.sorted[i1].x == token;
+  if (began || goes_on)
+    store_n<N>(p.parts + (2 * k + (began ? 0 : 1)) * p.dim + c, acc);
+  else
+    write_row<N, G>(p, token, c, acc);
+}
+
+// Joins the pieces of the tokens that cross a cut, one CTA per chunk in which such a token begins: its
+// groups take the pieces in turn, and their sums meet in a fixed order.
+template <typename G, int N>
+__global__ void __launch_bounds__(kThreads) join_kernel(const SumParams p) {
+  __shared__ float sums[kThreads * N];
+  const int n = *p.count;
+  const int64_t k = blockIdx.x, b1 = (k + 1) * p.chunk;
+  if (b1 >= n) return;
+  const uint32_t token = p.sorted[b1 - 1].x;
+  if (p.sorted[b1].x != token) return;                                    // nothing goes on here
+  if (k > 0 && p.sorted[b1 - p.chunk - 1].x == token) return;             // it began in an earlier chunk
+  const int last = (lower_bound(p.sorted, n, token + 1u) - 1) / p.chunk;  // the chunk in which it ends
+  const int g = p.cols.group(), c = p.cols.first(N);
+  const bool live = g < p.cols.groups && c < p.dim;
+  float acc[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  if (live) {
+    if (g == 0) load_n<N>(p.parts + (2 * k + 1) * p.dim + c, acc);
+#pragma unroll 4
+    for (int64_t q = k + 1 + g; q <= last; q += p.cols.groups) {
+      float v[N];
+      load_n<N>(p.parts + 2 * q * p.dim + c, v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] += v[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) sums[threadIdx.x * N + j] = acc[j];
+  __syncthreads();
+  if (!live || g > 0) return;
+  for (int h = 1; h < p.cols.groups; ++h)
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] += sums[(threadIdx.x + h * p.cols.width) * N + j];
+  write_row<N, G>(p, token, c, acc);
 }
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -195,6 +374,67 @@ int sm_count() {
 }
 
 bool dtype_ok(int d) { return d == M3_DTYPE_F32 || d == M3_DTYPE_BF16; }
+
+Columns columns(int dim, int n) {
+  const int all = (dim + n - 1) / n, width = all < kThreads ? all : kThreads;
+  return Columns{width, kThreads / width};
+}
+int slabs(int dim, int n, const Columns& c) { return (dim + n * c.width - 1) / (n * c.width); }
+
+// Whether rows of `size`-byte elements (base and strides) allow N elements at a time.
+bool whole(const void* p, int size, int n, int dim, int64_t s0, int64_t s1) {
+  const int bytes = size * n < 16 ? size * n : 16, e = bytes / size;
+  return dim % n == 0 && ((uintptr_t)p) % bytes == 0 && s0 % e == 0 && s1 % e == 0;
+}
+
+template <typename T, typename O, int N>
+void launch_embed(FwdParams p, cudaStream_t s) {
+  p.cols = columns(p.dim, N);
+  const int y = slabs(p.dim, N, p.cols);
+  const int64_t want = (p.rows + p.cols.groups - 1) / p.cols.groups, most = (int64_t)sm_count() * 8;
+  embed_kernel<T, O, N><<<dim3((unsigned)(want < most ? want : most), y), kThreads, 0, s>>>(p);
+}
+
+template <typename T, typename O>
+void launch_embed(const FwdParams& p, cudaStream_t s) {
+  auto fits = [&](int n) {
+    return whole(p.table, sizeof(T), n, p.dim, p.table_ld, 0) && whole(p.out, sizeof(O), n, p.dim, p.out_ld, 0);
+  };
+  if (fits(8)) return launch_embed<T, O, 8>(p, s);
+  if (fits(2)) return launch_embed<T, O, 2>(p, s);
+  launch_embed<T, O, 1>(p, s);
+}
+
+// Entries per chunk: enough chunks for 1024 threads of 8 columns on each of 148 SMs.
+constexpr int kMinChunk = 16, kMaxChunk = 256;
+
+int chunk_of(int64_t rows, int dim) {
+  int64_t c = rows * ((dim + 7) / 8) / (148 * 1024);  // not the device's: the sums' order depends on it
+  c = (c + 7) / 8 * 8;
+  return (int)(c < kMinChunk ? kMinChunk : c > kMaxChunk ? kMaxChunk : c);
+}
+
+template <typename D, typename G, int N>
+void launch_sum(SumParams p, int64_t rows, cudaStream_t s) {
+  p.cols = columns(p.dim, N);
+  const int y = slabs(p.dim, N, p.cols);
+  const int64_t chunks = (rows + p.chunk - 1) / p.chunk;
+  p.sum_ctas = (int)((chunks + p.cols.groups - 1) / p.cols.groups);
+  const int64_t want = (p.vocab + 32 * (kThreads / 32) - 1) / (32 * (kThreads / 32)), most = (int64_t)sm_count() * 8;
+  const int64_t clear = p.accumulate ? 0 : want < most ? want : most;
+  if (p.sum_ctas + clear > 0) sum_kernel<D, G, N><<<dim3((unsigned)(p.sum_ctas + clear), y), kThreads, 0, s>>>(p);
+  if (chunks > 1) join_kernel<G, N><<<dim3((unsigned)(chunks - 1), y), kThreads, 0, s>>>(p);
+}
+
+template <typename D, typename G>
+void launch_sum(const SumParams& p, int64_t rows, int64_t dy_outer, int64_t dy_inner, cudaStream_t s) {
+  auto fits = [&](int n) {
+    return whole(p.dy, sizeof(D), n, p.dim, dy_outer, dy_inner) && whole(p.grad, sizeof(G), n, p.dim, p.grad_ld, 0);
+  };
+  if (fits(8)) return launch_sum<D, G, 8>(p, rows, s);
+  if (fits(2)) return launch_sum<D, G, 2>(p, rows, s);
+  launch_sum<D, G, 1>(p, rows, s);
+}
 
 }  // namespace
 }  // namespace m3
@@ -213,21 +453,24 @@ extern "C" int m3_embed(const M3EmbedArgs* args, void* stream) {
   if (rows == 0) return M3_OK;
   if (!a.tokens || !a.table || !a.out) return set_error(M3_ERR_ARG, "m3_embed: NULL pointer");
   if (a.table_ld < a.dim || a.out_ld < a.dim) return set_error(M3_ERR_SHAPE, "m3_embed: bad leading dimension");
-  const FwdParams p{rows,     a.table_ld, a.out_ld, a.vocab, a.dim, a.scale, Rows{a.rows_inner, a.t_outer, a.t_inner},
-                    a.tokens, a.table,    a.out};
+  const size_t ts = a.table_dtype == M3_DTYPE_BF16 ? 2 : 4, os = a.out_dtype == M3_DTYPE_BF16 ? 2 : 4;
+  if (((uintptr_t)a.table) % ts || ((uintptr_t)a.out) % os)
+    return set_error(M3_ERR_ARG, "m3_embed: table and out must be aligned to their types");
+  const FwdParams p{rows,     a.table_ld, a.out_ld, a.vocab,  a.dim, a.scale, Rows{a.rows_inner, a.t_outer, a.t_inner},
+                    a.tokens, a.table,    a.out,    Columns{}};
   cudaStream_t s = (cudaStream_t)stream;
-  const int64_t want = (rows * a.dim + kThreads - 1) / kThreads, most = (int64_t)sm_count() * 8;
-  const unsigned grid = (unsigned)(want < most ? want : most);
-  const bool tb = a.table_dtype == M3_DTYPE_BF16, ob = a.out_dtype == M3_DTYPE_BF16;
-  auto* kern = tb ? (ob ? embed_kernel<__nv_bfloat16, __nv_bfloat16> : embed_kernel<__nv_bfloat16, float>)
-                  : (ob ? embed_kernel<float, __nv_bfloat16> : embed_kernel<float, float>);
-  kern<<<grid, kThreads, 0, s>>>(p);
+  using bf16 = __nv_bfloat16;
+  if (ts == 2)
+    os == 2 ? launch_embed<bf16, bf16>(p, s) : launch_embed<bf16, float>(p, s);
+  else
+    os == 2 ? launch_embed<float, bf16>(p, s) : launch_embed<float, float>(p, s);
   return check_launch("m3_embed");
 }
 
 extern "C" size_t m3_embed_bwd_workspace_size(int64_t rows, int32_t dim) {
   if (rows < 0 || rows > vocab::kMaxRows || dim <= 0) return 0;
-  return 2 * align256((size_t)rows * sizeof(uint2)) + 256;
+  const size_t chunks = ((size_t)rows + chunk_of(rows, dim) - 1) / chunk_of(rows, dim);
+  return 256 + 2 * align256((size_t)rows * sizeof(uint2)) + 2 * chunks * dim * sizeof(float);
 }
 
 extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
@@ -241,6 +484,9 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   if (rows > vocab::kMaxRows) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: more than 2^30 rows");
   if (!a.grad || (rows > 0 && (!a.tokens || !a.dy))) return set_error(M3_ERR_ARG, "m3_embed_bwd: NULL pointer");
   if (a.grad_ld < a.dim) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: bad leading dimension");
+  const size_t ds = a.dy_dtype == M3_DTYPE_BF16 ? 2 : 4, gs = a.grad_dtype == M3_DTYPE_BF16 ? 2 : 4;
+  if (((uintptr_t)a.dy) % ds || ((uintptr_t)a.grad) % gs)
+    return set_error(M3_ERR_ARG, "m3_embed_bwd: dy and grad must be aligned to their types");
   const size_t need = m3_embed_bwd_workspace_size(rows, a.dim);
   if (!a.workspace || a.workspace_bytes < need || ((uintptr_t)a.workspace) % 256)
     return set_error(M3_ERR_WORKSPACE, "m3_embed_bwd: 256-byte aligned workspace of " + std::to_string(need) +
@@ -269,12 +515,25 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
     if (dev < 64) attr[dev] = true;
   }
   sort_kernel<<<kSortCtas, kSortThreads, sizeof(SortSmem), s>>>(sp);
-  const SumParams p{a.grad_ld, a.dim,    a.accumulate,
-                    a.scale,   Rows{a.rows_inner, a.dy_outer, a.dy_inner},
-                    sp.buf[(sp.passes - 1) & 1], sp.count, a.dy, a.grad};
-  const bool db = a.dy_dtype == M3_DTYPE_BF16, gb = a.grad_dtype == M3_DTYPE_BF16;
-  auto* kern = db ? (gb ? sum_kernel<__nv_bfloat16, __nv_bfloat16> : sum_kernel<__nv_bfloat16, float>)
-                  : (gb ? sum_kernel<float, __nv_bfloat16> : sum_kernel<float, float>);
-  kern<<<(unsigned)a.vocab, kThreads, 0, s>>>(p);
+  const SumParams p{a.grad_ld,
+                    a.dim,
+                    chunk_of(rows, a.dim),
+                    a.vocab,
+                    a.accumulate,
+                    0,
+                    a.scale,
+                    Rows{a.rows_inner, a.dy_outer, a.dy_inner},
+                    sp.buf[(sp.passes - 1) & 1],
+                    sp.count,
+                    a.dy,
+                    a.grad,
+                    (float*)(ws + 256 + 2 * align256((size_t)rows * sizeof(uint2))),
+                    Columns{}};
+  using bf16 = __nv_bfloat16;
+  const bool gb = a.grad_dtype == M3_DTYPE_BF16;
+  if (a.dy_dtype == M3_DTYPE_BF16)
+    gb ? launch_sum<bf16, bf16>(p, rows, a.dy_outer, a.dy_inner, s) : launch_sum<bf16, float>(p, rows, a.dy_outer, a.dy_inner, s);
+  else
+    gb ? launch_sum<float, bf16>(p, rows, a.dy_outer, a.dy_inner, s) : launch_sum<float, float>(p, rows, a.dy_outer, a.dy_inner, s);
   return check_launch("m3_embed_bwd");
 }
