@@ -2,8 +2,8 @@
 //   out[r] = scale * table[token r]              grad[v] = scale * sum of dy[r] over token r == v
 // The gradient's rows are summed in the order of r (fp32), so that it is the same every call:
 // (token, r) pairs are put in order by a stable radix sort (one 8-CTA cluster), the sorted list is cut
-// into chunks of equal length, each summed by one group of threads, and the pieces of tokens that
-// cross a cut are joined.  The cuts depend on the sizes alone, so the result is the same every call.
+// into chunks of equal length, each summed by one group of threads, and the pieces of tokens longer
+// than that are joined.  The cuts depend on the sizes alone, so the result is the same every call.
 #include <cooperative_groups.h>
 
 #include "m3_internal.h"
@@ -38,31 +38,62 @@ struct FwdParams {
   Columns cols;
 };
 
-// N consecutive elements as floats and back; p is aligned to min(16 bytes, N elements).
+// N consecutive elements, as loaded (so that many loads can be under way before the first is looked
+// at) and as floats; the address is aligned to all of them.  (Eight floats are one 256-bit access: two
+// of 128 bits would each touch half of every 32-byte sector.)
 template <int N, typename T>
-__device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
-  if constexpr (N == 8 && sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else if constexpr (N == 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+struct Raw;
+template <>
+struct Raw<8, float> {
+  float f8[8];
+  __device__ __forceinline__ void load(const float* p) { ldg8(p, f8); }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = f8[i];
+  }
+};
+template <>
+struct Raw<8, __nv_bfloat16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
     const float2 a = bf2f(u.x), b = bf2f(u.y), c = bf2f(u.z), d = bf2f(u.w);
     f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = c.x, f[5] = c.y, f[6] = d.x, f[7] = d.y;
-  } else if constexpr (N == 2 && sizeof(T) == 4) {
-    const float2 a = *reinterpret_cast<const float2*>(p);
-    f[0] = a.x, f[1] = a.y;
-  } else if constexpr (N == 2) {
-    const float2 a = bf2f(*reinterpret_cast<const uint32_t*>(p));
-    f[0] = a.x, f[1] = a.y;
-  } else {
-    f[0] = ld(p);
   }
+};
+template <>
+struct Raw<2, float> {
+  float2 a;
+  __device__ __forceinline__ void load(const float* p) { a = *reinterpret_cast<const float2*>(p); }
+  __device__ __forceinline__ void get(float (&f)[2]) const { f[0] = a.x, f[1] = a.y; }
+};
+template <>
+struct Raw<2, __nv_bfloat16> {
+  uint32_t u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint32_t*>(p); }
+  __device__ __forceinline__ void get(float (&f)[2]) const {
+    const float2 a = bf2f(u);
+    f[0] = a.x, f[1] = a.y;
+  }
+};
+template <typename T>
+struct Raw<1, T> {
+  T u;
+  __device__ __forceinline__ void load(const T* p) { u = *p; }
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = ld(&u); }
+};
+template <int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
+  Raw<N, T> r;
+  r.load(p);
+  r.get(f);
 }
 template <int N, typename T>
 __device__ __forceinline__ void store_n(T* p, const float (&f)[N]) {
   if constexpr (N == 8 && sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]),
+                 "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                 : "memory");
   } else if constexpr (N == 8) {
     *reinterpret_cast<uint4*>(p) =
         make_uint4(f2bf(f2(f[0], f[1])), f2bf(f2(f[2], f[3])), f2bf(f2(f[4], f[5])), f2bf(f2(f[6], f[7])));
@@ -83,25 +114,30 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const FwdParams p) {
   if (g >= p.cols.groups || c >= p.dim) return;
   const T* table = reinterpret_cast<const T*>(p.table) + c;
   O* out = reinterpret_cast<O*>(p.out) + c;
-  const int64_t step = (int64_t)gridDim.x * p.cols.groups;
-  for (int64_t r0 = (int64_t)blockIdx.x * p.cols.groups + g; r0 < p.rows; r0 += step * kRows) {
+  const int64_t step = (int64_t)gridDim.x * p.cols.groups, start = (int64_t)blockIdx.x * p.cols.groups + g;
+  int64_t next[kRows];
+  auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) next[j] = r0 + j * step < p.rows ? p.tokens[p.trow.at((int)(r0 + j * step))] : -1;
+  };
+  fetch(start);
+  for (int64_t r0 = start; r0 < p.rows; r0 += step * kRows) {
     int64_t t[kRows];
-    float v[kRows][N];
+    Raw<N, T> v[kRows];
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) t[j] = r0 + j * step < p.rows ? p.tokens[p.trow.at((int)(r0 + j * step))] : -1;
+    for (int j = 0; j < kRows; ++j) t[j] = next[j];
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) {
-      const float none = t[j] < 0 ? 0.f : NAN;
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[j][i] = none;
-      if (t[j] >= 0 && t[j] < p.vocab) load_n<N>(table + t[j] * p.table_ld, v[j]);
-    }
+    for (int j = 0; j < kRows; ++j) v[j].load(table + (t[j] >= 0 && t[j] < p.vocab ? t[j] : 0) * p.table_ld);
+    fetch(r0 + step * kRows);
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
       if (r0 + j * step < p.rows) {
+        float f[N];
+        v[j].get(f);
+        const float none = t[j] < 0 ? 0.f : NAN;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[j][i] *= p.scale;
-        store_n<N>(out + (r0 + j * step) * p.out_ld, v[j]);
+        for (int i = 0; i < N; ++i) f[i] = t[j] >= 0 && t[j] < p.vocab ? f[i] * p.scale : none;
+        store_n<N>(out + (r0 + j * step) * p.out_ld, f);
       }
   }
 }
@@ -109,6 +145,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const FwdParams p) {
 // ---- stable radix sort of (token, r) ------------------------------------------------------
 constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
+constexpr int kSortAhead = 8;  // entries a lane has in flight
 
 struct SortParams {
   int64_t rows;
@@ -117,6 +154,8 @@ struct SortParams {
   const int64_t* tokens;
   uint2* buf[2];  // (token, r); the result is in buf[(passes - 1) & 1]
   int* count;     // entries in the result: the tokens inside [0, vocab)
+  unsigned char* clear;  // gradient whose rows of absent tokens the other CTAs clear, NULL = none
+  int64_t row_bytes, ld_bytes;
 };
 
 struct SortSmem {
@@ -125,6 +164,36 @@ struct SortSmem {
   int wsum[kSortWarps];
 };
 
+// Clears the gradient's rows of the tokens that do not occur, CTA by CTA (`cta` of `ctas`), while the
+// first cluster sorts: every CTA marks all tokens in a bitmap of its own, then clears its share.
+__device__ __forceinline__ void clear_absent(const SortParams& p, uint32_t* seen, int cta, int ctas) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < (p.vocab + 31) / 32; i += kSortThreads) seen[i] = 0u;
+  __syncthreads();
+  for (int64_t i = tid; i < p.rows; i += kSortThreads * kSortAhead) {
+    int64_t t[kSortAhead];
+#pragma unroll
+    for (int j = 0; j < kSortAhead; ++j) {
+      const int64_t at = i + j * kSortThreads;
+      t[j] = at < p.rows ? p.tokens[p.trow.at((int)at)] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kSortAhead; ++j)
+      if (t[j] >= 0 && t[j] < p.vocab) atomicOr(&seen[t[j] >> 5], 1u << (t[j] & 31));
+  }
+  __syncthreads();
+  const bool wide = ((uintptr_t)p.clear | (uint64_t)p.ld_bytes | (uint64_t)p.row_bytes) % 16 == 0;
+  for (int64_t v = (int64_t)cta * kSortWarps + warp; v < p.vocab; v += (int64_t)ctas * kSortWarps) {
+    if (seen[v >> 5] >> (v & 31) & 1u) continue;
+    unsigned char* g = p.clear + v * p.ld_bytes;
+    if (wide) {
+      for (int64_t b = lane * 16; b < p.row_bytes; b += 512) *reinterpret_cast<uint4*>(g + b) = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      for (int64_t b = lane * 2; b < p.row_bytes; b += 64) *reinterpret_cast<uint16_t*>(g + b) = 0;
+    }
+  }
+}
+
 // Each of the cluster's 256 warps owns a contiguous piece of the input; positions are handed out
 // digit by digit, then CTA by CTA, warp by warp and lane by lane, so equal digits keep their order.
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
@@ -132,6 +201,10 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
+  if (blockIdx.x >= kSortCtas) {
+    clear_absent(p, reinterpret_cast<uint32_t*>(smem_raw), blockIdx.x - kSortCtas, gridDim.x - kSortCtas);
+    return;
+  }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
   const int bins = 1 << p.bits;
   const unsigned lt = (1u << lane) - 1u;
@@ -144,22 +217,34 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
     int64_t i0 = (int64_t)(rank * kSortWarps + warp) * piece, i1 = i0 + piece;
     if (i0 > n) i0 = n;
     if (i1 > n) i1 = n;
-    // the first pass reads the tokens and leaves out those outside the table
-    auto fetch = [&](int64_t i, uint2& e) -> bool {
-      if (i >= i1) return false;
+    // the first pass reads the tokens and leaves out those outside the table (their token becomes -1)
+    auto fetch = [&](int64_t i, uint2(&e)[kSortAhead]) {
       if (pass > 0) {
-        e = __ldcg(src + i);
-        return true;
+#pragma unroll
+        for (int j = 0; j < kSortAhead; ++j) {
+          const int64_t at = i + 32 * j + lane;
+          e[j] = at < i1 ? __ldcg(src + at) : make_uint2(~0u, 0u);
+        }
+      } else {
+        int64_t t[kSortAhead];
+#pragma unroll
+        for (int j = 0; j < kSortAhead; ++j) {
+          const int64_t at = i + 32 * j + lane;
+          t[j] = at < i1 ? p.tokens[p.trow.at((int)at)] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < kSortAhead; ++j)
+          e[j] = make_uint2(t[j] >= 0 && t[j] < p.vocab ? (uint32_t)t[j] : ~0u, (uint32_t)(i + 32 * j + lane));
       }
-      const int64_t t = p.tokens[p.trow.at((int)i)];
-      e = make_uint2((uint32_t)t, (uint32_t)i);
-      return t >= 0 && t < p.vocab;
     };
     for (int b = lane; b < bins; b += 32) s.hist[warp][b] = 0;
     __syncwarp();
-    for (int64_t i = i0; i < i1; i += 32) {
-      uint2 e;
-      if (fetch(i + lane, e)) atomicAdd(&s.hist[warp][(e.x >> shift) & (bins - 1)], 1);
+    for (int64_t i = i0; i < i1; i += 32 * kSortAhead) {
+      uint2 e[kSortAhead];
+      fetch(i, e);
+#pragma unroll
+      for (int j = 0; j < kSortAhead; ++j)
+        if (e[j].x != ~0u) atomicAdd(&s.hist[warp][(e[j].x >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
     if (tid < bins) {
@@ -195,17 +280,21 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
     if (tid < bins)
       for (int w = 0; w < kSortWarps; ++w) s.hist[w][tid] += start + before;
     __syncthreads();
-    for (int64_t i = i0; i < i1; i += 32) {
-      uint2 e = make_uint2(0u, 0u);
-      const bool in = fetch(i + lane, e);
-      const int d = in ? (int)((e.x >> shift) & (bins - 1)) : bins;
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      int at = 0;
-      if (in) at = s.hist[warp][d] + __popc(same & lt);
-      __syncwarp();
-      if (in && (same & lt) == 0u) s.hist[warp][d] += __popc(same);
-      __syncwarp();
-      if (in) dst[at] = e;
+    for (int64_t i = i0; i < i1; i += 32 * kSortAhead) {
+      uint2 e[kSortAhead];
+      fetch(i, e);
+#pragma unroll
+      for (int j = 0; j < kSortAhead; ++j) {
+        const bool in = e[j].x != ~0u;
+        const int d = in ? (int)((e[j].x >> shift) & (bins - 1)) : bins;
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        int at = 0;
+        if (in) at = s.hist[warp][d] + __popc(same & lt);
+        __syncwarp();
+        if (in && (same & lt) == 0u) s.hist[warp][d] += __popc(same);
+        __syncwarp();
+        if (in) dst[at] = e[j];
+      }
     }
     n = sum;
     __threadfence();
@@ -216,11 +305,12 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
 
 // ---- row sums -----------------------------------------------------------------------------
 // Chunk k holds the sorted entries [k C, (k + 1) C).  A group walks its chunk and writes the rows of the
-// tokens that lie within it; of a token that goes on past an end it writes its piece to `parts`: slot 2 k
-// for one that began before the chunk, 2 k + 1 for one that begins in it.
+// tokens that begin in it, reading on where the last one ends within the next chunk (whose group then
+// leaves those entries out).  Of a longer token every chunk writes a piece to `parts`: slot 2 k + 1 where it
+// begins, 2 k in the others.
 struct SumParams {
   int64_t grad_ld;
-  int dim, chunk, vocab, accumulate, sum_ctas;
+  int dim, chunk, vocab, accumulate, clear, sum_ctas;  // clear: rows of absent tokens are still to be cleared
   float scale;
   Rows drow;
   const uint2* sorted;
@@ -257,6 +347,11 @@ __device__ __forceinline__ int lower_bound(const uint2* a, int n, uint32_t key) 
   return lo;
 }
 
+// The token, which occurs before position b, does not occur from b on.
+__device__ __forceinline__ bool ends_by(const uint2* a, int n, int64_t b, uint32_t token) {
+  return b >= n || a[b].x != token;
+}
+
 constexpr int kAhead = 8;  // entries in flight
 
 template <typename D, typename G, int N>
@@ -288,80 +383,123 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const SumParams p) {
   if (g >= p.cols.groups || c >= p.dim) return;
   const int64_t k = (int64_t)blockIdx.x * p.cols.groups + g, b0 = k * p.chunk;
   if (b0 >= n) return;
-  const int i0 = (int)b0, i1 = (int)min((int64_t)n, b0 + p.chunk);
+  const uint2* so = p.sorted;
+  int i0 = (int)b0, i1 = (int)min((int64_t)n, b0 + p.chunk);
   const D* dy = reinterpret_cast<const D*>(p.dy) + c;
-  uint32_t token = p.sorted[i0].x;
-  bool began = i0 > 0 && p.sorted[i0 - 1].x == token;  // the current token's entries began before the chunk
+  const uint32_t last = so[i1 - 1].x;
+  uint32_t token = so[i0].x;
+  bool began = i0 > 0 && so[i0 - 1].x == token;  // the current token's entries began before the chunk
+  bool goes_on = i1 < n && so[i1].x == last;
+  if (goes_on && !(began && last == token) && ends_by(so, n, b0 + 2 * p.chunk, last)) {
+    i1 += lower_bound(so + i1, min(p.chunk, n - i1), last + 1u);
+    goes_on = false;
+  }
+  if (began && (i0 == p.chunk || so[i0 - p.chunk - 1].x != token) && ends_by(so, n, b0 + p.chunk, token)) {
+    i0 += lower_bound(so + i0, min(p.chunk, n - i0), token + 1u);
+    if (i0 >= i1) return;
+    token = so[i0].x;
+    began = false;
+  }
   float acc[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) acc[j] = 0.f;
+  uint2 e[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) e[j] = so[min(i0 + j, i1 - 1)];
   for (int i = i0; i < i1; i += kAhead) {
-    uint2 e[kAhead];
-    float v[kAhead][N];
+    Raw<N, D> v[kAhead];
+    uint32_t t[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) e[j] = p.sorted[min(i + j, i1 - 1)];
+    for (int j = 0; j < kAhead; ++j) {
+      v[j].load(dy + p.drow.at((int)e[j].y));
+      t[j] = e[j].x;
+    }
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (i + j < i1) load_n<N>(dy + p.drow.at((int)e[j].y), v[j]);
+    for (int j = 0; j < kAhead; ++j) e[j] = so[min(i + kAhead + j, i1 - 1)];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (i + j < i1) {
-        if (e[j].x != token) {
-          if (began)
-            store_n<N>(p.parts + 2 * k * p.dim + c, acc);
-          else
-            write_row<N, G>(p, token, c, acc);
-          token = e[j].x;
-          began = false;
+    for (int j = 0; j < kAhead; ++j) {
+      if (i + j >= i1) break;
+      if (t[j] != token) {
+        if (began)
+          store_n<N>(p.parts + 2 * k * p.dim + c, acc);
+        else
+          write_row<N, G>(p, token, c, acc);
+        token = t[j];
+        began = false;
 #pragma unroll
-          for (int q = 0; q < N; ++q) acc[q] = 0.f;
-        }
-#pragma unroll
-        for (int q = 0; q < N; ++q) acc[q] += v[j][q];
+        for (int q = 0; q < N; ++q) acc[q] = 0.f;
       }
+      float f[N];
+      v[j].get(f);
+#pragma unroll
+      for (int q = 0; q < N; ++q) acc[q] += f[q];
+    }
   }
-  const bool goes_on = i1 < n && p.sorted[i1].x == token;
   if (began || goes_on)
     store_n<N>(p.parts + (2 * k + (began ? 0 : 1)) * p.dim + c, acc);
   else
     write_row<N, G>(p, token, c, acc);
 }
 
-// Joins the pieces of the tokens that cross a cut, one CTA per chunk in which such a token begins: its
-// groups take the pieces in turn, and their sums meet in a fixed order.
+// Joins the pieces of the long tokens.  A CTA looks at kJoinChunks chunks for tokens that begin in one and
+// go on past the next, and takes kJoinWidth threads' columns of them: its groups sum the pieces in
+// turn (a chunk whose first entry is still the token holds one), and their sums meet in a fixed order.
+constexpr int kJoinWidth = 8, kJoinChunks = 8, kJoinAhead = 4;
+
 template <typename G, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(const SumParams p) {
-  __shared__ float sums[kThreads * N];
-  const int n = *p.count;
-  const int64_t k = blockIdx.x, b1 = (k + 1) * p.chunk;
-  if (b1 >= n) return;
-  const uint32_t token = p.sorted[b1 - 1].x;
-  if (p.sorted[b1].x != token) return;                                    // nothing goes on here
-  if (k > 0 && p.sorted[b1 - p.chunk - 1].x == token) return;             // it began in an earlier chunk
-  const int last = (lower_bound(p.sorted, n, token + 1u) - 1) / p.chunk;  // the chunk in which it ends
-  const int g = p.cols.group(), c = p.cols.first(N);
-  const bool live = g < p.cols.groups && c < p.dim;
-  float acc[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) acc[j] = 0.f;
-  if (live) {
-    if (g == 0) load_n<N>(p.parts + (2 * k + 1) * p.dim + c, acc);
-#pragma unroll 4
-    for (int64_t q = k + 1 + g; q <= last; q += p.cols.groups) {
-      float v[N];
-      load_n<N>(p.parts + 2 * q * p.dim + c, v);
-#pragma unroll
-      for (int j = 0; j < N; ++j) acc[j] += v[j];
-    }
+  constexpr int kGroups = kThreads / kJoinWidth;
+  __shared__ float sums[kGroups][kJoinWidth * N];
+  const int n = *p.count, lane = threadIdx.x & 31;
+  const int64_t k = (int64_t)blockIdx.x * kJoinChunks + lane, b1 = (k + 1) * p.chunk;
+  bool goes_on = false;
+  uint32_t token_at = 0;
+  if (lane < kJoinChunks && b1 < n) {
+    token_at = p.sorted[b1 - 1].x;
+    goes_on = p.sorted[b1].x == token_at && !(k > 0 && p.sorted[b1 - p.chunk - 1].x == token_at) &&
+              !ends_by(p.sorted, n, b1 + p.chunk, token_at);
   }
+  const int g = threadIdx.x / kJoinWidth, w = threadIdx.x % kJoinWidth;
+  const int c = (blockIdx.y * kJoinWidth + w) * N;
+  for (unsigned m = __ballot_sync(0xffffffffu, goes_on); m; m &= m - 1) {  // the same in every warp
+    const int64_t first = (int64_t)blockIdx.x * kJoinChunks + __ffs(m) - 1;
+    const uint32_t token = __shfl_sync(0xffffffffu, token_at, __ffs(m) - 1);
+    float acc[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) sums[threadIdx.x * N + j] = acc[j];
-  __syncthreads();
-  if (!live || g > 0) return;
-  for (int h = 1; h < p.cols.groups; ++h)
+    for (int j = 0; j < N; ++j) acc[j] = 0.f;
+    if (c < p.dim) {
+      if (g == 0) load_n<N>(p.parts + (2 * first + 1) * p.dim + c, acc);
+      bool more = true;
+      for (int64_t q = first + 1 + g; more; q += kGroups * kJoinAhead) {
+        Raw<N, float> v[kJoinAhead];
+        uint32_t t[kJoinAhead];
 #pragma unroll
-    for (int j = 0; j < N; ++j) acc[j] += sums[(threadIdx.x + h * p.cols.width) * N + j];
-  write_row<N, G>(p, token, c, acc);
+        for (int j = 0; j < kJoinAhead; ++j) {
+          const int64_t at = q + j * kGroups, b = at * p.chunk;
+          t[j] = b < n ? p.sorted[b].x : ~0u;
+          v[j].load(p.parts + 2 * (b < n ? at : first) * p.dim + c);
+        }
+#pragma unroll
+        for (int j = 0; j < kJoinAhead; ++j) {
+          more = more && t[j] == token;
+          float f[N];
+          v[j].get(f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] += more ? f[i] : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) sums[g][w * N + j] = acc[j];
+    __syncthreads();
+    if (g == 0 && c < p.dim) {
+      for (int h = 1; h < kGroups; ++h)
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += sums[h][w * N + j];
+      write_row<N, G>(p, token, c, acc);
+    }
+    __syncthreads();
+  }
 }
 
 size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -371,6 +509,33 @@ int sm_count() {
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
   return c;
+}
+
+// How many of the sort's clusters run at once on this device (they do not tile its SMs), after
+// allowing the kernel its shared memory; 0 on an error.
+int sort_clusters() {
+  static int found[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && found[dev]) return found[dev];
+  if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortSmem)) !=
+      cudaSuccess)
+    return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSortCtas, 1, 1);
+  cfg.blockDim = dim3(kSortThreads, 1, 1);
+  cfg.dynamicSmemBytes = sizeof(SortSmem);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = kSortCtas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, sort_kernel, &cfg) != cudaSuccess) return 0;
+  if (n < 1) n = 1;
+  if (dev < 64) found[dev] = n;
+  return n;
 }
 
 bool dtype_ok(int d) { return d == M3_DTYPE_F32 || d == M3_DTYPE_BF16; }
@@ -383,13 +548,15 @@ int slabs(int dim, int n, const Columns& c) { return (dim + n * c.width - 1) / (
 
 // Whether rows of `size`-byte elements (base and strides) allow N elements at a time.
 bool whole(const void* p, int size, int n, int dim, int64_t s0, int64_t s1) {
-  const int bytes = size * n < 16 ? size * n : 16, e = bytes / size;
-  return dim % n == 0 && ((uintptr_t)p) % bytes == 0 && s0 % e == 0 && s1 % e == 0;
+  return dim % n == 0 && ((uintptr_t)p) % (size * n) == 0 && s0 % n == 0 && s1 % n == 0;
 }
 
 template <typename T, typename O, int N>
 void launch_embed(FwdParams p, cudaStream_t s) {
   p.cols = columns(p.dim, N);
+  // a small table's columns are cut so that a CTA's share of it stays in L1
+  const int keep = (128 << 10) / (int)(p.vocab < 4096 ? p.vocab * (int)sizeof(T) * N : 1 << 30);
+  if (keep >= 8 && keep < p.cols.width && p.rows > 8 * (int64_t)p.vocab) p.cols = Columns{keep / 8 * 8, kThreads / (keep / 8 * 8)};
   const int y = slabs(p.dim, N, p.cols);
   const int64_t want = (p.rows + p.cols.groups - 1) / p.cols.groups, most = (int64_t)sm_count() * 8;
   embed_kernel<T, O, N><<<dim3((unsigned)(want < most ? want : most), y), kThreads, 0, s>>>(p);
@@ -421,9 +588,11 @@ void launch_sum(SumParams p, int64_t rows, cudaStream_t s) {
   const int64_t chunks = (rows + p.chunk - 1) / p.chunk;
   p.sum_ctas = (int)((chunks + p.cols.groups - 1) / p.cols.groups);
   const int64_t want = (p.vocab + 32 * (kThreads / 32) - 1) / (32 * (kThreads / 32)), most = (int64_t)sm_count() * 8;
-  const int64_t clear = p.accumulate ? 0 : want < most ? want : most;
+  const int64_t clear = !p.clear ? 0 : want < most ? want : most;
   if (p.sum_ctas + clear > 0) sum_kernel<D, G, N><<<dim3((unsigned)(p.sum_ctas + clear), y), kThreads, 0, s>>>(p);
-  if (chunks > 1) join_kernel<G, N><<<dim3((unsigned)(chunks - 1), y), kThreads, 0, s>>>(p);
+  if (chunks > 1)
+    join_kernel<G, N><<<dim3((unsigned)((chunks + kJoinChunks - 2) / kJoinChunks), (p.dim + N * kJoinWidth - 1) / (N * kJoinWidth)), kThreads,
+                        0, s>>>(p);
 }
 
 template <typename D, typename G>
@@ -505,21 +674,24 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   sp.count = (int*)ws;
   sp.buf[0] = (uint2*)(ws + 256);
   sp.buf[1] = (uint2*)(ws + 256 + align256((size_t)rows * sizeof(uint2)));
-  static bool attr[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 64 || !attr[dev]) {
-    if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortSmem)) !=
-        cudaSuccess)
-      return check_launch("m3_embed_bwd: cudaFuncSetAttribute");
-    if (dev < 64) attr[dev] = true;
-  }
-  sort_kernel<<<kSortCtas, kSortThreads, sizeof(SortSmem), s>>>(sp);
+  const int clusters = sort_clusters();
+  if (clusters <= 0) return check_launch("m3_embed_bwd: sort_kernel attributes");
+  // Rows of absent tokens are cleared beside the sort by CTAs that each read all tokens; where that is
+  // more to read than there is to clear, or the bitmap does not fit, the sums' launch looks them up.
+  const int64_t row_bytes = (int64_t)a.dim * (int64_t)gs, all_bytes = row_bytes * a.vocab;
+  int64_t ctas = (int64_t)(clusters - 1) * kSortCtas;
+  if (ctas > all_bytes >> 17) ctas = (all_bytes >> 17) / kSortCtas * kSortCtas;  // at least 128 KB each
+  const bool beside = !a.accumulate && ctas > 0 && ctas * rows * 8 <= all_bytes / 2 && a.vocab <= (int)sizeof(SortSmem) * 8;
+  sp.clear = beside ? (unsigned char*)a.grad : nullptr;
+  sp.row_bytes = row_bytes;
+  sp.ld_bytes = a.grad_ld * (int64_t)gs;
+  sort_kernel<<<kSortCtas + (beside ? (unsigned)ctas : 0u), kSortThreads, sizeof(SortSmem), s>>>(sp);
   const SumParams p{a.grad_ld,
                     a.dim,
                     chunk_of(rows, a.dim),
                     a.vocab,
                     a.accumulate,
+                    !a.accumulate && !beside,
                     0,
                     a.scale,
                     Rows{a.rows_inner, a.dy_outer, a.dy_inner},
