@@ -605,8 +605,8 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
   p.hard = a.hard_weight;
   p.scale = a.grad_scale;
   if (a.reduction == M3_REDUCE_MEAN && !a.weights) p.scale /= (float)rows;
-  p.lrow = Rows{a.rows_inner, a.ld_outer, a.ld_inner};
-  p.grow = Rows{a.rows_inner, a.g_outer, a.g_inner};
+  p.lrow = Rows{a.rows_outer, a.rows_inner, a.ld_outer, a.ld_inner};
+  p.grow = Rows{a.rows_outer, a.rows_inner, a.g_outer, a.g_inner};
   p.logits = a.logits;
   p.grad = a.grad;
   p.ids = a.ids;

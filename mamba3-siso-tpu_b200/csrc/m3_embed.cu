@@ -15,6 +15,7 @@ namespace {
 using vocab::Rows;
 
 constexpr int kThreads = 256;
+constexpr int64_t kMaxLd = 1 << 30;  // elements between rows of a table
 
 // The threads of a CTA as groups over a row's columns, N columns a thread: at most kThreads threads a
 // group, wider rows take several CTAs (blockIdx.y).
@@ -28,8 +29,7 @@ struct Columns {
 
 // ---- lookup -------------------------------------------------------------------------------
 struct FwdParams {
-  int64_t rows, table_ld, out_ld;
-  int vocab, dim;
+  int rows, vocab, dim, table_ld, out_ld;  // 32-bit strides: one multiplication per address
   float scale;
   Rows trow;
   const int64_t* tokens;
@@ -114,30 +114,37 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const FwdParams p) {
   if (g >= p.cols.groups || c >= p.dim) return;
   const T* table = reinterpret_cast<const T*>(p.table) + c;
   O* out = reinterpret_cast<O*>(p.out) + c;
-  const int64_t step = (int64_t)gridDim.x * p.cols.groups, start = (int64_t)blockIdx.x * p.cols.groups + g;
-  int64_t next[kRows];
-  auto fetch = [&](int64_t r0) {
+  const int step = gridDim.x * p.cols.groups, start = blockIdx.x * p.cols.groups + g;
+  int next[kRows];  // table rows; -1: padding, -2: past the table
+  auto fetch = [&](int r0) {
+    int64_t t[kRows];
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) next[j] = r0 + j * step < p.rows ? p.tokens[p.trow.at((int)(r0 + j * step))] : -1;
+    for (int j = 0; j < kRows; ++j) t[j] = r0 + j * step < p.rows ? p.tokens[p.trow.at(r0 + j * step)] : -1;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) next[j] = t[j] < 0 ? -1 : t[j] < p.vocab ? (int)t[j] : -2;
   };
   fetch(start);
-  for (int64_t r0 = start; r0 < p.rows; r0 += step * kRows) {
-    int64_t t[kRows];
+  for (int r0 = start; r0 < p.rows; r0 += step * kRows) {
+    int t[kRows];
     Raw<N, T> v[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) t[j] = next[j];
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) v[j].load(table + (t[j] >= 0 && t[j] < p.vocab ? t[j] : 0) * p.table_ld);
+    for (int j = 0; j < kRows; ++j) v[j].load(table + (int64_t)max(t[j], 0) * p.table_ld);
     fetch(r0 + step * kRows);
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
       if (r0 + j * step < p.rows) {
         float f[N];
-        v[j].get(f);
-        const float none = t[j] < 0 ? 0.f : NAN;
+        if (t[j] >= 0) {
+          v[j].get(f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = t[j] >= 0 && t[j] < p.vocab ? f[i] * p.scale : none;
-        store_n<N>(out + (r0 + j * step) * p.out_ld, f);
+          for (int i = 0; i < N; ++i) f[i] *= p.scale;
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) f[i] = t[j] == -1 ? 0.f : NAN;
+        }
+        store_n<N>(out + (int64_t)(r0 + j * step) * p.out_ld, f);
       }
   }
 }
@@ -286,8 +293,13 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
 #pragma unroll
       for (int j = 0; j < kSortAhead; ++j) {
         const bool in = e[j].x != ~0u;
-        const int d = in ? (int)((e[j].x >> shift) & (bins - 1)) : bins;
-        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const int d = (int)((e[j].x >> shift) & (bins - 1));
+        // the lanes with the same digit, by its bits (a match instruction took twice the kernel's time)
+        unsigned same = __ballot_sync(0xffffffffu, in);
+        for (int b = 0; b < p.bits; ++b) {
+          const unsigned ones = __ballot_sync(0xffffffffu, (d >> b) & 1);
+          same &= (d >> b) & 1 ? ones : ~ones;
+        }
         int at = 0;
         if (in) at = s.hist[warp][d] + __popc(same & lt);
         __syncwarp();
@@ -309,8 +321,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
 // leaves those entries out).  Of a longer token every chunk writes a piece to `parts`: slot 2 k + 1 where it
 // begins, 2 k in the others.
 struct SumParams {
-  int64_t grad_ld;
-  int dim, chunk, vocab, accumulate, clear, sum_ctas;  // clear: rows of absent tokens are still to be cleared
+  int grad_ld, dim, chunk, vocab, accumulate, clear, sum_ctas;  // clear: rows of absent tokens are still to be cleared
   float scale;
   Rows drow;
   const uint2* sorted;
@@ -444,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) sum_kernel(const SumParams p) {
 // Joins the pieces of the long tokens.  A CTA looks at kJoinChunks chunks for tokens that begin in one and
 // go on past the next, and takes kJoinWidth threads' columns of them: its groups sum the pieces in
 // turn (a chunk whose first entry is still the token holds one), and their sums meet in a fixed order.
-constexpr int kJoinWidth = 8, kJoinChunks = 8, kJoinAhead = 4;
+constexpr int kJoinWidth = 8, kJoinChunks = 16, kJoinAhead = 4;
 
 template <typename G, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(const SumParams p) {
@@ -558,7 +569,7 @@ void launch_embed(FwdParams p, cudaStream_t s) {
   const int keep = (128 << 10) / (int)(p.vocab < 4096 ? p.vocab * (int)sizeof(T) * N : 1 << 30);
   if (keep >= 8 && keep < p.cols.width && p.rows > 8 * (int64_t)p.vocab) p.cols = Columns{keep / 8 * 8, kThreads / (keep / 8 * 8)};
   const int y = slabs(p.dim, N, p.cols);
-  const int64_t want = (p.rows + p.cols.groups - 1) / p.cols.groups, most = (int64_t)sm_count() * 8;
+  const int want = (p.rows + p.cols.groups - 1) / p.cols.groups, most = sm_count() * 8;
   embed_kernel<T, O, N><<<dim3((unsigned)(want < most ? want : most), y), kThreads, 0, s>>>(p);
 }
 
@@ -621,12 +632,21 @@ extern "C" int m3_embed(const M3EmbedArgs* args, void* stream) {
   if (rows > vocab::kMaxRows) return set_error(M3_ERR_SHAPE, "m3_embed: more than 2^30 rows");
   if (rows == 0) return M3_OK;
   if (!a.tokens || !a.table || !a.out) return set_error(M3_ERR_ARG, "m3_embed: NULL pointer");
-  if (a.table_ld < a.dim || a.out_ld < a.dim) return set_error(M3_ERR_SHAPE, "m3_embed: bad leading dimension");
+  if (a.table_ld < a.dim || a.out_ld < a.dim || a.table_ld > kMaxLd || a.out_ld > kMaxLd) return set_error(M3_ERR_SHAPE, "m3_embed: bad leading dimension");
   const size_t ts = a.table_dtype == M3_DTYPE_BF16 ? 2 : 4, os = a.out_dtype == M3_DTYPE_BF16 ? 2 : 4;
   if (((uintptr_t)a.table) % ts || ((uintptr_t)a.out) % os)
     return set_error(M3_ERR_ARG, "m3_embed: table and out must be aligned to their types");
-  const FwdParams p{rows,     a.table_ld, a.out_ld, a.vocab,  a.dim, a.scale, Rows{a.rows_inner, a.t_outer, a.t_inner},
-                    a.tokens, a.table,    a.out,    Columns{}};
+  const FwdParams p{(int)rows,
+                    a.vocab,
+                    a.dim,
+                    (int)a.table_ld,
+                    (int)a.out_ld,
+                    a.scale,
+                    Rows{a.rows_outer, a.rows_inner, a.t_outer, a.t_inner},
+                    a.tokens,
+                    a.table,
+                    a.out,
+                    Columns{}};
   cudaStream_t s = (cudaStream_t)stream;
   using bf16 = __nv_bfloat16;
   if (ts == 2)
@@ -652,7 +672,7 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
   if (rows > vocab::kMaxRows) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: more than 2^30 rows");
   if (!a.grad || (rows > 0 && (!a.tokens || !a.dy))) return set_error(M3_ERR_ARG, "m3_embed_bwd: NULL pointer");
-  if (a.grad_ld < a.dim) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: bad leading dimension");
+  if (a.grad_ld < a.dim || a.grad_ld > kMaxLd) return set_error(M3_ERR_SHAPE, "m3_embed_bwd: bad leading dimension");
   const size_t ds = a.dy_dtype == M3_DTYPE_BF16 ? 2 : 4, gs = a.grad_dtype == M3_DTYPE_BF16 ? 2 : 4;
   if (((uintptr_t)a.dy) % ds || ((uintptr_t)a.grad) % gs)
     return set_error(M3_ERR_ARG, "m3_embed_bwd: dy and grad must be aligned to their types");
@@ -669,7 +689,7 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   sp.vocab = a.vocab;
   sp.passes = (bits_all + kMaxBits - 1) / kMaxBits;
   sp.bits = (bits_all + sp.passes - 1) / sp.passes;
-  sp.trow = Rows{a.rows_inner, a.t_outer, a.t_inner};
+  sp.trow = Rows{a.rows_outer, a.rows_inner, a.t_outer, a.t_inner};
   sp.tokens = a.tokens;
   sp.count = (int*)ws;
   sp.buf[0] = (uint2*)(ws + 256);
@@ -686,7 +706,7 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   sp.row_bytes = row_bytes;
   sp.ld_bytes = a.grad_ld * (int64_t)gs;
   sort_kernel<<<kSortCtas + (beside ? (unsigned)ctas : 0u), kSortThreads, sizeof(SortSmem), s>>>(sp);
-  const SumParams p{a.grad_ld,
+  const SumParams p{(int)a.grad_ld,
                     a.dim,
                     chunk_of(rows, a.dim),
                     a.vocab,
@@ -694,7 +714,7 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
                     !a.accumulate && !beside,
                     0,
                     a.scale,
-                    Rows{a.rows_inner, a.dy_outer, a.dy_inner},
+                    Rows{a.rows_outer, a.rows_inner, a.dy_outer, a.dy_inner},
                     sp.buf[(sp.passes - 1) & 1],
                     sp.count,
                     a.dy,

@@ -521,8 +521,8 @@ extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
   p.cluster = 1;
   p.log2_cluster = 0;
   p.inv_t = 1.f / a.temperature;
-  p.lrow = Rows{a.rows_inner, a.ld_outer, a.ld_inner};
-  p.trow = Rows{a.rows_inner, a.t_outer, a.t_inner};
+  p.lrow = Rows{a.rows_outer, a.rows_inner, a.ld_outer, a.ld_inner};
+  p.trow = Rows{a.rows_outer, a.rows_inner, a.t_outer, a.t_inner};
   p.logits = a.logits;
   p.targets = a.targets;
   p.logprob = a.logprob;

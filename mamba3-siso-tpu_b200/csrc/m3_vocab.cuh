@@ -35,13 +35,17 @@ struct Divider {
 };
 
 // Element offset of row r = (r / inner) * outer_stride + (r % inner) * inner_stride.  (A 64-bit
-// division by every thread cost as much as 20 logits each.)
+// division by every thread cost as much as 20 logits each.)  `flat`: one stride does for all rows.
 struct Rows {
   Divider inner;
+  bool flat;
   int64_t outer_stride, inner_stride;
   Rows() = default;
-  Rows(int n, int64_t outer, int64_t in) : inner(n > 0 ? n : 1), outer_stride(outer), inner_stride(in) {}
+  Rows(int n_outer, int n, int64_t outer, int64_t in)
+      : inner(n > 0 ? n : 1), flat(n_outer <= 1 || outer == n * in || n <= 1), outer_stride(outer),
+        inner_stride(n <= 1 ? outer : in) {}
   __device__ __forceinline__ int64_t at(int r) const {
+    if (flat) return r * inner_stride;
     const int o = inner.div(r);
     return o * outer_stride + (r - o * inner.d) * inner_stride;
   }
