@@ -102,11 +102,16 @@ def rows2(t, nd):
     the last).  None if the outer ones do not collapse into one stride."""
     if nd == 0:
         return 0, 0
-    outer = [(s, st) for s, st in zip(t.shape[:nd - 1], t.stride()) if s != 1]
+    st = t.stride()
+    if nd == 1:
+        return 0, st[0]
+    if nd == 2:
+        return st[0], st[1]
+    outer = [ss for ss in zip(t.shape[:nd - 1], st) if ss[0] != 1]
     for (_, st0), (s1, st1) in zip(outer, outer[1:]):
         if st0 != s1 * st1:
             return None
-    return (outer[-1][1] if outer else 0), t.stride(nd - 1)
+    return (outer[-1][1] if outer else 0), st[nd - 1]
 
 
 def row_input(t, nd):
@@ -114,7 +119,7 @@ def row_input(t, nd):
     leading axes addressable by two strides, copied only where it is not, and those strides."""
     st = rows2(t, nd) if t.dim() == nd or t.stride(-1) == 1 or t.shape[-1] == 1 else None
     if st is None:
-        t = t.contiguous()
+        t = t.detach().contiguous()
         st = rows2(t, nd)
     return t, st
 
@@ -130,10 +135,25 @@ def row_counts(lead):
     return (outer, inner) if inner else (0, 1)
 
 
+def require_here(device, *ts):
+    """Every given tensor is on the CUDA device ``device``."""
+    if device.type != "cuda":
+        raise ValueError("the Mamba-3 SISO kernels run on CUDA tensors only (no CPU path)")
+    for t in ts:
+        if t is not None and t.device != device:
+            raise ValueError(f"every tensor must be on {device}, got one on {t.device}")
+
+
+# the public torch.cuda.current_stream builds a Stream object per call, a tenth of a small call's cost
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def call(fn, args, device):
     """One library call on the current stream of ``device``; raises on a non-zero status."""
-    if device.index is not None and device.index != torch.cuda.current_device():
+    if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            C.check(fn(args, stream_handle(device)))
+            rc = fn(args, stream_handle(device))
     else:
-        C.check(fn(args, stream_handle(device)))
+        rc = fn(args, _raw_stream(device.index) if _raw_stream else stream_handle(device))
+    if rc:
+        C.check(rc)

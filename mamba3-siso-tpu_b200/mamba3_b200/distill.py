@@ -21,41 +21,49 @@ from . import _tensors as T
 _REDUCE = {"none": C.M3_REDUCE_NONE, "sum": C.M3_REDUCE_SUM, "mean": C.M3_REDUCE_MEAN}
 
 
+def _side(name, t, shape, dtype, others):
+    """A side input as the kernel reads it: dense, int64 or f32."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        if not others(t.dtype):
+            raise ValueError(f"{name} must be {'integers' if dtype == torch.int64 else 'floating point'}, got {t.dtype}")
+        t = t.detach().to(dtype)
+    return t if t.is_contiguous() else t.detach().contiguous()
+
+
+def _is_int(dt):
+    return dt == torch.int32
+
+
+def _is_float(dt):
+    return dt.is_floating_point
+
+
 def _check(logits, ids, teacher, labels, weights, temperature, hard_weight, reduction):
     """Argument checks; returns the side inputs as the kernel reads them (dense int64 / f32)."""
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be (..., vocab), got {tuple(logits.shape)}")
-    T.require_cuda(logits, ids, teacher, labels, weights)
-    T.io_dtype(logits.dtype)
-    lead = logits.shape[:-1]
-    if ids.dim() != len(lead) + 1 or ids.shape[:-1] != lead or not 1 <= ids.shape[-1] <= C.M3_MAX_TOP:
+    shape = logits.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"logits must be (..., vocab), got {tuple(shape)}")
+    T.require_here(logits.device, ids, teacher, labels, weights)
+    lead = shape[:-1]
+    k = ids.shape[-1] if ids.dim() else 0
+    if not 1 <= k <= C.M3_MAX_TOP:
         raise ValueError(f"teacher_ids must be {tuple(lead)} + (k,), 1 <= k <= {C.M3_MAX_TOP}, got {tuple(ids.shape)}")
-    if teacher.shape != ids.shape:
-        raise ValueError(f"teacher_logits must have the shape of teacher_ids, got {tuple(teacher.shape)}")
     if not temperature > 0 or not 0 <= hard_weight <= 1:
         raise ValueError("need temperature > 0 and 0 <= hard_weight <= 1")
     if reduction not in _REDUCE:
         raise ValueError(f"reduction must be one of {sorted(_REDUCE)}, got {reduction!r}")
     if (labels is not None) != (hard_weight > 0):
         raise ValueError("labels go with hard_weight > 0")
-    for name, t in (("labels", labels), ("weights", weights)):
-        if t is not None and t.shape != lead:
-            raise ValueError(f"{name} must be {tuple(lead)}, got {tuple(t.shape)}")
-    for name, t in (("teacher_ids", ids), ("labels", labels)):
-        if t is not None and t.dtype not in (torch.int64, torch.int32):
-            raise ValueError(f"{name} must be int64 or int32, got {t.dtype}")
-    for name, t in (("teacher_logits", teacher), ("weights", weights)):
-        if t is not None and not t.dtype.is_floating_point:
-            raise ValueError(f"{name} must be floating point, got {t.dtype}")
-    for t in (ids, teacher, labels, weights):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"every tensor must be on {logits.device}, got one on {t.device}")
-
-    def dense(t, dtype):
-        return None if t is None else t.detach().to(dtype).contiguous()
-
-    return dense(ids, torch.int64), dense(teacher, torch.float32), dense(labels, torch.int64), dense(
-        weights, torch.float32)
+    entries = (*lead, k)
+    ids = _side("teacher_ids", ids, entries, torch.int64, _is_int)
+    teacher = _side("teacher_logits", teacher, entries, torch.float32, _is_float)
+    if labels is not None:
+        labels = _side("labels", labels, lead, torch.int64, _is_int)
+    if weights is not None:
+        weights = _side("weights", weights, lead, torch.float32, _is_float)
+    return ids, teacher, labels, weights
 
 
 def _run(logits, ids, teacher, labels, weights, temperature, hard_weight, reduction, grad=None, upstream=None,
@@ -63,28 +71,24 @@ def _run(logits, ids, teacher, labels, weights, temperature, hard_weight, reduct
     """One m3_distill call on checked inputs: the reduced loss, or the rows' losses."""
     lead, dev = logits.shape[:-1], logits.device
     nd = len(lead)
-    a = C.M3DistillArgs()
-    a.rows_outer, a.rows_inner = T.row_counts(lead)
-    a.vocab, a.k = logits.shape[-1], ids.shape[-1]
-    a.logits_dtype, a.reduction = T.io_dtype(logits.dtype), _REDUCE[reduction]
-    a.temperature, a.hard_weight, a.grad_scale = temperature, hard_weight, grad_scale
-    logits, (a.ld_outer, a.ld_inner) = T.row_input(logits, nd)
-    a.logits, a.ids, a.teacher = T.ptr(logits), T.ptr(ids), T.ptr(teacher)
-    a.labels, a.weights = T.ptr(labels), T.ptr(weights)
-    row_loss = torch.empty(lead, dtype=torch.float32, device=dev)
-    a.row_loss = T.ptr(row_loss)
-    loss = scratch = None
-    if reduction != "none":
+    outer, inner = T.row_counts(lead)
+    logits, (ld_outer, ld_inner) = T.row_input(logits, nd)
+    g_outer, g_inner = (0, 0) if grad is None else T.rows2(grad, nd)
+    loss = row_loss = None
+    if reduction == "none":
+        row_loss = torch.empty(lead, dtype=torch.float32, device=dev)
+        at = row_loss.data_ptr()
+        loss_at = scratch_at = None
+    else:  # the workspace: the sum of weights, the rows' losses
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        a.loss = T.ptr(loss)
-        if reduction == "mean" and weights is not None:
-            scratch = torch.empty(1, dtype=torch.float32, device=dev)
-            a.weight_sum = T.ptr(scratch)
-    if grad is not None:
-        a.grad = T.ptr(grad)
-        a.g_outer, a.g_inner = T.rows2(grad, nd)
-    if upstream is not None:
-        a.upstream, a.upstream_stride = T.ptr(upstream), int(upstream.dim() > 0 and upstream.numel() > 1)
+        work = torch.empty(1 + outer * inner, dtype=torch.float32, device=dev)
+        loss_at, scratch_at = loss.data_ptr(), work.data_ptr()
+        at = scratch_at + 4
+    stride = 0 if upstream is None or upstream.dim() == 0 or upstream.numel() == 1 else 1
+    a = C.M3DistillArgs(outer, inner, logits.shape[-1], ids.shape[-1], T.io_dtype(logits.dtype), _REDUCE[reduction],
+                        temperature, hard_weight, grad_scale, logits.data_ptr(), ld_outer, ld_inner, ids.data_ptr(),
+                        teacher.data_ptr(), T.ptr(labels), T.ptr(weights), T.ptr(upstream), stride, at, loss_at,
+                        scratch_at, T.ptr(grad), g_outer, g_inner)
     T.call(C.lib().m3_distill, a, dev)
     return row_loss if loss is None else loss
 
@@ -123,10 +127,9 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     side = _check(logits, teacher_ids, teacher_logits, labels, weights, temperature, hard_weight, reduction)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillFn.apply(logits, *side, float(temperature), float(hard_weight), reduction)
-    return _run(logits.detach(), *side, temperature, hard_weight, reduction)
+    return _run(logits, *side, temperature, hard_weight, reduction)
 
 
-@torch.no_grad()
 def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
                           temperature: float = 1.0, labels: Optional[torch.Tensor] = None, hard_weight: float = 0.0,
                           weights: Optional[torch.Tensor] = None, reduction: str = "mean", grad_scale: float = 1.0,
@@ -140,6 +143,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     nd = logits.dim() - 1
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.requires_grad and out.is_leaf and torch.is_grad_enabled():
+        raise ValueError("out must not be a leaf that requires grad")
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype} on {logits.device}")
     elif not _writable_rows(out, nd):

@@ -16,25 +16,28 @@ from . import _tensors as T
 
 
 def _check_tokens(tokens, ref):
-    T.require_cuda(tokens, ref)
-    if tokens.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"tokens must be int64 or int32, got {tokens.dtype}")
-    if tokens.device != ref.device:
-        raise ValueError(f"tokens must be on {ref.device}, got {tokens.device}")
+    """The tokens as the kernels read them (int64)."""
+    T.require_here(ref.device, tokens)
+    if tokens.dtype != torch.int64:
+        if tokens.dtype != torch.int32:
+            raise ValueError(f"tokens must be int64 or int32, got {tokens.dtype}")
+        tokens = tokens.to(torch.int64)
+    return tokens
 
 
 def _lookup(table, tokens, scale, dtype):
-    lead = tokens.shape
-    a = C.M3EmbedArgs()
-    a.rows_outer, a.rows_inner = T.row_counts(lead)
-    a.vocab, a.dim = table.shape
-    a.table_dtype, a.out_dtype, a.scale = T.io_dtype(table.dtype), T.io_dtype(dtype), scale
-    tokens, (a.t_outer, a.t_inner) = T.row_input(tokens.to(torch.int64), len(lead))
-    if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
-        table = table.contiguous()
-    out = torch.empty(*lead, a.dim, dtype=dtype, device=table.device)
-    a.tokens, a.table, a.table_ld, a.out, a.out_ld = T.ptr(tokens), T.ptr(table), table.stride(0), T.ptr(out), a.dim
-    T.call(C.lib().m3_embed, a, table.device)
+    lead, dev = tokens.shape, table.device
+    vocab, dim = table.shape
+    outer, inner = T.row_counts(lead)
+    tokens, (t_outer, t_inner) = T.row_input(tokens, len(lead))
+    ld, unit = table.stride()
+    if unit != 1 or ld < dim:
+        table = table.detach().contiguous()
+        ld = dim
+    out = torch.empty((*lead, dim), dtype=dtype, device=dev)
+    a = C.M3EmbedArgs(outer, inner, vocab, dim, T.io_dtype(table.dtype), T.io_dtype(dtype), scale, 0,
+                      tokens.data_ptr(), t_outer, t_inner, table.data_ptr(), ld, out.data_ptr(), dim)
+    T.call(C.lib().m3_embed, a, dev)
     return out
 
 
@@ -59,15 +62,13 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     gives a NaN row.  Differentiable in ``table`` (a dense gradient in its dtype)."""
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"table must be (vocab, dim), got {tuple(table.shape)}")
-    _check_tokens(tokens, table)
+    tokens = _check_tokens(tokens, table)
     dtype = table.dtype if dtype is None else dtype
-    T.io_dtype(table.dtype), T.io_dtype(dtype)
-    if torch.is_grad_enabled() and table.requires_grad:
+    if table.requires_grad and torch.is_grad_enabled():
         return _EmbedFn.apply(table, tokens, float(scale), dtype)
-    return _lookup(table.detach(), tokens, scale, dtype)
+    return _lookup(table, tokens, scale, dtype)
 
 
-@torch.no_grad()
 def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: float = 1.0,
                    dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The gradient of `embed_tokens` with respect to its table: ``dy (..., D)`` -> ``(vocab, D)``
@@ -78,23 +79,22 @@ def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: fl
         raise ValueError(f"dy must be {tuple(tokens.shape)} + (dim,), got {tuple(dy.shape)}")
     if vocab < 1:
         raise ValueError(f"vocab must be >= 1, got {vocab}")
-    _check_tokens(tokens, dy)
+    tokens = _check_tokens(tokens, dy)
     lead, dim, dev = tokens.shape, dy.shape[-1], dy.device
     add = out is not None
     if not add:
-        out = torch.empty(vocab, dim, dtype=dtype, device=dev)
+        out = torch.empty((vocab, dim), dtype=dtype, device=dev)
     elif out.shape != (vocab, dim) or out.device != dev or (dim > 1 and out.stride(1) != 1) or out.stride(0) < dim:
         raise ValueError(f"out must be ({vocab}, {dim}) on {dev} with contiguous rows")
-    a = C.M3EmbedBwdArgs()
-    a.rows_outer, a.rows_inner = T.row_counts(lead)
-    a.vocab, a.dim, a.dy_dtype, a.grad_dtype = vocab, dim, T.io_dtype(dy.dtype), T.io_dtype(out.dtype)
-    a.scale, a.accumulate = scale, int(add)
     nd = len(lead)
-    tokens, (a.t_outer, a.t_inner) = T.row_input(tokens.to(torch.int64), nd)
-    dy, (a.dy_outer, a.dy_inner) = T.row_input(dy, nd)
+    outer, inner = T.row_counts(lead)
+    tokens, (t_outer, t_inner) = T.row_input(tokens, nd)
+    dy, (dy_outer, dy_inner) = T.row_input(dy, nd)
     lib = C.lib()
-    ws = torch.empty(lib.m3_embed_bwd_workspace_size(a.rows_outer * a.rows_inner, dim), dtype=torch.uint8, device=dev)
-    a.tokens, a.dy, a.grad, a.grad_ld = T.ptr(tokens), T.ptr(dy), T.ptr(out), out.stride(0)
-    a.workspace, a.workspace_bytes = T.ptr(ws), ws.numel()
+    size = lib.m3_embed_bwd_workspace_size(outer * inner, dim)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    a = C.M3EmbedBwdArgs(outer, inner, vocab, dim, T.io_dtype(dy.dtype), T.io_dtype(out.dtype), scale, int(add),
+                         tokens.data_ptr(), t_outer, t_inner, dy.data_ptr(), dy_outer, dy_inner, out.data_ptr(),
+                         out.stride(0), ws.data_ptr(), size)
     T.call(lib.m3_embed_bwd, a, dev)
     return out

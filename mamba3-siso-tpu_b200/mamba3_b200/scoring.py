@@ -26,7 +26,6 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]      # (..., top)
 
 
-@torch.no_grad()
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0,
                    temperature: float = 1.0) -> TokenLogprobs:
     """``logits (..., V)`` bf16 or f32, ``targets (...)`` int -> `TokenLogprobs`.
@@ -35,37 +34,37 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     equal logits the lower id is the higher alternative.  A row whose largest logit is not
     finite (all -inf, or any +inf / NaN) has no distribution: its floats are NaN.  Views such
     as ``logits[:, :-1]`` and ``tokens[:, 1:]`` are read in place.  No gradient."""
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be (..., vocab), got {tuple(logits.shape)}")
-    T.require_cuda(logits, targets)
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
-    top = int(top)
+    shape, dev = logits.shape, logits.device
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"logits must be (..., vocab), got {tuple(shape)}")
+    lead, vocab = shape[:-1], shape[-1]
+    T.require_here(dev, targets)
     if not 0 <= top <= min(vocab, C.M3_MAX_TOP):
         raise ValueError(f"top must be in [0, {min(vocab, C.M3_MAX_TOP)}], got {top}")
     if not temperature > 0:
         raise ValueError(f"temperature must be > 0, got {temperature}")
-    if targets is not None and (targets.shape != lead or targets.device != logits.device):
-        raise ValueError(f"targets must be {tuple(lead)} on {logits.device}, got {tuple(targets.shape)} on "
-                         f"{targets.device}")
-    if targets is not None and targets.dtype not in (torch.int64, torch.int32):
-        raise ValueError(f"targets must be int64 or int32, got {targets.dtype}")
-    a = C.M3ScoreArgs()
-    a.logits_dtype = T.io_dtype(logits.dtype)
-    a.rows_outer, a.rows_inner = T.row_counts(lead)
-    a.vocab, a.top, a.temperature = vocab, top, temperature
-    nd, dev, f32 = len(lead), logits.device, torch.float32
-    logits, (a.ld_outer, a.ld_inner) = T.row_input(logits, nd)
-    a.logits = T.ptr(logits)
-    logprob = top_logprob = top_ids = None
-    if targets is not None:
-        targets, (a.t_outer, a.t_inner) = T.row_input(targets.to(torch.int64), nd)
-        logprob = torch.empty(lead, dtype=f32, device=dev)
-        a.targets, a.logprob = T.ptr(targets), T.ptr(logprob)
-    entropy, lse = torch.empty(lead, dtype=f32, device=dev), torch.empty(lead, dtype=f32, device=dev)
-    a.entropy, a.lse = T.ptr(entropy), T.ptr(lse)
+    dtype = T.io_dtype(logits.dtype)
+    nd, f32 = len(lead), torch.float32
+    outer, inner = T.row_counts(lead)
+    logits, (ld_outer, ld_inner) = T.row_input(logits, nd)
+    t_ptr = t_outer = t_inner = logprob = top_logprob = top_ids = None
+    if targets is None:
+        entropy, lse = torch.empty((2, *lead), dtype=f32, device=dev).unbind(0)
+    else:
+        if targets.shape != lead:
+            raise ValueError(f"targets must be {tuple(lead)}, got {tuple(targets.shape)}")
+        if targets.dtype != torch.int64:
+            if targets.dtype != torch.int32:
+                raise ValueError(f"targets must be int64 or int32, got {targets.dtype}")
+            targets = targets.to(torch.int64)
+        targets, (t_outer, t_inner) = T.row_input(targets, nd)
+        t_ptr = targets.data_ptr()
+        entropy, lse, logprob = torch.empty((3, *lead), dtype=f32, device=dev).unbind(0)
     if top:
-        top_logprob = torch.empty(*lead, top, dtype=f32, device=dev)
-        top_ids = torch.empty(*lead, top, dtype=torch.int64, device=dev)
-        a.top_logprob, a.top_ids = T.ptr(top_logprob), T.ptr(top_ids)
+        top_logprob = torch.empty((*lead, top), dtype=f32, device=dev)
+        top_ids = torch.empty((*lead, top), dtype=torch.int64, device=dev)
+    a = C.M3ScoreArgs(outer, inner, vocab, top, dtype, temperature, logits.data_ptr(), ld_outer, ld_inner, t_ptr,
+                      t_outer or 0, t_inner or 0, T.ptr(logprob), entropy.data_ptr(), lse.data_ptr(),
+                      T.ptr(top_logprob), T.ptr(top_ids))
     T.call(C.lib().m3_token_logprobs, a, dev)
     return TokenLogprobs(logprob, entropy, lse, top_logprob, top_ids)
