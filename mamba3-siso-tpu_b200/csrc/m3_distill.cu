@@ -323,10 +323,8 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
     }
   };
   walk<T, kNV, TB>(v, n, tid, GRAD ? Keep::kYes : Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
-    float mt = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kNV; ++j)
-      if (full.value || base + j * TB < n) mt = fmaxf(mt, vec_max<T>(d[j]));
+    VecMax<T> vm[kNV];
+    const float mt = vecs_max<T, kNV>(d, vm, [&](int j) { return full.value || base + j * TB < n; });
     raise(warp_max(mt));
     const float ref = finite_or_0(m);
 #pragma unroll
@@ -427,8 +425,9 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       row_of[warp][j * 32 + lane] = d[j];
-      m = fmaxf(m, vec_max<T>(d[j]));
     }
+    VecMax<T> vm[NV];
+    m = vecs_max<T, NV>(d, vm, [](int) { return true; });
     if (GRAD)
       for (int i = lane; i < kSeen; i += 32) seen_of[warp][i] = 0u;
     m = warp_max(m);

@@ -23,7 +23,7 @@ constexpr int kVecCap = 512, kCandCap = 512;
 
 struct Params {
   int rows, vocab, top, cluster, log2_cluster;
-  float inv_t;
+  float inv_t, c, plain_most;
   Rows lrow, trow;
   const void* logits;
   const int64_t* targets;
@@ -31,69 +31,69 @@ struct Params {
   int64_t* top_ids;
 };
 
-// Sums against a maximum, in log2 units: s = sum 2^d, u = sum 2^d d, d = (x - m) log2(e) / T.
+// The maximum, and against the reference r: s = sum 2^d, u = sum 2^d d.
 struct Part {
-  float m, s, u;
+  float m, r, s, u;
 };
-
-__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ Part no_part() { return Part{-INFINITY, kLowRef, 0.f, 0.f}; }
 
 template <typename T>
-__device__ __forceinline__ void add_vec(const uint4& v, float m, float c, float2& s, float2& u) {
+__device__ __forceinline__ void add_vec(const uint4& v, float r, float c, float2& s, float2& u) {
   float2 f[kVec<T> / 2];
-  unpack<T>(v, f);
+  unpack<T>(clamp_low<T>(v), f);
 #pragma unroll
   for (int j = 0; j < kVec<T> / 2; ++j) {
-    const float2 d = mul2(add2(f[j], f2s(-m)), f2s(c));
+    const float2 d = fma2(f[j], f2s(c), f2s(-r));
     const float2 e = f2(ex2(d.x), ex2(d.y));
     s = add2(s, e);
-    u = fma2(e, f2(fmaxf(d.x, -1e4f), fmaxf(d.y, -1e4f)), u);  // 2^d is 0 there: 0 * -inf is 0
+    u = fma2(e, d, u);
   }
 }
 
-// Joins the parts held by the lanes of a warp (lanes without one: m = -inf, s = u = 0).
-__device__ __forceinline__ Part join(Part p, float c) {
-  const float m = warp_max(p.m);
-  // a warp of masked entries may lie further below than fp32 reaches: 2^d is 0, s d has to stay finite
-  const float d = fmaxf((p.m - m) * c, -1e4f);
-  const float e = p.m == -INFINITY ? 0.f : ex2(d);
+// Joins the parts held by the lanes of a warp.
+__device__ __forceinline__ Part join(Part p) {
   Part r;
-  r.m = m;
+  r.m = warp_max(p.m);
+  r.r = warp_max(p.r);
+  const float d = p.r - r.r, e = ex2(d);  // 0 for a lane without a part
   r.s = warp_sum(p.s * e);
   r.u = warp_sum((p.u + p.s * d) * e);
-  // a part with NaN has s = NaN under any maximum
   return r;
 }
 
-struct Row {
-  float m, ln_z, inv_t;
-  __device__ __forceinline__ float logprob(float x) const { return (x - m) * inv_t - ln_z; }
-};
-
-__device__ __forceinline__ Row finish(const Params& p, const Part& r, int row, bool write) {
-  const float l2 = r.m == -INFINITY ? NAN : log2f(r.s);
-  Row w{r.m, l2 * kLn2, p.inv_t};
-  if (write) {
-    p.lse[row] = fmaf(r.m, p.inv_t, w.ln_z);
-    p.entropy[row] = (l2 - r.u / r.s) * kLn2;
+// The terms [lo, hi) of a row that is not plain, every `step`-th from lo + first, against its maximum.
+template <typename T>
+__device__ __noinline__ Part slow_part(const T* x, int lo, int hi, int first, int step, float m, float c) {
+  float s = 0.f, u = 0.f;
+  for (int i = lo + first; i < hi; i += step) {
+    const float d = (ld(x + i) - m) * c, e = ex2(d);
+    s += e;
+    u = fmaf(e, fmaxf(d, -1e4f), u);  // e is 0 there: 0 * -inf would not be
   }
-  return w;
+  return Part{m, 0.f, s, u};
 }
 
-__device__ __forceinline__ void write_target(const Params& p, const Row& w, int row, int64_t t, float xt) {
-  p.logprob[row] = t < 0 ? 0.f : t >= p.vocab ? NAN : w.logprob(xt);
+__device__ __forceinline__ Log2P distribution(const Part& a, bool plain, float c) {
+  return Log2P{plain, c, plain ? a.r : a.m, log2f(a.s)};
+}
+__device__ __forceinline__ void write_row(const Params& p, const Part& a, const Log2P& q, int row) {
+  p.lse[row] = q.lse(p.inv_t);
+  p.entropy[row] = (q.l2 - a.u / a.s) * kLn2;
+}
+__device__ __forceinline__ void write_target(const Params& p, const Log2P& q, int row, int64_t t, float xt) {
+  p.logprob[row] = t < 0 ? 0.f : t >= p.vocab ? NAN : q.ln(xt, p.inv_t);
 }
 
 // ---- one CTA or one cluster per row -------------------------------------------------------
 template <int NW, bool TOP>
 struct Smem {
   Part part[NW];
-  Part parts[kMaxCluster];
+  Part parts[kMaxCluster], again[kMaxCluster];
 };
 template <int NW>
 struct Smem<NW, true> {
   Part part[NW];
-  Part parts[kMaxCluster];
+  Part parts[kMaxCluster], again[kMaxCluster];
   float bound[NW];
   int n_vec, n_cand;
   int vec_at[kVecCap];
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
   const Split sp = split_row(x, V);
   const int per = (sp.full + cl - 1) >> p.log2_cluster, v0 = min(sp.full, rank * per), n = min(per, sp.full - v0);
   const uint4* v = reinterpret_cast<const uint4*>(x + sp.head) + v0;
-  const float c = p.inv_t * kLog2e;
+  const float c = p.c;
   if (cl > 1) cluster_arrive_relaxed();  // peers have started before anyone writes to their shared memory
 
   int64_t t = -1;
@@ -163,21 +163,23 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
     t = p.targets[p.trow.at(row)];
     if (t >= 0 && t < V) xt = ld(x + t);
   }
-  float m = -INFINITY, mine = -INFINITY;  // the warp's maximum, this lane's
+  float m = -INFINITY, ref = kLowRef, mine = -INFINITY;  // the warp's maximum and reference, this lane's maximum
   float2 s2 = f2s(0.f), u2 = f2s(0.f);
   auto raise = [&](float to) {  // the sums against a new maximum
     if (to > m) {
-      if (m != -INFINITY) {
-        const float dm = fmaxf((m - to) * c, -1e4f), e = ex2(dm);
-        u2 = mul2(fma2(s2, f2s(dm), u2), f2s(e));
-        s2 = mul2(s2, f2s(e));
-      }
       m = to;
+      const float r = ref_of(m, c);
+      if (r > ref) {
+        const float dr = ref - r, e = ex2(dr);
+        u2 = mul2(fma2(s2, f2s(dr), u2), f2s(e));
+        s2 = mul2(s2, f2s(e));
+        ref = r;
+      }
     }
   };
   // warps all of whose lanes see a vector, and how many lane maxima each of them gives
   const int wide = min(NW, n >> 5), r = wide ? (p.top + wide - 1) / wide : 33;
-  float bound = -INFINITY;  // of the row
+  float bound = -INFINITY, own = -INFINITY;  // of the row, of this warp
   if constexpr (TOP) {
     if (lane == 0) s.bound[warp] = r <= 32 && warp >= wide ? INFINITY : -INFINITY;
     if (tid == 0) s.n_vec = s.n_cand = 0;
@@ -186,30 +188,26 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
   auto raise_bound = [&]() {  // after a change of a lane's maximum
     if constexpr (TOP) {
       if (r > 32 || warp >= wide) return;
-      float left = mine, b = 0.f;
+      float left = mine;
       for (int i = 0; i < r; ++i) {
-        b = warp_max(left);
-        const unsigned at = __ballot_sync(0xffffffffu, left == b);
+        own = warp_max(left);
+        const unsigned at = __ballot_sync(0xffffffffu, left == own);
         if (lane == __ffs(at) - 1) left = -INFINITY;
       }
-      if (lane == 0) *(volatile float*)&s.bound[warp] = b;
+      if (lane == 0) *(volatile float*)&s.bound[warp] = own;
     }
   };
   walk<T, kNV, TB>(v, n, tid, Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
-    float mt = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kNV; ++j)
-      if (full.value || base + j * TB < n) mt = fmaxf(mt, vec_max<T>(d[j]));
+    VecMax<T> vm[kNV];
+    const float mt = vecs_max<T, kNV>(d, vm, [&](int j) { return full.value || base + j * TB < n; });
     raise(warp_max(mt));
-    const float ref = finite_or_0(m);
 #pragma unroll
     for (int j = 0; j < kNV; ++j)
       if (full.value || base + j * TB < n) add_vec<T>(d[j], ref, c, s2, u2);
     if constexpr (TOP) {
-      if (__any_sync(0xffffffffu, mt > mine)) {
-        mine = fmaxf(mine, mt);
-        raise_bound();
-      }
+      const bool higher = mt > mine && mt > own;  // below `own` nothing changes the r-th largest
+      mine = fmaxf(mine, mt);
+      if (__any_sync(0xffffffffu, higher)) raise_bound();
       if (base == 0) __syncthreads();  // a first bound from every warp; later ones may be read late
       __syncwarp();
       bound = -warp_max(lane < NW ? -*(volatile float*)&s.bound[lane] : -INFINITY);
@@ -217,7 +215,7 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
 #pragma unroll
         for (int j = 0; j < kNV; ++j) {
           const int q = base + j * TB + tid;
-          if ((full.value || q < n) && vec_max<T>(d[j]) >= bound) {
+          if ((full.value || q < n) && vm[j].reaches(bound)) {
             const int at = atomicAdd(&s.n_vec, 1);
             if (at < kVecCap) {
               s.vec[at] = d[j];
@@ -233,19 +231,21 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
     const int i = edge_index(sp, lane, rank == 0, rank == cl - 1);
     const float xe = i >= 0 ? ld(x + i) : -INFINITY;
     raise(warp_max(xe));
-    const float d = (xe - finite_or_0(m)) * c, e = ex2(d);
+    const float d = fmaf(xe > -1e30f || xe != xe ? xe : -1e30f, c, -ref), e = ex2(d);
     s2.x += e;
-    u2.x = fmaf(e, fmaxf(d, -1e4f), u2.x);
+    u2.x = fmaf(e, d, u2.x);
     if constexpr (TOP)
       if (i >= 0) s.cand[atomicAdd(&s.n_cand, 1)] = rank_word(xe, i);
   }
-  Part a{m, warp_sum(s2.x + s2.y), warp_sum(u2.x + u2.y)};
+  Part a{m, ref, warp_sum(s2.x + s2.y), warp_sum(u2.x + u2.y)};
   if (lane == 0) s.part[warp] = a;
   __syncthreads();
-  a = join(lane < NW ? s.part[lane] : Part{-INFINITY, 0.f, 0.f}, c);
+  a = join(lane < NW ? s.part[lane] : no_part());
+  // this share's entries, its vectors' first
+  const int first = sp.head + v0 * E, lo = rank == 0 ? 0 : first, hi = rank == cl - 1 ? V : first + n * E;
 
   if constexpr (TOP) {
-    const int k = p.top, first = sp.head + v0 * E;  // element 0 of this share's vectors
+    const int k = p.top;
     bound = -warp_max(lane < NW ? -s.bound[lane] : -INFINITY);
     const int nv = s.n_vec;
     if (nv <= kVecCap)
@@ -259,7 +259,6 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
     __syncthreads();
     // the sum is NaN iff the share holds NaN or +inf, which the comparisons above do not order
     if (nv > kVecCap || s.n_cand > kCandCap || a.s != a.s) {
-      const int lo = rank == 0 ? 0 : first, hi = rank == cl - 1 ? V : first + n * E;
       exact_top<T, TB>(x, lo, hi, min(k, hi - lo), s);
     }
     const int nc = s.n_cand;
@@ -287,10 +286,32 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    a = join(lane < cl ? s.parts[lane] : Part{-INFINITY, 0.f, 0.f}, c);
+    a = join(lane < cl ? s.parts[lane] : no_part());
   }
-  const Row w = finish(p, a, row, rank == 0 && tid == 0);
-  if (p.targets && rank == 0 && tid == 0) write_target(p, w, row, t, xt);
+  const bool plain = fabsf(a.m) * c <= p.plain_most;
+  if (!plain) {  // the same for all threads of the row
+    a = slow_part(x, lo, hi, tid, TB, a.m, c);
+    a.s = warp_sum(a.s);
+    a.u = warp_sum(a.u);
+    __syncthreads();
+    if (lane == 0) s.part[warp] = a;
+    __syncthreads();
+    const float m_all = a.m;
+    a = join(lane < NW ? s.part[lane] : Part{m_all, 0.f, 0.f, 0.f});
+    if (cl > 1) {
+      if (tid < cl) *peer(&s.again[rank], tid) = a;
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      a = join(lane < cl ? s.again[lane] : Part{m_all, 0.f, 0.f, 0.f});
+    }
+    a.m = m_all;
+  }
+  const Log2P w = distribution(a, plain, c);
+  if (rank == 0 && tid == 0) {
+    write_row(p, a, w, row);
+    if (p.targets) write_target(p, w, row, t, xt);
+  }
 
   if constexpr (TOP) {
     const int k = p.top;
@@ -316,28 +337,46 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
       const int at = s.before[i];
       if (e != 0 && at < k) {
         p.top_ids[(int64_t)row * k + at] = rank_index(e);
-        p.top_logprob[(int64_t)row * k + at] = w.logprob(key_value((uint32_t)(e >> 32)));
+        p.top_logprob[(int64_t)row * k + at] = w.ln(key_value((uint32_t)(e >> 32)), p.inv_t);
       }
     }
   }
 }
 
 // ---- one warp per row ---------------------------------------------------------------------
-// The (logit, lower index) order as one word: 32 bits for bf16 rows of at most 512 entries.
+// The (logit, lower index) order as one word; 0 is below every entry.  bf16: the 16-bit key and the
+// complement of the index, for rows of at most 512 entries.
 template <typename T>
 struct Word;
 template <>
 struct Word<__nv_bfloat16> {
   using type = uint32_t;
-  static __device__ __forceinline__ type make(float x, int i) { return (key_of(x) & 0xFFFF0000u) | (0xFFFFu - i); }
-  static __device__ __forceinline__ float value(type w) { return key_value(w >= 0xFFFF0000u ? ~0u : (w & 0x80000000u) ? w & 0xFFFF0000u : w | 0xFFFFu); }
+  static __device__ __forceinline__ void make(const uint4& v, int i0, type* w) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t k;  // + 0: -0 becomes 0, every NaN 0x7FFF; then the order of the bits, both halves at once
+      asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(k) : "r"(u[j]), "r"(0u));
+      k ^= ((k >> 15) & 0x00010001u) * 0x7FFFu ^ 0x80008000u;
+      w[2 * j] = k * 65536u + (uint32_t)(0xFFFF - i0 - 2 * j);
+      w[2 * j + 1] = (k & 0xFFFF0000u) + (uint32_t)(0xFFFF - i0 - 2 * j - 1);
+    }
+  }
+  static __device__ __forceinline__ float value(type w) {
+    const uint32_t b = w & 0xFFFF0000u;
+    return __uint_as_float(w & 0x80000000u ? b & 0x7FFF0000u : ~b & 0xFFFF0000u);
+  }
   static __device__ __forceinline__ int index(type w) { return 0xFFFF - (int)(w & 0xFFFFu); }
   static __device__ __forceinline__ type max(type w) { return __reduce_max_sync(0xffffffffu, w); }
 };
 template <>
 struct Word<float> {
   using type = uint64_t;
-  static __device__ __forceinline__ type make(float x, int i) { return rank_word(x, i); }
+  static __device__ __forceinline__ void make(const uint4& v, int i0, type* w) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = rank_word(__uint_as_float(u[j]), i0 + j);
+  }
   static __device__ __forceinline__ float value(type w) { return key_value((uint32_t)(w >> 32)); }
   static __device__ __forceinline__ int index(type w) { return rank_index(w); }
   static __device__ __forceinline__ type max(type w) {
@@ -365,81 +404,116 @@ __device__ __forceinline__ void sort_desc(W (&w)[N]) {
           }
 }
 
-constexpr int kWarpThreads = 256, kWarpRows = kWarpThreads / 32;
+// A warp takes `batch` (at most 32) rows one after the other, the next one's vectors on their way, and
+// keeps row i's sums in lane i, so that what is done once per row is done for all of them at once.
+constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
 
 template <typename T, int NV, bool TOP>
-__global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p) {
-  constexpr int E = kVec<T>;
+__global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p, int batch) {
+  constexpr int E = kVec<T>, N = NV * E;
   const int lane = threadIdx.x & 31, V = p.vocab;
-  const int step = gridDim.x * kWarpRows;
-  const float c = p.inv_t * kLog2e;
-  int row = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
-  const T* x = nullptr;
+  const float c = p.c;
+  const int row0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * batch, rows = min(batch, p.rows - row0);
+  if (rows <= 0) return;
   uint4 d[NV];
-  auto load = [&](int r) {
-    x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(r);
-    const int shift = row_shift(x);
+  int shift = 0;
+  auto load = [&](int row) {
+    const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
+    shift = row_shift(x);
+    const bool whole = shift == 0 && V % E == 0;  // no ragged vector
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int lo = (j * 32 + lane) * E - shift;
-      d[j] = lo < V ? load_vec(x, lo, V) : neg_inf_vec<T>();
-    }
-  };
-  if (row < p.rows) load(row);
-  while (row < p.rows) {
-    const T* xr = x;
-    const int shift = row_shift(xr);
-    int64_t t = -1;
-    if (p.targets && lane == 0) t = p.targets[p.trow.at(row)];
-    float m = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) m = fmaxf(m, vec_max<T>(d[j]));
-    m = warp_max(m);
-    const float ref = finite_or_0(m);
-    float2 s2 = f2s(0.f), u2 = f2s(0.f);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) add_vec<T>(d[j], ref, c, s2, u2);
-    typename Word<T>::type wd[TOP ? NV * E : 1];
-    if constexpr (TOP) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float2 f[E / 2];
-        unpack<T>(d[j], f);
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const int idx = (j * 32 + lane) * E - shift + i;
-          wd[j * E + i] = idx >= 0 && idx < V ? Word<T>::make(i & 1 ? f[i / 2].y : f[i / 2].x, idx) : 0;
-        }
+      d[j] = neg_inf_vec<T>();
+      if (whole) {
+        if (lo < V) d[j] = load_once(reinterpret_cast<const uint4*>(x + lo));
+      } else if (lo < V) {
+        d[j] = load_vec(x, lo, V);
       }
     }
-    const int next = row + step;
-    if (next < p.rows) load(next);  // on its way while this row is finished
-    float xt = 0.f;
-    if (t >= 0 && t < V) xt = ld(xr + t);
-    const Part a{m, warp_sum(s2.x + s2.y), warp_sum(u2.x + u2.y)};
-    const Row w = finish(p, a, row, lane == 0);
-    if (p.targets && lane == 0) write_target(p, w, row, t, xt);
+  };
+  load(row0);
+  Part keep = no_part();
+  for (int i = 0; i < rows; ++i) {
+    const int at = shift;
+    Part a = no_part();
+    VecMax<T> vm[NV];
+    a.m = warp_max(vecs_max<T, NV>(d, vm, [](int) { return true; }));
+    a.r = ref_of(a.m, c);
+    float2 s2 = f2s(0.f), u2 = f2s(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) add_vec<T>(d[j], a.r, c, s2, u2);
+    typename Word<T>::type wd[TOP ? N : 1];
     if constexpr (TOP) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) Word<T>::make(d[j], (j * 32 + lane) * E - at, wd + j * E);
+      // entries before the row's start rank nowhere; those past its end lose to all of its own
+      if (at > 0) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (lane == 0 && j < at) wd[j] = 0;
+      }
+    }
+    if (i + 1 < rows) load(row0 + i + 1);
+    a.s = warp_sum(s2.x + s2.y);
+    a.u = warp_sum(u2.x + u2.y);
+    const bool plain = fabsf(a.m) * c <= p.plain_most;
+    if (!plain) {
+      a = slow_part(reinterpret_cast<const T*>(p.logits) + p.lrow.at(row0 + i), 0, V, lane, 32, a.m, c);
+      a.s = warp_sum(a.s);
+      a.u = warp_sum(a.u);
+    }
+    if (lane == i) keep = a;
+    if constexpr (TOP) {
+      const Log2P q = distribution(a, plain, c);
+      const int64_t out = (int64_t)(row0 + i) * p.top;
       sort_desc(wd);
-      typename Word<T>::type keep = 0;
-      for (int j = 0; j < p.top; ++j) {
+      typename Word<T>::type mine = 0;
+      auto take = [&](int left) {  // the largest word leaves its lane's list, of which `left` words still matter
         const auto best = Word<T>::max(wd[0]);
         if (wd[0] == best) {
 #pragma unroll
-          for (int i = 0; i + 1 < NV * E; ++i) wd[i] = wd[i + 1];
-          wd[NV * E - 1] = 0;
+          for (int e = 0; e + 1 < N; ++e)
+            if (e < left) wd[e] = wd[e + 1];
+          wd[N - 1] = 0;
         }
-        if (lane == (j & 31)) keep = best;
-        if ((j & 31) == 31 || j == p.top - 1) {
-          const int i = (j & ~31) + lane;
-          if (i <= j) {
-            p.top_ids[(int64_t)row * p.top + i] = Word<T>::index(keep);
-            p.top_logprob[(int64_t)row * p.top + i] = w.logprob(Word<T>::value(keep));
+        return best;
+      };
+      auto put = [&](int k0, int n) {
+        if (lane < n) {
+          p.top_ids[out + k0 + lane] = Word<T>::index(mine);
+          p.top_logprob[out + k0 + lane] = q.ln(Word<T>::value(mine), p.inv_t);
+        }
+      };
+      if (p.top <= 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < p.top) {
+            const auto best = take(7 - j);
+            if (lane == j) mine = best;
           }
+        put(0, p.top);
+      } else {
+        for (int k0 = 0; k0 < p.top; k0 += 32) {
+          const int n = min(32, p.top - k0);
+          for (int j = 0; j < n; ++j) {
+            const auto best = take(N);
+            if (lane == j) mine = best;
+          }
+          put(k0, n);
         }
       }
     }
-    row = next;
+  }
+  if (lane < rows) {
+    const int row = row0 + lane;
+    const Log2P q = distribution(keep, fabsf(keep.m) * c <= p.plain_most, c);
+    write_row(p, keep, q, row);
+    if (p.targets) {
+      const int64_t t = p.targets[p.trow.at(row)];
+      const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
+      write_target(p, q, row, t, t >= 0 && t < V ? ld(x + t) : 0.f);
+    }
   }
 }
 
@@ -468,8 +542,11 @@ int launch_cta(const Params& p, cudaStream_t s) {
 
 template <typename T, int NV, bool TOP>
 int launch_warp(const Params& p, cudaStream_t s) {
-  const int want = (p.rows + kWarpRows - 1) / kWarpRows, most = sm_count() * 8;
-  score_warp_kernel<T, NV, TOP><<<(unsigned)(want < most ? want : most), kWarpThreads, 0, s>>>(p);
+  // batches as long as 32 warps on every SM have one
+  int batch = p.rows / (sm_count() * 32);
+  batch = batch < 1 ? 1 : batch > 32 ? 32 : batch;
+  const int warps = (p.rows + batch - 1) / batch;
+  score_warp_kernel<T, NV, TOP><<<(unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, 0, s>>>(p, batch);
   return check_launch("m3_token_logprobs");
 }
 
@@ -521,6 +598,8 @@ extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
   p.cluster = 1;
   p.log2_cluster = 0;
   p.inv_t = 1.f / a.temperature;
+  p.c = kLog2e / a.temperature;
+  p.plain_most = plain_most(p.c);
   p.lrow = Rows{a.rows_outer, a.rows_inner, a.ld_outer, a.ld_inner};
   p.trow = Rows{a.rows_outer, a.rows_inner, a.t_outer, a.t_inner};
   p.logits = a.logits;

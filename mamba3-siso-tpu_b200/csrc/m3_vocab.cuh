@@ -200,16 +200,63 @@ __device__ __forceinline__ void unpack(const uint4& u, float2 (&f)[kVec<T> / 2])
   }
 }
 
-// The largest element (NaN ignored).
+// The largest elements of a vector (NaN ignored), two side by side for bf16.
 template <typename T>
-__device__ __forceinline__ float vec_max(const uint4& u) {
-  if constexpr (sizeof(T) == 2) {
+struct VecMax;
+template <>
+struct VecMax<__nv_bfloat16> {
+  __nv_bfloat162 m;
+  __device__ __forceinline__ void of(const uint4& u) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
-  } else {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
   }
+  __device__ __forceinline__ void none() { m = __float2bfloat162_rn(-INFINITY); }
+  __device__ __forceinline__ void join(const VecMax& o) { m = __hmax2(m, o.m); }
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(m), __high2float(m)); }
+  // some element is at least b, a logit (so that bf16 holds it)
+  __device__ __forceinline__ bool reaches(float b) const { return !__hblt2(m, __float2bfloat162_rn(b)); }
+};
+template <>
+struct VecMax<float> {
+  float m;
+  __device__ __forceinline__ void of(const uint4& u) {
+    m = fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  __device__ __forceinline__ void none() { m = -INFINITY; }
+  __device__ __forceinline__ void join(const VecMax& o) { m = fmaxf(m, o.m); }
+  __device__ __forceinline__ float value() const { return m; }
+  __device__ __forceinline__ bool reaches(float b) const { return m >= b; }
+};
+
+// The largest element of the vectors with `use(j)`; vm: of each of them.
+template <typename T, int NV, typename F>
+__device__ __forceinline__ float vecs_max(const uint4 (&d)[NV], VecMax<T> (&vm)[NV], F use) {
+  VecMax<T> m;
+  m.none();
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if (use(j)) {
+      vm[j].of(d[j]);
+      m.join(vm[j]);
+    }
+  return m.value();
+}
+
+// max(x, -1e30) per element, NaN kept: finite where -inf would make 0 * -inf.
+template <typename T>
+__device__ __forceinline__ uint4 clamp_low(const uint4& u) {
+  uint4 r;
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 2)  // 0xF149 = bf16(-1e30)
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(o[j]) : "r"(w[j]), "r"(0xF149F149u));
+    else
+      asm("max.NaN.f32 %0, %1, %2;" : "=r"(o[j]) : "r"(w[j]), "r"(0xF149F2CAu));
+  }
+  r = make_uint4(o[0], o[1], o[2], o[3]);
+  return r;
 }
 
 __device__ __forceinline__ float warp_max(float v) {
@@ -217,6 +264,35 @@ __device__ __forceinline__ float warp_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+
+// ---- the sums of a softmax ------------------------------------------------------------------
+// In log2 units: c = log2(e) / T, terms 2^(c x - R) by one fused multiply-add and one SFU exponential.
+// R is the ceiling of c times the largest logit so far: a whole number, so that sums against different
+// R are joined by exact powers of two and the result does not depend on how R was rounded.  Holds for
+// |c x| up to 1e19 ("plain" rows).  A row whose largest logit is beyond that (a mask of the type's lowest
+// value over every entry, infinities, NaN) is summed again as 2^(c (x - max)).
+constexpr float kLowRef = -1e20f;
+
+__device__ __forceinline__ float ref_of(float m, float c) { return fmaxf(ceilf(m * c), kLowRef); }
+// The most that |max| c may be for a plain row; none is with c so small or large that the clamp at
+// -1e30 would not lie between kLowRef and fp32's range.
+inline float plain_most(float c) { return c >= 1e-9f && c <= 1e8f ? 1e19f : -1.f; }
+
+// The logarithm of the distribution at x, given either form's reference (R, or the maximum) and log2 of the sum.
+struct Log2P {
+  bool plain;
+  float c, ref, l2;
+  __device__ __forceinline__ float exponent(float x) const { return plain ? fmaf(x, c, -ref) : (x - ref) * c; }
+  __device__ __forceinline__ float lse(float inv_t) const {  // natural, of x / T
+    return plain ? (ref + l2) * kLn2 : fmaf(ref, inv_t, l2 * kLn2);
+  }
+  __device__ __forceinline__ float ln(float x, float inv_t) const {
+    const float d = exponent(x);
+    // log2(e) x may overflow where x does not
+    if (fabsf(d) == INFINITY && fabsf(x) != INFINITY) return fmaf(x, inv_t, -lse(inv_t));
+    return (d - l2) * kLn2;
+  }
+};
 
 // ---- clusters -------------------------------------------------------------------------------
 __device__ __forceinline__ int cluster_rank() {
