@@ -4,10 +4,10 @@
 // and with hard labels CE = lse(x) - x_label, dCE/dx = softmax(x) - onehot.
 // One read of the logits from memory and one write of their gradient.  Each warp walks its share of a
 // row with a running maximum and sums against it; the parts of the row's warps meet at one barrier;
-// then the row is walked again, from L2 (so that the rows in flight have to fit there), and its
-// gradient written.  One warp holds the teacher's entries, four to a lane.  The dense gradient k_s q is stored
-// first; then each entry's place is stored again as k_s q - p, from the same fp32 values, so that
-// every element is rounded once.
+// then the row is walked again, its first tile still in registers and its second in shared memory, the
+// rest from L2 (so that the rows in flight have to fit there), and its gradient written.  One warp holds
+// the teacher's entries.  The dense gradient k_s q is stored first; then each entry's place is stored
+// again as k_s q - p, from the same fp32 values, so that every element is rounded once.
 #include "m3_internal.h"
 #include "m3_vocab.cuh"
 
@@ -18,11 +18,11 @@ using namespace vocab;
 
 constexpr int kNV = 8;          // vectors a thread loads at a time
 constexpr int kMaxCluster = 8;  // CTAs per row (portable size)
-constexpr int kEnt = M3_MAX_TOP / 32;  // entries a lane holds
+constexpr int kEnt = M3_MAX_TOP / 32;  // entries a lane holds at most
 
 struct Params {
   int rows, vocab, k, cluster, log2_cluster;
-  float temperature, inv_t, hard, scale;  // scale: grad_scale, over the row count for an unweighted mean
+  float temperature, inv_t, c, plain_most, hard, scale;  // scale: grad_scale, over the row count for an unweighted mean
   Rows lrow, grow;
   const void* logits;
   void* grad;
@@ -33,176 +33,94 @@ struct Params {
   float* row_loss;
 };
 
-// Sums against a maximum: s = sum e^((x - m) / T), s1 = sum e^(x - m) (only with hard labels).
+// The maximum, and the sums s = sum 2^(c x - r) and, with hard labels, s1 = sum 2^(log2(e) x - r1).
 struct Part {
-  float m, s, s1;
+  float m, r, s, r1, s1;
 };
-
-__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ Part no_part() { return Part{-INFINITY, kLowRef, 0.f, kLowRef, 0.f}; }
 
 template <typename T, bool HARD>
-__device__ __forceinline__ void add_vec(const uint4& v, float m, float c, float2& s, float2& s1) {
+__device__ __forceinline__ void add_vec(const uint4& v, float r, float r1, float c, float2& s, float2& s1) {
   float2 f[kVec<T> / 2];
   unpack<T>(v, f);
 #pragma unroll
   for (int j = 0; j < kVec<T> / 2; ++j) {
-    const float2 x = add2(f[j], f2s(-m));
-    const float2 d = mul2(x, f2s(c));
+    const float2 d = fma2(f[j], f2s(c), f2s(-r));
     s = add2(s, f2(ex2(d.x), ex2(d.y)));
     if (HARD) {
-      const float2 d1 = mul2(x, f2s(kLog2e));
+      const float2 d1 = fma2(f[j], f2s(kLog2e), f2s(-r1));
       s1 = add2(s1, f2(ex2(d1.x), ex2(d1.y)));
     }
   }
 }
 
 template <bool HARD>
-__device__ __forceinline__ Part join(Part p, float c) {
-  Part r;
-  r.m = warp_max(p.m);
-  const bool none = p.m == -INFINITY;
-  r.s = warp_sum(p.s * (none ? 0.f : ex2((p.m - r.m) * c)));
-  r.s1 = HARD ? warp_sum(p.s1 * (none ? 0.f : ex2((p.m - r.m) * kLog2e))) : 1.f;
-  return r;
+__device__ __forceinline__ Part join(Part p) {
+  Part q;
+  q.m = warp_max(p.m);
+  q.r = warp_max(p.r);
+  q.s = warp_sum(p.s * ex2(p.r - q.r));
+  q.r1 = HARD ? warp_max(p.r1) : 0.f;
+  q.s1 = HARD ? warp_sum(p.s1 * ex2(p.r1 - q.r1)) : 1.f;
+  return q;
 }
 
-// The teacher's entries of a row, held by one warp: entry lane + 32 e.
-struct Entries {
-  int id[kEnt];  // -1: absent
-  float t[kEnt], x[kEnt];
-};
-
-enum { kSoft = 1, kHard = 2, kBad = 4 };  // a row's terms; kBad: an id or label past the vocabulary
-
-// `ids` are loaded as they are, absent and bad ones become -1.
-template <bool HARD>
-__device__ __forceinline__ int load_entries(const Params& p, int row, float w, int64_t label, Entries& en) {
-  const int lane = threadIdx.x & 31;
-  bool any = false, bad = false;
-#pragma unroll
-  for (int e = 0; e < kEnt; ++e) {
-    en.id[e] = -1;
-    en.t[e] = -INFINITY;
-    if (32 * e < p.k) {
-      const int j = lane + 32 * e;
-      if (j < p.k) {
-        const int64_t id = p.ids[(int64_t)row * p.k + j];
-        const float t = p.teacher[(int64_t)row * p.k + j];
-        bad |= id >= p.vocab;
-        if (id >= 0 && id < p.vocab) {
-          en.id[e] = (int)id;
-          en.t[e] = t;
-          any = true;
-        }
-      }
-    }
+// The terms [lo, hi) of a row that is not plain, every `step`-th from lo + first, against its maximum.
+template <typename T>
+__device__ __noinline__ Part slow_part(const T* x, int lo, int hi, int first, int step, float m, float c) {
+  float s = 0.f, s1 = 0.f;
+  for (int i = lo + first; i < hi; i += step) {
+    const float d = ld(x + i) - m;
+    s += ex2(d * c);
+    s1 += ex2(d * kLog2e);
   }
-  any = __any_sync(0xffffffffu, any || bad);
-  bad = __any_sync(0xffffffffu, bad) || (HARD && label >= p.vocab);
-  int f = (any && (!HARD || p.hard < 1.f) ? kSoft : 0) | (HARD && label >= 0 ? kHard : 0);
-  if (w == 0.f) f = 0;
-  return f && bad ? kBad : f;
+  return Part{m, 0.f, s, 0.f, s1};
 }
 
-// The teacher's probabilities and their logarithms; an absent entry has probability 0.
-__device__ __forceinline__ void teacher_softmax(const Params& p, const Entries& en, float (&pr)[kEnt], float (&lp)[kEnt]) {
-  float tm = -INFINITY, es = 0.f;
-#pragma unroll
-  for (int e = 0; e < kEnt; ++e)
-    if (32 * e < p.k) tm = fmaxf(tm, en.t[e]);
-  tm = warp_max(tm);
-#pragma unroll
-  for (int e = 0; e < kEnt; ++e)
-    if (32 * e < p.k) {
-      lp[e] = (en.t[e] - tm) * p.inv_t;
-      pr[e] = en.id[e] >= 0 ? ex2(lp[e] * kLog2e) : 0.f;
-      es += pr[e];
-    }
-  es = warp_sum(es);
-  const float ls = log2f(es) * kLn2, inv = 1.f / es;
-#pragma unroll
-  for (int e = 0; e < kEnt; ++e)
-    if (32 * e < p.k) {
-      pr[e] *= inv;
-      lp[e] -= ls;
-    }
-}
-
-// The loss of a row, by the warp that holds its entries.
-template <bool HARD>
-__device__ __forceinline__ float row_loss(const Params& p, const Part& a, int flags, float w, const Entries& en,
-                                          const float (&pr)[kEnt], const float (&lp)[kEnt], float xl) {
-  if (flags == 0) return 0.f;
-  if (flags & kBad) return NAN;
-  const float ln_z = a.m == -INFINITY ? NAN : log2f(a.s) * kLn2;
-  float kl = 0.f;
-#pragma unroll
-  for (int e = 0; e < kEnt; ++e)
-    if (32 * e < p.k && en.id[e] >= 0 && pr[e] != 0.f) kl = fmaf(pr[e], lp[e] - (en.x[e] - a.m) * p.inv_t + ln_z, kl);
-  kl = warp_sum(kl);
-  float loss = flags & kSoft ? (1.f - p.hard) * p.temperature * p.temperature * kl : 0.f;
-  if (HARD && (flags & kHard)) loss += p.hard * ((a.m == -INFINITY ? NAN : log2f(a.s1) * kLn2) - (xl - a.m));
-  return w * loss;
-}
-
-// The gradient of a row at a logit x: ks e^((x - m) / T) + kh e^(x - m), less `as` p for an entry and
-// `ah` for the label.
-struct Coef {
-  float m, c, ks, kh, as, ah;
+// A row's distributions (at T, and at 1 for the label) and the factors of its gradient
+//   ks 2^(c x - ref) + kh 2^(log2(e) x - ref1),  less `as` p at an entry and `ah` at the label.
+struct Row {
+  Log2P q, q1;
+  float s, s1, ks, kh, as, ah;
   template <bool HARD>
-  __device__ __forceinline__ float2 at(float2 x) const {
-    const float2 y = add2(x, f2s(-m)), d = mul2(y, f2s(c));
+  __device__ __forceinline__ float2 plain(float2 x) const {
+    const float2 d = fma2(x, f2s(q.c), f2s(-q.ref));
     float2 g = mul2(f2(ex2(d.x), ex2(d.y)), f2s(ks));
     if (HARD) {
-      const float2 d1 = mul2(y, f2s(kLog2e));
+      const float2 d1 = fma2(x, f2s(kLog2e), f2s(-q1.ref));
       g = fma2(f2(ex2(d1.x), ex2(d1.y)), f2s(kh), g);
     }
     return g;
   }
-  // at an entry of probability `a` and / or the label, each share less its own target
   template <bool HARD>
-  __device__ __forceinline__ float at_entry(float x, float a, bool label) const {
-    float g = ks * ex2((x - m) * c) - as * a;
-    if (HARD) g += kh * ex2((x - m) * kLog2e) - (label ? ah : 0.f);
-    return g;
+  __device__ __forceinline__ float dense(float x) const {
+    const float g = ks * ex2(q.exponent(x));
+    return HARD ? fmaf(kh, ex2(q1.exponent(x)), g) : g;
+  }
+  // At an entry given probability `a`, or the label: each share's probability less its target before the
+  // factor, so that equal ones cancel exactly.
+  template <bool HARD>
+  __device__ __forceinline__ float at(float x, float a, bool label) const {
+    const float g = as * (ex2(q.exponent(x)) / s - a);
+    return HARD ? g + ah * (ex2(q1.exponent(x)) / s1 - (label ? 1.f : 0.f)) : g;
   }
 };
 
-template <bool HARD>
-__device__ __forceinline__ Coef coefficients(const Params& p, const Part& a, int row, int flags, float w) {
-  float r = p.scale * w;
-  if (p.weight_sum) r /= *p.weight_sum;
-  if (p.upstream) r *= p.upstream[row * p.upstream_stride];
-  Coef g;
-  g.m = a.m;
-  g.c = p.inv_t * kLog2e;
-  g.as = flags & kSoft ? r * (1.f - p.hard) * p.temperature : 0.f;
-  g.ah = HARD && (flags & kHard) ? r * p.hard : 0.f;
-  g.ks = flags & kSoft ? g.as / a.s : 0.f;
-  g.kh = HARD && (flags & kHard) ? g.ah / a.s1 : 0.f;
-  if (flags & kBad) g.ks = NAN;
-  return g;
-}
-
 template <typename T, bool HARD>
-__device__ __forceinline__ uint4 grad_vec(const uint4& v, const Coef& k) {
+__device__ __forceinline__ uint4 grad_vec(const uint4& v, const Row& r) {
   float2 f[kVec<T> / 2];
   unpack<T>(v, f);
 #pragma unroll
-  for (int j = 0; j < kVec<T> / 2; ++j) f[j] = k.at<HARD>(f[j]);
+  for (int j = 0; j < kVec<T> / 2; ++j) f[j] = r.plain<HARD>(f[j]);
   if constexpr (sizeof(T) == 2)
     return make_uint4(f2bf(f[0]), f2bf(f[1]), f2bf(f[2]), f2bf(f[3]));
   else
     return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
 }
 
-// The E elements at g; `vec`: g is 16-byte aligned.
+// The E elements at g, whatever its alignment.
 template <typename T>
-__device__ __forceinline__ void store_vec(T* g, const uint4& u, bool vec, uint64_t policy) {
-  if (vec) {
-    store_stream(g, u, policy);
-    return;
-  }
+__device__ __forceinline__ void store_elements(T* g, const uint4& u) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int j = 0; j < kVec<T>; ++j) {
@@ -213,76 +131,155 @@ __device__ __forceinline__ void store_vec(T* g, const uint4& u, bool vec, uint64
   }
 }
 
-// Stores the gradient again at the entries (and the label) within [lo, hi), by the warp that holds
-// them.  An id that occurs twice (its bit in `seen`, hi - lo clear bits, is set already; without
-// `seen` it is always looked for) is stored once, with all its probabilities.  ids, amounts: k words of
-// shared memory for that search.
-template <typename T, bool HARD>
-__device__ __forceinline__ void store_entries(const Params& p, T* g, int lo, int hi, const Coef& k, const Entries& en,
-                                              const float (&pr)[kEnt], int64_t label, float xl, uint32_t* seen,
-                                              int* ids, float* amounts) {
+// ---- the teacher's entries, by the warp that holds them: entry lane + 32 e in place e of a lane ----
+template <int KE>
+struct Entries {
+  int id[KE];  // -1: absent
+  float x[KE], p[KE], lp[KE];  // logit; probability and its logarithm
+};
+
+enum { kSoft = 1, kHard = 2, kBad = 4 };  // a row's terms; kBad: an id or label past the vocabulary
+
+// Entry e, its id and teacher logit as they are given.  1: present, 2: bad.
+template <int KE>
+__device__ __forceinline__ int put_entry(Entries<KE>& en, int e, int64_t id, float t, int vocab) {
+  const bool there = id >= 0 && id < vocab;
+  en.id[e] = there ? (int)id : -1;
+  en.lp[e] = there ? t : -INFINITY;
+  return there ? 1 : id >= vocab ? 2 : 0;
+}
+// The row's terms from the `or` of put_entry over its entries.
+template <bool HARD>
+__device__ __forceinline__ int row_flags(const Params& p, int found, float w, int64_t label) {
+  found = __reduce_or_sync(0xffffffffu, found);
+  const bool bad = (found & 2) || (HARD && label >= p.vocab);
+  int f = (found && (!HARD || p.hard < 1.f) ? kSoft : 0) | (HARD && label >= 0 ? kHard : 0);
+  if (w == 0.f || !(f || bad)) return 0;
+  return bad ? kBad : f;
+}
+
+template <int KE>
+__device__ __forceinline__ void teacher_softmax(const Params& p, Entries<KE>& en) {
+  float tm = -INFINITY, es = 0.f;
+#pragma unroll
+  for (int e = 0; e < KE; ++e) tm = fmaxf(tm, en.lp[e]);
+  tm = warp_max(tm);
+#pragma unroll
+  for (int e = 0; e < KE; ++e) {
+    en.lp[e] = (en.lp[e] - tm) * p.inv_t;
+    en.p[e] = en.id[e] >= 0 ? ex2(en.lp[e] * kLog2e) : 0.f;
+    es += en.p[e];
+  }
+  es = warp_sum(es);
+  const float ls = log2f(es) * kLn2, inv = rcp_approx(es);
+#pragma unroll
+  for (int e = 0; e < KE; ++e) {
+    en.p[e] = en.id[e] >= 0 ? en.p[e] * inv : 0.f;
+    en.lp[e] -= ls;
+  }
+}
+
+template <bool HARD, int KE>
+__device__ __forceinline__ float row_loss(const Params& p, const Row& r, int flags, float w, const Entries<KE>& en,
+                                          float xl) {
+  if (flags == 0) return 0.f;
+  if (flags & kBad) return NAN;
+  float kl = 0.f;
+#pragma unroll
+  for (int e = 0; e < KE; ++e)  // an entry of probability 0 has no term
+    if (en.p[e] != 0.f) kl = fmaf(en.p[e], en.lp[e] - r.q.ln(en.x[e], p.inv_t), kl);
+  kl = warp_sum(kl);
+  float loss = flags & kSoft ? (1.f - p.hard) * p.temperature * p.temperature * kl : 0.f;
+  if (HARD && (flags & kHard)) loss -= p.hard * r.q1.ln(xl, 1.f);
+  return w * loss;
+}
+
+// `norm`: grad_scale over the mean's divisor.
+template <bool HARD>
+__device__ __forceinline__ Row make_row(const Params& p, const Part& a, bool plain, int row, int flags, float w, float norm) {
+  Row r;
+  r.s = a.s;
+  r.s1 = a.s1;
+  r.q = Log2P{plain, p.c, plain ? a.r : a.m, log2f(a.s)};
+  r.q1 = Log2P{plain, kLog2e, plain ? a.r1 : a.m, HARD ? log2f(a.s1) : 0.f};
+  float g = norm * w;
+  if (p.upstream) g *= p.upstream[row * p.upstream_stride];
+  r.as = flags & kSoft ? g * (1.f - p.hard) * p.temperature : 0.f;
+  r.ah = HARD && (flags & kHard) ? g * p.hard : 0.f;
+  r.ks = flags & kBad ? NAN : flags & kSoft ? r.as * rcp_approx(a.s) : 0.f;
+  r.kh = HARD && (flags & kHard) ? r.ah * rcp_approx(a.s1) : 0.f;
+  return r;
+}
+
+// Stores the gradient again at the entries (and the label) within [lo, hi).  An id that occurs twice (its
+// bit in `seen`, hi - lo clear bits, is set already; without `seen` it is always looked for) is stored once,
+// with all its probabilities.  ids, probs: k words each for that search.
+template <typename T, bool HARD, int KE>
+__device__ __forceinline__ void store_entries(const Params& p, T* g, int lo, int hi, const Row& r, int flags,
+                                              const Entries<KE>& en, int64_t label, float xl, uint32_t* seen, int* ids,
+                                              float* probs) {
   const int lane = threadIdx.x & 31;
-  const bool hard = HARD && k.ah != 0.f;
+  const bool hard = HARD && (flags & kHard);  // a share that is off has a factor of 0
   bool twice = seen == nullptr, hit = false;
 #pragma unroll
-  for (int e = 0; e < kEnt; ++e)
-    if (32 * e < p.k) {
-      const int id = en.id[e];
-      if (seen && id >= lo && id < hi) {
-        const uint32_t bit = 1u << ((id - lo) & 31);
-        twice |= (atomicOr(&seen[(id - lo) >> 5], bit) & bit) != 0u;
-      }
-      hit |= id >= 0 && id == label;
+  for (int e = 0; e < KE; ++e) {
+    const int id = en.id[e];
+    if (seen && id >= lo && id < hi) {
+      const uint32_t bit = 1u << ((id - lo) & 31);
+      twice |= (atomicOr(&seen[(id - lo) >> 5], bit) & bit) != 0u;
     }
+    hit |= id >= 0 && id == label;
+  }
   twice = __any_sync(0xffffffffu, twice);
   if (twice) {
 #pragma unroll
-    for (int e = 0; e < kEnt; ++e)
+    for (int e = 0; e < KE; ++e)
       if (lane + 32 * e < p.k) {
         ids[lane + 32 * e] = en.id[e];
-        amounts[lane + 32 * e] = pr[e];
+        probs[lane + 32 * e] = en.p[e];
       }
     __syncwarp();
   }
 #pragma unroll
-  for (int e = 0; e < kEnt; ++e)
-    if (32 * e < p.k) {
-      const int id = en.id[e];
-      bool first = id >= lo && id < hi;
-      float a = pr[e];
-      if (twice && first) {
-        a = 0.f;
-        for (int j = 0; j < p.k; ++j)
-          if (ids[j] == id) {
-            a += amounts[j];
-            if (j < lane + 32 * e) first = false;
-          }
-      }
-      if (first) stg<T>(g + id, k.at_entry<HARD>(en.x[e], a, id == label));
+  for (int e = 0; e < KE; ++e) {
+    const int id = en.id[e];
+    bool first = id >= lo && id < hi;
+    float a = en.p[e];
+    if (twice && first) {
+      a = 0.f;
+      for (int i = 0; i < p.k; ++i)
+        if (ids[i] == id) {
+          a += probs[i];
+          if (i < lane + 32 * e) first = false;
+        }
     }
+    if (first) stg<T>(g + id, r.at<HARD>(en.x[e], a, id == label));
+  }
   if (HARD) {
     hit = __any_sync(0xffffffffu, hit);
-    if (hard && !hit && lane == 0 && label >= lo && label < hi) stg<T>(g + label, k.at_entry<HARD>(xl, 0.f, true));
+    if (hard && !hit && lane == 0 && label >= lo && label < hi) stg<T>(g + label, r.at<HARD>(xl, 0.f, true));
   }
 }
 
 // ---- one CTA or one cluster per row -------------------------------------------------------
 template <int TB, bool GRAD>
-struct Smem {
+struct alignas(16) Smem {
   static constexpr int kSeen = GRAD ? 8 * TB : 4;  // a bit per element of a share of up to 256 TB
+  alignas(16) uint32_t seen[kSeen];                // cleared as 16-byte vectors
+  int ids[M3_MAX_TOP];
+  float probs[M3_MAX_TOP];
   Part part[TB / 32];
-  Part parts[kMaxCluster];
+  Part parts[kMaxCluster], again[kMaxCluster];
   int flags;
-  int ids[GRAD ? M3_MAX_TOP : 1];
-  float amounts[GRAD ? M3_MAX_TOP : 1];
-  alignas(16) uint32_t seen[kSeen];  // cleared as 16-byte vectors
 };
 
 template <typename T, int TB, bool HARD, bool GRAD>
 __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) {
-  constexpr int E = kVec<T>, NW = TB / 32;
+  constexpr int E = kVec<T>, NW = TB / 32, kTile = kNV * TB;
   using S = Smem<TB, GRAD>;
-  __shared__ S s;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  S& s = *reinterpret_cast<S*>(smem_raw);
+  uint4* cache = reinterpret_cast<uint4*>(smem_raw + sizeof(S));  // GRAD: the second tile
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int cl = p.cluster, rank = cl > 1 ? cluster_rank() : 0;
   const int row = (int)blockIdx.x >> p.log2_cluster;
@@ -291,191 +288,311 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   const Split sp = split_row(x, V);
   const int per = (sp.full + cl - 1) >> p.log2_cluster, v0 = min(sp.full, rank * per), n = min(per, sp.full - v0);
   const uint4* v = reinterpret_cast<const uint4*>(x + sp.head) + v0;
-  const float c = p.inv_t * kLog2e;
+  // this share's entries, its vectors' first
+  const int first = sp.head + v0 * E, lo = rank == 0 ? 0 : first, hi = rank == cl - 1 ? V : first + n * E;
+  const float c = p.c;
   if (cl > 1) cluster_arrive_relaxed();  // peers have started before anyone writes to their shared memory
 
   const float w = p.weights ? p.weights[row] : 1.f;
   const int64_t label = HARD ? p.labels[row] : -1;
-  Entries en;
-  float xl = 0.f, pr[kEnt], lp[kEnt];
-  const bool holder = warp == 0 && (GRAD || rank == 0);  // this warp holds the entries
+  float xl = 0.f;
+  const bool holder = warp == 0 && (GRAD || rank == 0);
+  Entries<kEnt> en;
   if (warp == 0) {
-    const int f = load_entries<HARD>(p, row, w, label, en);
-    if (lane == 0) s.flags = f;
-    if (holder) {  // read here: below, the gradient may overwrite the logits
+    int found = 0;
 #pragma unroll
-      for (int e = 0; e < kEnt; ++e) en.x[e] = 32 * e < p.k && en.id[e] >= 0 ? ld(x + en.id[e]) : 0.f;
-      if (HARD && label >= 0 && label < V) xl = ld(x + label);
+    for (int e = 0; e < kEnt; ++e) {
+      const int j = lane + 32 * e;
+      const bool there = j < p.k;
+      found |= put_entry(en, e, there ? p.ids[(int64_t)row * p.k + j] : -1, there ? p.teacher[(int64_t)row * p.k + j] : 0.f, V);
     }
+    const int f = row_flags<HARD>(p, found, w, label);
+    if (lane == 0) s.flags = f;
+    // read here: below, the gradient may overwrite the logits
+#pragma unroll
+    for (int e = 0; e < kEnt; ++e) en.x[e] = en.id[e] >= 0 ? ld(x + en.id[e]) : 0.f;
+    if (HARD && label >= 0 && label < V) xl = ld(x + label);
   }
   if constexpr (GRAD)
     for (int i = tid; i < S::kSeen / 4; i += TB) reinterpret_cast<uint4*>(s.seen)[i] = make_uint4(0u, 0u, 0u, 0u);
 
-  float m = -INFINITY;  // the warp's maximum
+  float m = -INFINITY, ref = kLowRef, ref1 = kLowRef;  // the warp's maximum and references
   float2 s2 = f2s(0.f), t2 = f2s(0.f);
   auto raise = [&](float to) {  // the sums against a new maximum
     if (to > m) {
-      if (m != -INFINITY) {
-        s2 = mul2(s2, f2s(ex2((m - to) * c)));
-        if (HARD) t2 = mul2(t2, f2s(ex2((m - to) * kLog2e)));
-      }
       m = to;
+      const float r = ref_of(m, c);
+      s2 = mul2(s2, f2s(ex2(ref - r)));
+      ref = r;
+      if (HARD) {
+        const float r1 = ref_of(m, kLog2e);
+        t2 = mul2(t2, f2s(ex2(ref1 - r1)));
+        ref1 = r1;
+      }
     }
   };
-  walk<T, kNV, TB>(v, n, tid, GRAD ? Keep::kYes : Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
+  const uint64_t policy = l2_policy(GRAD ? Keep::kYes : Keep::kNo);
+  uint4 d[kNV];
+  auto load = [&](int base, uint64_t pol) {
+#pragma unroll
+    for (int j = 0; j < kNV; ++j) d[j] = load_stream(v + base + tid + j * TB, pol);
+  };
+  auto sum = [&](int base, auto full) {
     VecMax<T> vm[kNV];
     const float mt = vecs_max<T, kNV>(d, vm, [&](int j) { return full.value || base + j * TB < n; });
     raise(warp_max(mt));
-    const float ref = finite_or_0(m);
 #pragma unroll
     for (int j = 0; j < kNV; ++j)
-      if (full.value || base + j * TB < n) add_vec<T, HARD>(d[j], ref, c, s2, t2);
-  });
+      if (full.value || base + j * TB < n) add_vec<T, HARD>(d[j], ref, ref1, c, s2, t2);
+  };
+  auto load_rest = [&](int base, uint64_t pol) {
+#pragma unroll
+    for (int j = 0; j < kNV; ++j) {
+      const int i = base + j * TB + tid;
+      d[j] = neg_inf_vec<T>();
+      if (i < n) d[j] = load_stream(v + i, pol);
+    }
+  };
+  // the ragged tile first, then the full ones down to tile 0, which stays in d
+  const int tiles = n / kTile, rest = tiles * kTile;
+  if (rest < n) {
+    load_rest(rest, policy);
+    sum(rest, Flag<false>());
+  }
+  for (int t = tiles - 1; t >= 0; --t) {
+    load(t * kTile, policy);
+    sum(t * kTile, Flag<true>());
+    if (GRAD && t == 1) {
+#pragma unroll
+      for (int j = 0; j < kNV; ++j) cache[j * TB + tid] = d[j];
+    }
+  }
   int edge = -1;  // this lane's element of the row's edges
   float xe = -INFINITY;
   if (warp == NW - 1) {
     edge = edge_index(sp, lane, rank == 0, rank == cl - 1);
     if (edge >= 0) xe = ld(x + edge);
     raise(warp_max(xe));
-    s2.x += ex2((xe - finite_or_0(m)) * c);
-    if (HARD) t2.x += ex2((xe - finite_or_0(m)) * kLog2e);
+    s2.x += ex2(fmaf(xe, c, -ref));
+    if (HARD) t2.x += ex2(fmaf(xe, kLog2e, -ref1));
   }
-  Part a{m, warp_sum(s2.x + s2.y), HARD ? warp_sum(t2.x + t2.y) : 0.f};
+  Part a{m, ref, warp_sum(s2.x + s2.y), ref1, HARD ? warp_sum(t2.x + t2.y) : 0.f};
   if (lane == 0) s.part[warp] = a;
-  if (holder) teacher_softmax(p, en, pr, lp);
+  if (holder) teacher_softmax(p, en);
   __syncthreads();
-  const Part none{-INFINITY, 0.f, 0.f};
-  a = join<HARD>(lane < NW ? s.part[lane] : none, c);
-  if (cl > 1) {
+  a = join<HARD>(lane < NW ? s.part[lane] : no_part());
+  auto exchange = [&](Part(&parts)[kMaxCluster], const Part& none) {
     __syncwarp();
-    cluster_wait();
-    if (tid < cl) *peer(&s.parts[rank], tid) = a;
+    if (tid < cl) *peer(&parts[rank], tid) = a;
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    a = join<HARD>(lane < cl ? s.parts[lane] : none, c);
+    a = join<HARD>(lane < cl ? parts[lane] : none);
+  };
+  if (cl > 1) {
+    __syncwarp();
+    cluster_wait();
+    exchange(s.parts, no_part());
+  }
+  const bool plain = fabsf(a.m) * fmaxf(c, kLog2e) <= p.plain_most;
+  if (!plain) {  // the same for all threads of the row
+    const Part none{a.m, 0.f, 0.f, 0.f, 0.f};
+    a = slow_part(x, lo, hi, tid, TB, a.m, c);
+    a.s = warp_sum(a.s);
+    a.s1 = warp_sum(a.s1);
+    __syncthreads();
+    if (lane == 0) s.part[warp] = a;
+    __syncthreads();
+    a = join<HARD>(lane < NW ? s.part[lane] : none);
+    if (cl > 1) exchange(s.again, none);
+    a.m = none.m;
   }
   const int flags = s.flags;
+  float norm = p.scale;
+  if (GRAD && p.weight_sum) norm /= *p.weight_sum;
+  const Row r = make_row<HARD>(p, a, plain, row, flags, w, norm);
   if (warp == 0 && rank == 0) {
-    const float loss = row_loss<HARD>(p, a, flags, w, en, pr, lp, xl);
+    const float loss = row_loss<HARD>(p, r, flags, w, en, xl);
     if (lane == 0) p.row_loss[row] = loss;
   }
   if constexpr (GRAD) {
     T* g = reinterpret_cast<T*>(p.grad) + p.grow.at(row);
-    T* gv = g + sp.head + v0 * E;  // this share's vectors, aligned or not
-    const bool vec = row_shift(gv) == 0;
-    const Coef k = coefficients<HARD>(p, a, row, flags, w);
-    const uint64_t first = l2_policy(Keep::kNo);
-    if (flags) {
-      walk<T, kNV, TB>(v, n, tid, Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
-#pragma unroll
-        for (int j = 0; j < kNV; ++j) {
-          const int q = base + j * TB + tid;
-          if (full.value || base + j * TB < n) {
-            const uint4 u = grad_vec<T, HARD>(d[j], k);
-            if (full.value || q < n) store_vec<T>(gv + (int64_t)q * E, u, vec, first);
-          }
-        }
-      });
+    T* gv = g + first;  // this share's vectors
+    const uint64_t go = l2_policy(Keep::kNo);
+    if (flags == 0) {
+      for (int i = lo + tid; i < hi; i += TB) stg<T>(g + i, 0.f);
+    } else if (!plain) {
+      for (int i = lo + tid; i < hi; i += TB) stg<T>(g + i, r.dense<HARD>(ld(x + i)));
     } else {
-      for (int q = tid; q < n; q += TB) store_vec<T>(gv + (int64_t)q * E, make_uint4(0u, 0u, 0u, 0u), vec, first);
+      auto write = [&](int b, auto full, auto aligned) {
+#pragma unroll
+        for (int j = 0; j < kNV; ++j)
+          if (full.value || b + j * TB < n) {
+            const uint4 u = grad_vec<T, HARD>(d[j], r);
+            if (full.value || b + j * TB + tid < n) {
+              if (aligned.value)
+                store_stream(reinterpret_cast<uint4*>(gv) + b + tid + j * TB, u, go);
+              else
+                store_elements(gv + (int64_t)(b + tid + j * TB) * E, u);
+            }
+          }
+      };
+      auto walk_again = [&](auto aligned) {
+        if (tiles > 0) write(0, Flag<true>(), aligned);
+        if (tiles > 1) {
+#pragma unroll
+          for (int j = 0; j < kNV; ++j) d[j] = cache[j * TB + tid];
+          write(kTile, Flag<true>(), aligned);
+        }
+        for (int t = 2; t < tiles; ++t) {
+          load(t * kTile, go);
+          write(t * kTile, Flag<true>(), aligned);
+        }
+        if (rest < n) {
+          if (tiles > 0) load_rest(rest, go);
+          write(rest, Flag<false>(), aligned);
+        }
+      };
+      if (row_shift(gv) == 0)
+        walk_again(Flag<true>());
+      else
+        walk_again(Flag<false>());
+      if (edge >= 0) stg<T>(g + edge, r.plain<HARD>(f2s(xe)).x);
     }
-    if (edge >= 0) stg<T>(g + edge, flags ? k.at<HARD>(f2s(xe)).x : 0.f);
     __syncthreads();
-    if (warp == 0 && flags && !(flags & kBad)) {
-      const int lo = rank == 0 ? 0 : sp.head + v0 * E, hi = rank == cl - 1 ? V : sp.head + (v0 + n) * E;
-      store_entries<T, HARD>(p, g, lo, hi, k, en, pr, label, xl, hi - lo <= 32 * S::kSeen ? s.seen : nullptr, s.ids,
-                             s.amounts);
-    }
+    if (warp == 0 && flags && !(flags & kBad))
+      store_entries<T, HARD>(p, g, lo, hi, r, flags, en, label, xl, hi - lo <= 32 * S::kSeen ? s.seen : nullptr, s.ids,
+                             s.probs);
   }
 }
 
 // ---- one warp per row ---------------------------------------------------------------------
-constexpr int kWarpThreads = 256, kWarpRows = kWarpThreads / 32;
+// A warp takes `batch` (at most 32) rows one after the other, the next one's vectors and entries on
+// their way; lane i keeps row i's weight, label and loss.
+constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
 
-template <typename T, int NV, bool HARD, bool GRAD>
-__global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params p) {
-  constexpr int E = kVec<T>, kSeen = NV * E;  // words of 32 bits: one bit per element
-  __shared__ uint4 row_of[kWarpRows][NV * 32];
-  __shared__ uint32_t seen_of[kWarpRows][GRAD ? kSeen : 1];
-  __shared__ int ids_of[kWarpRows][GRAD ? M3_MAX_TOP : 1];
-  __shared__ float amounts_of[kWarpRows][GRAD ? M3_MAX_TOP : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, V = p.vocab;
-  const int step = gridDim.x * kWarpRows;
-  const float c = p.inv_t * kLog2e;
-  int row = blockIdx.x * kWarpRows + warp;
+template <typename T, int NV, bool GRAD>
+struct alignas(16) WarpSmem {
+  uint4 row[NV * 32];
+  int ids[GRAD ? M3_MAX_TOP : 1];
+  float probs[GRAD ? M3_MAX_TOP : 1];
+  uint32_t seen[GRAD ? NV * kVec<T> : 1];  // a bit per element
+};
+
+// KE: 1 for up to 32 entries, which are most lists, else kEnt.
+template <typename T, int NV, int KE, bool HARD, bool GRAD>
+__global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params p, int batch) {
+  constexpr int E = kVec<T>;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  WarpSmem<T, NV, GRAD>& s = reinterpret_cast<WarpSmem<T, NV, GRAD>*>(smem_raw)[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31, V = p.vocab;
+  const float c = p.c;
+  const int row0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * batch, rows = min(batch, p.rows - row0);
+  if (rows <= 0) return;
+  const float w_all = lane < rows && p.weights ? p.weights[row0 + lane] : 1.f;
+  const int64_t label_all = HARD && lane < rows ? p.labels[row0 + lane] : -1;
+  const float norm = GRAD && p.weight_sum ? p.scale / *p.weight_sum : p.scale;
   uint4 d[NV];
   int shift = 0;
-  auto load = [&](int r) {
-    const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(r);
+  int64_t id[KE];
+  float t[KE];
+  auto load = [&](int row) {
+    const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
     shift = row_shift(x);
+    const bool whole = shift == 0 && V % E == 0;  // no ragged vector
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int lo = (j * 32 + lane) * E - shift;
-      d[j] = lo < V ? load_vec(x, lo, V) : neg_inf_vec<T>();
+      d[j] = neg_inf_vec<T>();
+      if (whole) {
+        if (lo < V) d[j] = load_once(reinterpret_cast<const uint4*>(x + lo));
+      } else if (lo < V) {
+        d[j] = load_vec(x, lo, V);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < KE; ++e) {
+      const int j = lane + 32 * e;
+      id[e] = j < p.k ? p.ids[(int64_t)row * p.k + j] : -1;
+      t[e] = j < p.k ? p.teacher[(int64_t)row * p.k + j] : 0.f;
     }
   };
-  if (row < p.rows) load(row);
-  for (; row < p.rows; row += step) {
-    const float w = p.weights ? p.weights[row] : 1.f;
-    const int64_t label = HARD ? p.labels[row] : -1;
-    Entries en;
-    const int flags = load_entries<HARD>(p, row, w, label, en);
-    float m = -INFINITY;
+  load(row0);
+  float loss_all = 0.f;
+  for (int i = 0; i < rows; ++i) {
+    const int row = row0 + i, at = shift;
+    const float w = __shfl_sync(0xffffffffu, w_all, i);
+    const int64_t label = HARD ? __shfl_sync(0xffffffffu, label_all, i) : -1;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      row_of[warp][j * 32 + lane] = d[j];
-    }
-    VecMax<T> vm[NV];
-    m = vecs_max<T, NV>(d, vm, [](int) { return true; });
+    for (int j = 0; j < NV; ++j) s.row[j * 32 + lane] = d[j];
     if (GRAD)
-      for (int i = lane; i < kSeen; i += 32) seen_of[warp][i] = 0u;
-    m = warp_max(m);
-    const float ref = finite_or_0(m);
+      for (int j = lane; j < NV * E; j += 32) s.seen[j] = 0u;
+    Part a = no_part();
+    VecMax<T> vm[NV];
+    a.m = warp_max(vecs_max<T, NV>(d, vm, [](int) { return true; }));
+    a.r = ref_of(a.m, c);
+    a.r1 = ref_of(a.m, kLog2e);
     float2 s2 = f2s(0.f), t2 = f2s(0.f);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) add_vec<T, HARD>(d[j], ref, c, s2, t2);
+    for (int j = 0; j < NV; ++j) add_vec<T, HARD>(d[j], a.r, a.r1, c, s2, t2);
     __syncwarp();
-    const T* xs = reinterpret_cast<const T*>(row_of[warp]) + shift;
+    const T* xs = reinterpret_cast<const T*>(s.row) + at;
+    Entries<KE> en;
+    int found = 0;
 #pragma unroll
-    for (int e = 0; e < kEnt; ++e) en.x[e] = 32 * e < p.k && en.id[e] >= 0 ? ld(xs + en.id[e]) : 0.f;
-    const float xl = HARD && label >= 0 && label < V ? ld(xs + label) : 0.f;
-    float pr[kEnt], lp[kEnt];
-    teacher_softmax(p, en, pr, lp);
-    const Part a{m, warp_sum(s2.x + s2.y), HARD ? warp_sum(t2.x + t2.y) : 1.f};
-    const float loss = row_loss<HARD>(p, a, flags, w, en, pr, lp, xl);
-    if (lane == 0) p.row_loss[row] = loss;
-    const int at = shift;
-    uint4 u[GRAD ? NV : 1];
-    Coef k;
-    if constexpr (GRAD) {
-      k = coefficients<HARD>(p, a, row, flags, w);
-#pragma unroll
-      for (int j = 0; j < NV; ++j) u[j] = flags ? grad_vec<T, HARD>(d[j], k) : make_uint4(0u, 0u, 0u, 0u);
+    for (int e = 0; e < KE; ++e) {
+      found |= put_entry(en, e, id[e], t[e], V);
+      en.x[e] = en.id[e] >= 0 ? ld(xs + en.id[e]) : 0.f;
     }
-    if (row + step < p.rows) load(row + step);  // on its way while this row is finished
+    const int flags = row_flags<HARD>(p, found, w, label);
+    const float xl = HARD && label >= 0 && label < V ? ld(xs + label) : 0.f;
+    teacher_softmax(p, en);
+    a.s = warp_sum(s2.x + s2.y);
+    a.s1 = HARD ? warp_sum(t2.x + t2.y) : 1.f;
+    const bool plain = fabsf(a.m) * fmaxf(c, kLog2e) <= p.plain_most;
+    if (!plain) {
+      a = slow_part(xs, 0, V, lane, 32, a.m, c);
+      a.s = warp_sum(a.s);
+      a.s1 = warp_sum(a.s1);
+    }
+    const Row r = make_row<HARD>(p, a, plain, row, flags, w, norm);
+    const float loss = row_loss<HARD>(p, r, flags, w, en, xl);
+    if (lane == i) loss_all = loss;
     if constexpr (GRAD) {
       T* g = reinterpret_cast<T*>(p.grad) + p.grow.at(row);
-      const bool vec = row_shift(g) == at;
-      const uint64_t first = l2_policy(Keep::kNo);
+      if (flags == 0) {
+        for (int e = lane; e < V; e += 32) stg<T>(g + e, 0.f);
+      } else if (!plain) {
+        for (int e = lane; e < V; e += 32) stg<T>(g + e, r.dense<HARD>(ld(xs + e)));
+      } else {
+        const bool aligned = row_shift(g) == at;
+        const uint64_t go = l2_policy(Keep::kNo);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int lo = (j * 32 + lane) * E - at;
-        if (lo >= 0 && lo + E <= V) {
-          store_vec<T>(g + lo, u[j], vec, first);
-        } else if (lo < V) {
-          const T* e = reinterpret_cast<const T*>(&u[j]);
+        for (int j = 0; j < NV; ++j) {
+          const int lo = (j * 32 + lane) * E - at;
+          const uint4 u = grad_vec<T, HARD>(d[j], r);
+          if (lo >= 0 && lo + E <= V) {
+            if (aligned)
+              store_stream(g + lo, u, go);
+            else
+              store_elements(g + lo, u);
+          } else if (lo < V) {
+            const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-          for (int i = 0; i < E; ++i)
-            if (lo + i >= 0 && lo + i < V) g[lo + i] = e[i];
+            for (int q = 0; q < E; ++q)
+              if (lo + q >= 0 && lo + q < V) g[lo + q] = e[q];
+          }
         }
       }
+      if (i + 1 < rows) load(row + 1);
       __syncwarp();
-      if (flags && !(flags & kBad))
-        store_entries<T, HARD>(p, g, 0, V, k, en, pr, label, xl, seen_of[warp], ids_of[warp], amounts_of[warp]);
+      if (flags && !(flags & kBad)) store_entries<T, HARD>(p, g, 0, V, r, flags, en, label, xl, s.seen, s.ids, s.probs);
+    } else {
+      if (i + 1 < rows) load(row + 1);
     }
     __syncwarp();  // the row's shared memory is free again
   }
+  if (lane < rows) p.row_loss[row0 + lane] = loss_all;
 }
 
 // out = scale * (sum of n values) / (*div_by, if given), by one cluster in a fixed order.
@@ -524,15 +641,47 @@ int launch_cta(const Params& p, cudaStream_t s) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  constexpr size_t kSmem = sizeof(Smem<TB, GRAD>) + (GRAD ? sizeof(uint4) * kNV * TB : 0);
+  if constexpr (kSmem > 48 * 1024) {
+    static bool done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !done[dev]) {
+      if (cudaFuncSetAttribute(distill_kernel<T, TB, HARD, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)kSmem) != cudaSuccess)
+        return check_launch("m3_distill: cudaFuncSetAttribute");
+      if (dev < 64) done[dev] = true;
+    }
+  }
+  cfg.dynamicSmemBytes = kSmem;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_kernel<T, TB, HARD, GRAD>, p);
   return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_distill: ") + cudaGetErrorString(e));
 }
 
+template <typename T, int NV, int KE, bool HARD, bool GRAD>
+int launch_warp_k(const Params& p, cudaStream_t s) {
+  const int batch = warp_batch(p.rows, sm_count());
+  const int warps = (p.rows + batch - 1) / batch;
+  constexpr size_t kSmem = kWarps * sizeof(WarpSmem<T, NV, GRAD>);
+  if constexpr (kSmem > 48 * 1024) {
+    static bool done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !done[dev]) {
+      if (cudaFuncSetAttribute(distill_warp_kernel<T, NV, KE, HARD, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)kSmem) != cudaSuccess)
+        return check_launch("m3_distill: cudaFuncSetAttribute");
+      if (dev < 64) done[dev] = true;
+    }
+  }
+  distill_warp_kernel<T, NV, KE, HARD, GRAD>
+      <<<(unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, kSmem, s>>>(p, batch);
+  return check_launch("m3_distill");
+}
+
 template <typename T, int NV, bool HARD, bool GRAD>
 int launch_warp(const Params& p, cudaStream_t s) {
-  const int want = (p.rows + kWarpRows - 1) / kWarpRows, most = sm_count() * 8;
-  distill_warp_kernel<T, NV, HARD, GRAD><<<(unsigned)(want < most ? want : most), kWarpThreads, 0, s>>>(p);
-  return check_launch("m3_distill");
+  return p.k <= 32 ? launch_warp_k<T, NV, 1, HARD, GRAD>(p, s) : launch_warp_k<T, NV, kEnt, HARD, GRAD>(p, s);
 }
 
 // A row goes to a warp while its vectors fit the lanes' registers, else to a CTA, and with few rows to
@@ -550,11 +699,11 @@ int launch(Params p, int nvec, cudaStream_t s) {
   p.cluster = cl;
   while ((1 << p.log2_cluster) < cl) ++p.log2_cluster;
   if ((int64_t)p.rows * cl > 0x7FFFFFFF) return set_error(M3_ERR_SHAPE, "m3_distill: too many rows");
-  // a second walk finds its row in L2 only while the rows in flight (1024 / threads per SM) fit there
-  if (nvec <= kNV * 128 * cl) return launch_cta<T, 128, HARD, GRAD>(p, s);
-  const bool fits = (int64_t)nvec * 16 * 4 * sms <= (int64_t)64 << 20;
-  return (GRAD && !fits) || (int64_t)p.rows * cl <= 2 * sms ? launch_cta<T, 512, HARD, GRAD>(p, s)
-                                                             : launch_cta<T, 256, HARD, GRAD>(p, s);
+  // the fewest threads for which two tiles are the row; longer rows are read again from L2, which holds
+  // the rows in flight of two CTAs per SM better than of four
+  if (nvec <= 2 * kNV * 128 * cl) return launch_cta<T, 128, HARD, GRAD>(p, s);
+  if (nvec <= 2 * kNV * 256 * cl && (int64_t)p.rows * cl > 2 * sms) return launch_cta<T, 256, HARD, GRAD>(p, s);
+  return launch_cta<T, 512, HARD, GRAD>(p, s);
 }
 
 template <typename T>
@@ -601,6 +750,8 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
   p.k = a.k;
   p.temperature = a.temperature;
   p.inv_t = 1.f / a.temperature;
+  p.c = kLog2e / a.temperature;
+  p.plain_most = plain_most(p.c);
   p.hard = a.hard_weight;
   p.scale = a.grad_scale;
   if (a.reduction == M3_REDUCE_MEAN && !a.weights) p.scale /= (float)rows;

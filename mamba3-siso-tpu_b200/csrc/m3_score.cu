@@ -542,9 +542,7 @@ int launch_cta(const Params& p, cudaStream_t s) {
 
 template <typename T, int NV, bool TOP>
 int launch_warp(const Params& p, cudaStream_t s) {
-  // batches as long as 32 warps on every SM have one
-  int batch = p.rows / (sm_count() * 32);
-  batch = batch < 1 ? 1 : batch > 32 ? 32 : batch;
+  const int batch = warp_batch(p.rows, sm_count());
   const int warps = (p.rows + batch - 1) / batch;
   score_warp_kernel<T, NV, TOP><<<(unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, 0, s>>>(p, batch);
   return check_launch("m3_token_logprobs");

@@ -18,6 +18,13 @@ inline int most_vectors(const void* x, int n, int size, int64_t outer, int64_t i
   return (shift + n + e - 1) / e;
 }
 
+// Rows a warp takes: several waves of CTAs, so that the last one costs little (at 27 rows a warp,
+// 131072 rows were 607 CTAs for 592 places, and took 142 us instead of 85).
+inline int warp_batch(int rows, int sms) {
+  const int batch = rows / (sms * 128);
+  return batch < 1 ? 1 : batch > 32 ? 32 : batch;
+}
+
 // n / d for 0 <= n < 2^31, 1 <= d < 2^31, by one multiplication: with s = ceil(log2 d) and
 // m = ceil(2^(31 + s) / d) < 2^32, m d exceeds 2^(31 + s) by less than d <= 2^s,
 // so n m / 2^(31 + s) exceeds n / d by less than 1 / d.
