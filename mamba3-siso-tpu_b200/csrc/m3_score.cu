@@ -84,6 +84,18 @@ __device__ __forceinline__ void write_target(const Params& p, const Log2P& q, in
   p.logprob[row] = t < 0 ? 0.f : t >= p.vocab ? NAN : q.ln(xt, p.inv_t);
 }
 
+// Everything a row has but its alternatives, by one thread.
+template <typename T>
+__device__ __forceinline__ void finish_row(const Params& p, const Part& a, int row) {
+  const Log2P q = distribution(a, fabsf(a.m) * p.c <= p.plain_most, p.c);
+  write_row(p, a, q, row);
+  if (p.targets) {
+    const int64_t t = p.targets[p.trow.at(row)];
+    const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
+    write_target(p, q, row, t, t >= 0 && t < p.vocab ? ld(x + t) : 0.f);
+  }
+}
+
 // ---- one CTA or one cluster per row -------------------------------------------------------
 template <int NW, bool TOP>
 struct Smem {
@@ -104,22 +116,38 @@ struct Smem<NW, true> {
   int count[NW];
 };
 
-// The `need` first of the entries [lo, hi) in the order of rank_word, unsorted, by selection on the
-// bits of the key and then of the index.  All threads of the CTA.
-template <typename T, int TB, typename S>
-__device__ __noinline__ void exact_top(const T* x, int lo, int hi, int need, S& s) {
-  constexpr int NW = TB / 32;
-  const int tid = threadIdx.x;
-  auto count = [&](auto pred) {
-    int n = 0;
-    for (int i = lo + tid; i < hi; i += TB) n += pred(key_of(ld(x + i)), i) ? 1 : 0;
+// The threads that work on a share together.
+template <int TB, typename S>
+struct CtaGroup {
+  S& s;
+  static constexpr int kSize = TB;
+  __device__ __forceinline__ int id() const { return threadIdx.x; }
+  __device__ __forceinline__ void sync() const { __syncthreads(); }
+  __device__ __forceinline__ int sum(int n) const {
     n = __reduce_add_sync(0xffffffffu, n);
     __syncthreads();
-    if ((tid & 31) == 0) s.count[tid >> 5] = n;
+    if ((threadIdx.x & 31) == 0) s.count[threadIdx.x >> 5] = n;
     __syncthreads();
     n = 0;
-    for (int w = 0; w < NW; ++w) n += s.count[w];
+    for (int w = 0; w < TB / 32; ++w) n += s.count[w];
     return n;
+  }
+};
+struct WarpGroup {
+  static constexpr int kSize = 32;
+  __device__ __forceinline__ int id() const { return threadIdx.x & 31; }
+  __device__ __forceinline__ void sync() const { __syncwarp(); }
+  __device__ __forceinline__ int sum(int n) const { return __reduce_add_sync(0xffffffffu, n); }
+};
+
+// The `need` first of the entries [lo, hi) in the order of rank_word into cand[0, need), unsorted, by
+// selection on the bits of the key and then of the index.  All threads of the group; n_cand: shared.
+template <typename T, typename G>
+__device__ __noinline__ void exact_top(const T* x, int lo, int hi, int need, uint64_t* cand, int* n_cand, G g) {
+  auto count = [&](auto pred) {
+    int n = 0;
+    for (int i = lo + g.id(); i < hi; i += G::kSize) n += pred(key_of(ld(x + i)), i) ? 1 : 0;
+    return g.sum(n);
   };
   uint32_t key = 0;  // the need-th largest key
   for (int b = 31; b >= 0; --b) {
@@ -132,14 +160,14 @@ __device__ __noinline__ void exact_top(const T* x, int lo, int hi, int need, S& 
     const int t = last | (1 << b);
     if (count([&](uint32_t k, int i) { return k == key && i < t; }) < ties) last = t;
   }
-  if (tid == 0) s.n_cand = 0;
-  __syncthreads();
-  for (int i = lo + tid; i < hi; i += TB) {
+  if (g.id() == 0) *n_cand = 0;
+  g.sync();
+  for (int i = lo + g.id(); i < hi; i += G::kSize) {
     const float v = ld(x + i);
     const uint32_t k = key_of(v);
-    if (k > key || (k == key && i <= last)) s.cand[atomicAdd(&s.n_cand, 1)] = rank_word(v, i);
+    if (k > key || (k == key && i <= last)) cand[atomicAdd(n_cand, 1)] = rank_word(v, i);
   }
-  __syncthreads();
+  g.sync();
 }
 
 template <typename T, int TB, bool TOP>
@@ -259,7 +287,7 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
     __syncthreads();
     // the sum is NaN iff the share holds NaN or +inf, which the comparisons above do not order
     if (nv > kVecCap || s.n_cand > kCandCap || a.s != a.s) {
-      exact_top<T, TB>(x, lo, hi, min(k, hi - lo), s);
+      exact_top(x, lo, hi, min(k, hi - lo), s.cand, &s.n_cand, CtaGroup<TB, Smem<NW, TOP>>{s});
     }
     const int nc = s.n_cand;
     uint64_t* list = s.list[rank];
@@ -505,16 +533,155 @@ __global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p
       }
     }
   }
-  if (lane < rows) {
-    const int row = row0 + lane;
-    const Log2P q = distribution(keep, fabsf(keep.m) * c <= p.plain_most, c);
-    write_row(p, keep, q, row);
-    if (p.targets) {
-      const int64_t t = p.targets[p.trow.at(row)];
-      const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
-      write_target(p, q, row, t, t >= 0 && t < V ? ld(x + t) : 0.f);
+  if (lane < rows) finish_row<T>(p, keep, row0 + lane);
+}
+
+// ---- one warp per longer row --------------------------------------------------------------
+// The CTA's walk by a single warp, without barriers: rows of up to some thousand entries are over too
+// soon for a CTA's.  BEST: 0 without alternatives; else the bound is the top-th largest of every lane's BEST
+// largest vector maxima (1 for up to 8 alternatives; 2 for up to 32, where the lanes' maxima alone would
+// let a hundred candidates through and overflow the lists).
+constexpr int kRowVecCap = 96, kRowCandCap = 128, kRowMostTop = 32;
+
+struct RowSmem {
+  uint4 vec[kRowVecCap];
+  int vec_at[kRowVecCap];
+  uint64_t cand[kRowCandCap];
+  int n_cand;
+};
+
+template <typename T, int BEST>
+__global__ void __launch_bounds__(kWarpThreads) score_rows_kernel(const Params p, int batch) {
+  constexpr int E = kVec<T>;
+  constexpr bool TOP = BEST > 0;
+  __shared__ RowSmem smem[TOP ? kWarps : 1];
+  RowSmem& s = smem[TOP ? threadIdx.x >> 5 : 0];
+  const int lane = threadIdx.x & 31, V = p.vocab, k = p.top;
+  const unsigned lt = (1u << lane) - 1u;
+  const float c = p.c;
+  const int row0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * batch, rows = min(batch, p.rows - row0);
+  if (rows <= 0) return;
+  Part keep = no_part();
+  for (int i = 0; i < rows; ++i) {
+    const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row0 + i);
+    const Split sp = split_row(x, V);
+    const uint4* v = reinterpret_cast<const uint4*>(x + sp.head);
+    const int n = sp.full;
+    float m = -INFINITY, ref = kLowRef, best[2] = {-INFINITY, -INFINITY}, bound = -INFINITY;
+    float2 s2 = f2s(0.f), u2 = f2s(0.f);
+    int nv = 0, nc = 0;  // vectors and candidates put aside
+    auto raise = [&](float to) {
+      if (to > m) {
+        m = to;
+        const float r = ref_of(m, c), dr = ref - r, e = ex2(dr);
+        u2 = mul2(fma2(s2, f2s(dr), u2), f2s(e));
+        s2 = mul2(s2, f2s(e));
+        ref = r;
+      }
+    };
+    walk<T, kNV, 32>(v, n, lane, Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
+      VecMax<T> vm[kNV];
+      const float mt = vecs_max<T, kNV>(d, vm, [&](int j) { return full.value || base + j * 32 < n; });
+      raise(warp_max(mt));
+#pragma unroll
+      for (int j = 0; j < kNV; ++j)
+        if (full.value || base + j * 32 < n) add_vec<T>(d[j], ref, c, s2, u2);
+      if constexpr (TOP) {
+        bool higher;  // a change of the top-th largest
+        if (BEST == 1) {
+          higher = mt > best[0] && mt > bound;
+          best[0] = fmaxf(best[0], mt);
+        } else {
+          const float before = best[1];
+#pragma unroll
+          for (int j = 0; j < kNV; ++j)
+            if (full.value || base + j * 32 < n) {
+              const float f = vm[j].value();
+              best[1] = fmaxf(best[1], fminf(best[0], f));
+              best[0] = fmaxf(best[0], f);
+            }
+          higher = mt > before && mt > bound;
+        }
+        if (__any_sync(0xffffffffu, higher)) {
+          float left = best[0], next = BEST > 1 ? best[1] : -INFINITY;
+          for (int q = 0; q < k; ++q) {
+            bound = warp_max(left);
+            const unsigned at = __ballot_sync(0xffffffffu, left == bound);
+            if (lane == __ffs(at) - 1) {
+              left = next;
+              next = -INFINITY;
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, mt >= bound)) {
+#pragma unroll
+          for (int j = 0; j < kNV; ++j) {
+            if (!full.value && base + j * 32 >= n) break;
+            const bool put = (full.value || base + j * 32 + lane < n) && vm[j].reaches(bound);
+            const unsigned who = __ballot_sync(0xffffffffu, put);
+            const int at = nv + __popc(who & lt);
+            if (put && at < kRowVecCap) {
+              s.vec[at] = d[j];
+              s.vec_at[at] = base + j * 32 + lane;
+            }
+            nv += __popc(who);
+          }
+        }
+      }
+    });
+    {
+      const int q = edge_index(sp, lane, true, true);
+      const float xe = q >= 0 ? ld(x + q) : -INFINITY;
+      raise(warp_max(xe));
+      const float d = fmaf(xe > -1e30f || xe != xe ? xe : -1e30f, c, -ref), e = ex2(d);
+      s2.x += e;
+      u2.x = fmaf(e, d, u2.x);
+      if constexpr (TOP) {
+        const unsigned who = __ballot_sync(0xffffffffu, q >= 0);
+        if (q >= 0) s.cand[__popc(who & lt)] = rank_word(xe, q);
+        nc = __popc(who);
+      }
+    }
+    Part a{m, ref, warp_sum(s2.x + s2.y), warp_sum(u2.x + u2.y)};
+    const bool odd = a.s != a.s, plain = fabsf(a.m) * c <= p.plain_most;
+    if (!plain) {
+      a = slow_part(x, 0, V, lane, 32, a.m, c);
+      a.s = warp_sum(a.s);
+      a.u = warp_sum(a.u);
+    }
+    if (lane == i) keep = a;
+    if constexpr (TOP) {
+      __syncwarp();
+      if (nv <= kRowVecCap)
+        for (int j0 = 0; j0 < nv * E; j0 += 32) {
+          const int j = j0 + lane;
+          const float xv = j < nv * E ? ld(reinterpret_cast<const T*>(s.vec) + j) : -INFINITY;
+          const bool put = j < nv * E && xv >= bound;
+          const unsigned who = __ballot_sync(0xffffffffu, put);
+          const int at = nc + __popc(who & lt);
+          if (put && at < kRowCandCap) s.cand[at] = rank_word(xv, sp.head + s.vec_at[j / E] * E + j % E);
+          nc += __popc(who);
+        }
+      __syncwarp();
+      if (nv > kRowVecCap || nc > kRowCandCap || odd) {
+        exact_top(x, 0, V, k, s.cand, &s.n_cand, WarpGroup{});
+        nc = k;
+      }
+      const Log2P q = distribution(a, plain, c);
+      const int64_t out = (int64_t)(row0 + i) * k;
+      for (int j = lane; j < nc; j += 32) {
+        const uint64_t w = s.cand[j];
+        int above = 0;
+        for (int o = 0; o < nc; ++o) above += s.cand[o] > w ? 1 : 0;
+        if (above < k) {
+          p.top_ids[out + above] = rank_index(w);
+          p.top_logprob[out + above] = q.ln(key_value((uint32_t)(w >> 32)), p.inv_t);
+        }
+      }
+      __syncwarp();  // the lists are free again
     }
   }
+  if (lane < rows) finish_row<T>(p, keep, row0 + lane);
 }
 
 int sm_count() {
@@ -548,16 +715,27 @@ int launch_warp(const Params& p, cudaStream_t s) {
   return check_launch("m3_token_logprobs");
 }
 
-// A row goes to a warp while its vectors fit the lanes' registers (with alternatives: while a lane
-// can keep its 8 or 16 entries sorted), else to a CTA, and with few rows to a cluster.
+template <typename T, int BEST>
+int launch_rows(const Params& p, cudaStream_t s) {
+  const int batch = warp_batch(p.rows, sm_count());
+  const int warps = (p.rows + batch - 1) / batch;
+  score_rows_kernel<T, BEST><<<(unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, 0, s>>>(p, batch);
+  return check_launch("m3_token_logprobs");
+}
+
+// A row goes to a warp while its vectors fit the lanes' registers (one each; with many alternatives two, which
+// a lane can keep sorted), or while there are warps' worth of rows and it is a few tiles; else to a CTA, and
+// with few rows to a cluster.
 template <typename T, bool TOP>
 int launch(Params p, int nvec, cudaStream_t s) {
   if (nvec <= 32) return launch_warp<T, 1, TOP>(p, s);
-  if (nvec <= 64) return launch_warp<T, 2, TOP>(p, s);
-  if constexpr (!TOP) {
-    if (nvec <= 128) return launch_warp<T, 4, TOP>(p, s);
-    if (nvec <= 256) return launch_warp<T, 8, TOP>(p, s);
+  const bool few = !TOP || p.top <= kRowMostTop;
+  if (few && (nvec <= 32 * kNV || (nvec <= 4 * 32 * kNV && p.rows >= 16 * sm_count()))) {
+    if constexpr (!TOP) return launch_rows<T, 0>(p, s);
+    return p.top <= 8 ? launch_rows<T, 1>(p, s) : launch_rows<T, 2>(p, s);
   }
+  if constexpr (TOP)
+    if (nvec <= 64) return launch_warp<T, 2, TOP>(p, s);
   // few rows: several CTAs per row until they cover the SMs
   const int sms = sm_count();
   int cl = 1;
