@@ -298,21 +298,26 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   float xl = 0.f;
   const bool holder = warp == 0 && (GRAD || rank == 0);
   Entries<kEnt> en;
+  int64_t given[kEnt];
+  float logit[kEnt];
   if (warp == 0) {
-    int found = 0;
 #pragma unroll
     for (int e = 0; e < kEnt; ++e) {
       const int j = lane + 32 * e;
-      const bool there = j < p.k;
-      found |= put_entry(en, e, there ? p.ids[(int64_t)row * p.k + j] : -1, there ? p.teacher[(int64_t)row * p.k + j] : 0.f, V);
+      given[e] = j < p.k ? p.ids[(int64_t)row * p.k + j] : -1;
+      logit[e] = j < p.k ? p.teacher[(int64_t)row * p.k + j] : 0.f;
     }
+  }
+  auto gather = [&]() {  // once the first tile is on its way; before the gradient may overwrite the logits
+    int found = 0;
+#pragma unroll
+    for (int e = 0; e < kEnt; ++e) found |= put_entry(en, e, given[e], logit[e], V);
     const int f = row_flags<HARD>(p, found, w, label);
     if (lane == 0) s.flags = f;
-    // read here: below, the gradient may overwrite the logits
 #pragma unroll
     for (int e = 0; e < kEnt; ++e) en.x[e] = en.id[e] >= 0 ? ld(x + en.id[e]) : 0.f;
     if (HARD && label >= 0 && label < V) xl = ld(x + label);
-  }
+  };
   if constexpr (GRAD)
     for (int i = tid; i < S::kSeen / 4; i += TB) reinterpret_cast<uint4*>(s.seen)[i] = make_uint4(0u, 0u, 0u, 0u);
 
@@ -355,17 +360,22 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   };
   // the ragged tile first, then the full ones down to tile 0, which stays in d
   const int tiles = n / kTile, rest = tiles * kTile;
-  if (rest < n) {
+  if (rest < n)
     load_rest(rest, policy);
+  else if (tiles > 0)
+    load(rest - kTile, policy);
+  if (warp == 0) gather();
+  if (rest < n) {
     sum(rest, Flag<false>());
+    if (tiles > 0) load(rest - kTile, policy);
   }
   for (int t = tiles - 1; t >= 0; --t) {
-    load(t * kTile, policy);
     sum(t * kTile, Flag<true>());
     if (GRAD && t == 1) {
 #pragma unroll
       for (int j = 0; j < kNV; ++j) cache[j * TB + tid] = d[j];
     }
+    if (t > 0) load((t - 1) * kTile, policy);
   }
   int edge = -1;  // this lane's element of the row's edges
   float xe = -INFINITY;
@@ -471,9 +481,13 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
 // their way; lane i keeps row i's weight, label and loss.
 constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
 
+// The entries' logits come from a copy of a short row in shared memory, of a longer one from L2.
+template <int NV>
+constexpr bool kCopy = NV <= 8;
+
 template <typename T, int NV, bool GRAD>
 struct alignas(16) WarpSmem {
-  uint4 row[NV * 32];
+  uint4 row[kCopy<NV> ? NV * 32 : 1];
   int ids[GRAD ? M3_MAX_TOP : 1];
   float probs[GRAD ? M3_MAX_TOP : 1];
   uint32_t seen[GRAD ? NV * kVec<T> : 1];  // a bit per element
@@ -523,10 +537,26 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
     const int row = row0 + i, at = shift;
     const float w = __shfl_sync(0xffffffffu, w_all, i);
     const int64_t label = HARD ? __shfl_sync(0xffffffffu, label_all, i) : -1;
+    const T* xs = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
+    if constexpr (kCopy<NV>) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) s.row[j * 32 + lane] = d[j];
+      for (int j = 0; j < NV; ++j) s.row[j * 32 + lane] = d[j];
+      xs = reinterpret_cast<const T*>(s.row) + at;
+    }
     if (GRAD)
       for (int j = lane; j < NV * E; j += 32) s.seen[j] = 0u;
+    Entries<KE> en;
+    int found = 0;
+    float xl = 0.f;
+    auto gather = [&]() {
+#pragma unroll
+      for (int e = 0; e < KE; ++e) {
+        found |= put_entry(en, e, id[e], t[e], V);
+        en.x[e] = en.id[e] >= 0 ? ld(xs + en.id[e]) : 0.f;
+      }
+      if (HARD && label >= 0 && label < V) xl = ld(xs + label);
+    };
+    if constexpr (!kCopy<NV>) gather();  // on their way during the sums
     Part a = no_part();
     VecMax<T> vm[NV];
     a.m = warp_max(vecs_max<T, NV>(d, vm, [](int) { return true; }));
@@ -536,16 +566,8 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
 #pragma unroll
     for (int j = 0; j < NV; ++j) add_vec<T, HARD>(d[j], a.r, a.r1, c, s2, t2);
     __syncwarp();
-    const T* xs = reinterpret_cast<const T*>(s.row) + at;
-    Entries<KE> en;
-    int found = 0;
-#pragma unroll
-    for (int e = 0; e < KE; ++e) {
-      found |= put_entry(en, e, id[e], t[e], V);
-      en.x[e] = en.id[e] >= 0 ? ld(xs + en.id[e]) : 0.f;
-    }
+    if constexpr (kCopy<NV>) gather();
     const int flags = row_flags<HARD>(p, found, w, label);
-    const float xl = HARD && label >= 0 && label < V ? ld(xs + label) : 0.f;
     teacher_softmax(p, en);
     a.s = warp_sum(s2.x + s2.y);
     a.s1 = HARD ? warp_sum(t2.x + t2.y) : 1.f;
@@ -604,7 +626,7 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
   const int tid = threadIdx.x, rank = cluster_rank();
   cluster_arrive_relaxed();
   float s = 0.f;
-#pragma unroll 4
+#pragma unroll 16
   for (int64_t i = (int64_t)rank * kSumThreads + tid; i < n; i += kSumCtas * kSumThreads) s += v[i];
   s = warp_sum(s);
   if ((tid & 31) == 0) sm[tid >> 5] = s;
@@ -692,6 +714,7 @@ int launch(Params p, int nvec, cudaStream_t s) {
   if (nvec <= 64) return launch_warp<T, 2, HARD, GRAD>(p, s);
   if (nvec <= 128) return launch_warp<T, 4, HARD, GRAD>(p, s);
   if (nvec <= 256) return launch_warp<T, 8, HARD, GRAD>(p, s);
+  if (nvec <= 512 && p.rows >= 16 * sm_count()) return launch_warp<T, 16, HARD, GRAD>(p, s);
   // few rows: several CTAs per row until they cover the SMs
   const int sms = sm_count();
   int cl = 1;

@@ -19,7 +19,7 @@ using namespace vocab;
 
 constexpr int kNV = 8;          // vectors a thread loads at a time
 constexpr int kMaxCluster = 8;  // CTAs per row (portable size)
-constexpr int kVecCap = 512, kCandCap = 512;
+constexpr int kCandCap = 1024;  // a power of two
 
 struct Params {
   int rows, vocab, top, cluster, log2_cluster;
@@ -103,13 +103,15 @@ struct Smem {
   Part parts[kMaxCluster], again[kMaxCluster];
 };
 template <int NW>
+constexpr int kVecCap = NW <= 4 ? 512 : 1024;  // vectors put aside
+template <int NW>
 struct Smem<NW, true> {
   Part part[NW];
   Part parts[kMaxCluster], again[kMaxCluster];
   float bound[NW];
   int n_vec, n_cand;
-  int vec_at[kVecCap];
-  uint4 vec[kVecCap];
+  int vec_at[kVecCap<NW>];
+  uint4 vec[kVecCap<NW>];
   uint64_t cand[kCandCap];
   uint64_t list[kMaxCluster][M3_MAX_TOP];  // every CTA's alternatives, descending, 0 past the end
   int before[M3_MAX_TOP];                  // entries of the row above this CTA's i-th
@@ -168,6 +170,30 @@ __device__ __noinline__ void exact_top(const T* x, int lo, int hi, int need, uin
     if (k > key || (k == key && i <= last)) cand[atomicAdd(n_cand, 1)] = rank_word(v, i);
   }
   g.sync();
+}
+
+// Counting ranks n candidates in n^2 / TB steps, a bitonic network in n log^2 n / 4 TB.
+constexpr int kCountMost = 192;
+
+// cand[0, n), n <= kCandCap, into descending order (Batcher's bitonic network), 0 behind them.
+template <int TB>
+__device__ __noinline__ void sort_candidates(uint64_t* cand, int n) {
+  int size = 1;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += TB) cand[i] = 0;
+  __syncthreads();
+  for (int len = 2; len <= size; len *= 2)
+    for (int gap = len / 2; gap > 0; gap /= 2) {
+      for (int t = threadIdx.x; t < size / 2; t += TB) {
+        const int i = 2 * t - (t & (gap - 1)), j = i + gap;
+        const uint64_t a = cand[i], b = cand[j];
+        if ((a < b) == ((i & len) == 0)) {
+          cand[i] = b;
+          cand[j] = a;
+        }
+      }
+      __syncthreads();
+    }
 }
 
 template <typename T, int TB, bool TOP>
@@ -245,7 +271,7 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
           const int q = base + j * TB + tid;
           if ((full.value || q < n) && vm[j].reaches(bound)) {
             const int at = atomicAdd(&s.n_vec, 1);
-            if (at < kVecCap) {
+            if (at < kVecCap<NW>) {
               s.vec[at] = d[j];
               s.vec_at[at] = q;
             }
@@ -276,28 +302,35 @@ __global__ void __launch_bounds__(TB, 1024 / TB) score_kernel(const Params p) {
     const int k = p.top;
     bound = -warp_max(lane < NW ? -s.bound[lane] : -INFINITY);
     const int nv = s.n_vec;
-    if (nv <= kVecCap)
-      for (int i = tid; i < nv * E; i += TB) {
-        const float xv = ld(reinterpret_cast<const T*>(s.vec) + i);
-        if (xv >= bound) {
-          const int at = atomicAdd(&s.n_cand, 1);
-          if (at < kCandCap) s.cand[at] = rank_word(xv, first + s.vec_at[i / E] * E + i % E);
-        }
+    if (nv <= kVecCap<NW>)
+      for (int i0 = warp * 32; i0 < nv * E; i0 += TB) {
+        const int i = i0 + lane;
+        const float xv = i < nv * E ? ld(reinterpret_cast<const T*>(s.vec) + i) : -INFINITY;
+        const unsigned who = __ballot_sync(0xffffffffu, i < nv * E && xv >= bound);
+        int at = 0;
+        if (lane == 0 && who) at = atomicAdd(&s.n_cand, __popc(who));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+        if ((who >> lane & 1u) && at < kCandCap) s.cand[at] = rank_word(xv, first + s.vec_at[i / E] * E + i % E);
       }
     __syncthreads();
     // the sum is NaN iff the share holds NaN or +inf, which the comparisons above do not order
-    if (nv > kVecCap || s.n_cand > kCandCap || a.s != a.s) {
+    if (nv > kVecCap<NW> || s.n_cand > kCandCap || a.s != a.s) {
       exact_top(x, lo, hi, min(k, hi - lo), s.cand, &s.n_cand, CtaGroup<TB, Smem<NW, TOP>>{s});
     }
     const int nc = s.n_cand;
     uint64_t* list = s.list[rank];
-    for (int i = tid; i < nc; i += TB) {
-      const uint64_t w = s.cand[i];
-      int above = 0;
-      for (int j = 0; j < nc; ++j) above += s.cand[j] > w ? 1 : 0;
-      if (above < k) list[above] = w;
+    if (nc <= kCountMost) {
+      for (int i = tid; i < nc; i += TB) {
+        const uint64_t w = s.cand[i];
+        int above = 0;
+        for (int j = 0; j < nc; ++j) above += s.cand[j] > w ? 1 : 0;
+        if (above < k) list[above] = w;
+      }
+      for (int i = nc + tid; i < k; i += TB) list[i] = 0;
+    } else {
+      sort_candidates<TB>(s.cand, nc);
+      for (int i = tid; i < k; i += TB) list[i] = s.cand[i];
     }
-    for (int i = nc + tid; i < k; i += TB) list[i] = 0;
     for (int i = tid; i < k; i += TB) s.before[i] = i;
     __syncthreads();
   }
