@@ -1,7 +1,7 @@
 // Embedding lookup with scaling, and the table's gradient by sorted tokens.
 //   out[r] = scale * table[token r]              grad[v] = scale * sum of dy[r] over token r == v
 // The gradient's rows are summed in the order of r (fp32), so that it is the same every call:
-// (token, r) pairs are put in order by a stable radix sort (one 8-CTA cluster), the sorted list is cut
+// (token, r) pairs are put in order by a stable radix sort (one 16-CTA cluster), the sorted list is cut
 // into chunks of equal length, each summed by one group of threads, and the pieces of tokens longer
 // than that are joined.  The cuts depend on the sizes alone, so the result is the same every call.
 #include <cooperative_groups.h>
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const FwdParams p) {
 }
 
 // ---- stable radix sort of (token, r) ------------------------------------------------------
-constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSortCtas = 16, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 constexpr int kSortAhead = 8;  // entries a lane has in flight
 
@@ -161,7 +161,13 @@ struct SortParams {
   const int64_t* tokens;
   uint2* buf[2];  // (token, r); the result is in buf[(passes - 1) & 1]
   int* count;     // entries in the result: the tokens inside [0, vocab)
-  unsigned char* clear;  // gradient whose rows of absent tokens the other CTAs clear, NULL = none
+};
+
+struct ClearParams {
+  int rows, vocab;
+  Rows trow;
+  const int64_t* tokens;
+  unsigned char* grad;
   int64_t row_bytes, ld_bytes;
 };
 
@@ -171,47 +177,51 @@ struct SortSmem {
   int wsum[kSortWarps];
 };
 
-// Clears the gradient's rows of the tokens that do not occur, CTA by CTA (`cta` of `ctas`), while the
-// first cluster sorts: every CTA marks all tokens in a bitmap of its own, then clears its share.
-__device__ __forceinline__ void clear_absent(const SortParams& p, uint32_t* seen, int cta, int ctas) {
+// Clears the gradient's rows of the tokens that do not occur while the cluster before it in the stream
+// sorts: every CTA marks all tokens in a bitmap of its own, then clears its share.
+constexpr int kClearThreads = 1024, kClearWarps = kClearThreads / 32, kClearAhead = 8;
+constexpr int kClearMostVocab = 48 * 1024 * 8;  // bits of the bitmap
+
+__global__ void __launch_bounds__(kClearThreads) clear_kernel(const ClearParams p) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  uint32_t* seen = reinterpret_cast<uint32_t*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < (p.vocab + 31) / 32; i += kSortThreads) seen[i] = 0u;
+  for (int i = tid; i < (p.vocab + 31) / 32; i += kClearThreads) seen[i] = 0u;
   __syncthreads();
-  for (int64_t i = tid; i < p.rows; i += kSortThreads * kSortAhead) {
-    int64_t t[kSortAhead];
+  for (int64_t i = tid; i < p.rows; i += kClearThreads * kClearAhead) {
+    int64_t t[kClearAhead];
 #pragma unroll
-    for (int j = 0; j < kSortAhead; ++j) {
-      const int64_t at = i + j * kSortThreads;
+    for (int j = 0; j < kClearAhead; ++j) {
+      const int64_t at = i + j * kClearThreads;
       t[j] = at < p.rows ? p.tokens[p.trow.at((int)at)] : -1;
     }
 #pragma unroll
-    for (int j = 0; j < kSortAhead; ++j)
+    for (int j = 0; j < kClearAhead; ++j)
       if (t[j] >= 0 && t[j] < p.vocab) atomicOr(&seen[t[j] >> 5], 1u << (t[j] & 31));
   }
   __syncthreads();
-  const bool wide = ((uintptr_t)p.clear | (uint64_t)p.ld_bytes | (uint64_t)p.row_bytes) % 16 == 0;
-  for (int64_t v = (int64_t)cta * kSortWarps + warp; v < p.vocab; v += (int64_t)ctas * kSortWarps) {
+  const bool wide = ((uintptr_t)p.grad | (uint64_t)p.ld_bytes | (uint64_t)p.row_bytes) % 16 == 0;
+  for (int64_t v = (int64_t)blockIdx.x * kClearWarps + warp; v < p.vocab; v += (int64_t)gridDim.x * kClearWarps) {
     if (seen[v >> 5] >> (v & 31) & 1u) continue;
-    unsigned char* g = p.clear + v * p.ld_bytes;
+    unsigned char* g = p.grad + v * p.ld_bytes;
     if (wide) {
       for (int64_t b = lane * 16; b < p.row_bytes; b += 512) *reinterpret_cast<uint4*>(g + b) = make_uint4(0u, 0u, 0u, 0u);
     } else {
       for (int64_t b = lane * 2; b < p.row_bytes; b += 64) *reinterpret_cast<uint16_t*>(g + b) = 0;
     }
   }
+  // the kernel behind this one reads what the sort writes
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Each of the cluster's 256 warps owns a contiguous piece of the input; positions are handed out
+// Each of the cluster's 512 warps owns a contiguous piece of the input; positions are handed out
 // digit by digit, then CTA by CTA, warp by warp and lane by lane, so equal digits keep their order.
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
-  if (blockIdx.x >= kSortCtas) {
-    clear_absent(p, reinterpret_cast<uint32_t*>(smem_raw), blockIdx.x - kSortCtas, gridDim.x - kSortCtas);
-    return;
-  }
+  asm volatile("griddepcontrol.launch_dependents;");  // a clear_kernel behind this one may start
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
   const int bins = 1 << p.bits;
   const unsigned lt = (1u << lane) - 1u;
@@ -460,7 +470,7 @@ constexpr int kJoinWidth = 8, kJoinChunks = 16, kJoinAhead = 4;
 template <typename G, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(const SumParams p) {
   constexpr int kGroups = kThreads / kJoinWidth;
-  __shared__ float sums[kGroups][kJoinWidth * N];
+  __shared__ float sums[kThreads / 32][kJoinWidth * N];
   const int n = *p.count, lane = threadIdx.x & 31;
   const int64_t k = (int64_t)blockIdx.x * kJoinChunks + lane, b1 = (k + 1) * p.chunk;
   bool goes_on = false;
@@ -500,11 +510,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const SumParams p) {
         }
       }
     }
+    // the groups of a warp, then the warps
 #pragma unroll
-    for (int j = 0; j < N; ++j) sums[g][w * N + j] = acc[j];
+    for (int o = kJoinWidth; o < 32; o *= 2)
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+    if (lane < kJoinWidth)
+#pragma unroll
+      for (int j = 0; j < N; ++j) sums[threadIdx.x >> 5][w * N + j] = acc[j];
     __syncthreads();
-    if (g == 0 && c < p.dim) {
-      for (int h = 1; h < kGroups; ++h)
+    if (threadIdx.x < kJoinWidth && c < p.dim) {
+#pragma unroll
+      for (int h = 1; h < kThreads / 32; ++h)
 #pragma unroll
         for (int j = 0; j < N; ++j) acc[j] += sums[h][w * N + j];
       write_row<N, G>(p, token, c, acc);
@@ -522,31 +539,18 @@ int sm_count() {
   return c;
 }
 
-// How many of the sort's clusters run at once on this device (they do not tile its SMs), after
-// allowing the kernel its shared memory; 0 on an error.
-int sort_clusters() {
-  static int found[64] = {};
+// Allows the sort its shared memory and its cluster of 16, once per device.
+int sort_setup() {
+  static bool done[64] = {};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  if (dev < 64 && found[dev]) return found[dev];
+  if (cudaGetDevice(&dev) != cudaSuccess) return check_launch("m3_embed_bwd: cudaGetDevice");
+  if (dev < 64 && done[dev]) return M3_OK;
   if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortSmem)) !=
-      cudaSuccess)
-    return 0;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kSortCtas, 1, 1);
-  cfg.blockDim = dim3(kSortThreads, 1, 1);
-  cfg.dynamicSmemBytes = sizeof(SortSmem);
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = kSortCtas;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, sort_kernel, &cfg) != cudaSuccess) return 0;
-  if (n < 1) n = 1;
-  if (dev < 64) found[dev] = n;
-  return n;
+          cudaSuccess ||
+      cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return check_launch("m3_embed_bwd: cudaFuncSetAttribute");
+  if (dev < 64) done[dev] = true;
+  return M3_OK;
 }
 
 bool dtype_ok(int d) { return d == M3_DTYPE_F32 || d == M3_DTYPE_BF16; }
@@ -569,7 +573,7 @@ void launch_embed(FwdParams p, cudaStream_t s) {
   const int keep = (128 << 10) / (int)(p.vocab < 4096 ? p.vocab * (int)sizeof(T) * N : 1 << 30);
   if (keep >= 8 && keep < p.cols.width && p.rows > 8 * (int64_t)p.vocab) p.cols = Columns{keep / 8 * 8, kThreads / (keep / 8 * 8)};
   const int y = slabs(p.dim, N, p.cols);
-  const int want = (p.rows + p.cols.groups - 1) / p.cols.groups, most = sm_count() * 8;
+  const int want = (p.rows + p.cols.groups - 1) / p.cols.groups, most = (sm_count() * 8 + y - 1) / y;
   embed_kernel<T, O, N><<<dim3((unsigned)(want < most ? want : most), y), kThreads, 0, s>>>(p);
 }
 
@@ -694,18 +698,30 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   sp.count = (int*)ws;
   sp.buf[0] = (uint2*)(ws + 256);
   sp.buf[1] = (uint2*)(ws + 256 + align256((size_t)rows * sizeof(uint2)));
-  const int clusters = sort_clusters();
-  if (clusters <= 0) return check_launch("m3_embed_bwd: sort_kernel attributes");
+  if (const int rc = sort_setup()) return rc;
+  sort_kernel<<<kSortCtas, kSortThreads, sizeof(SortSmem), s>>>(sp);
   // Rows of absent tokens are cleared beside the sort by CTAs that each read all tokens; where that is
   // more to read than there is to clear, or the bitmap does not fit, the sums' launch looks them up.
   const int64_t row_bytes = (int64_t)a.dim * (int64_t)gs, all_bytes = row_bytes * a.vocab;
-  int64_t ctas = (int64_t)(clusters - 1) * kSortCtas;
-  if (ctas > all_bytes >> 17) ctas = (all_bytes >> 17) / kSortCtas * kSortCtas;  // at least 128 KB each
-  const bool beside = !a.accumulate && ctas > 0 && ctas * rows * 8 <= all_bytes / 2 && a.vocab <= (int)sizeof(SortSmem) * 8;
-  sp.clear = beside ? (unsigned char*)a.grad : nullptr;
-  sp.row_bytes = row_bytes;
-  sp.ld_bytes = a.grad_ld * (int64_t)gs;
-  sort_kernel<<<kSortCtas + (beside ? (unsigned)ctas : 0u), kSortThreads, sizeof(SortSmem), s>>>(sp);
+  int64_t ctas = sm_count() - kSortCtas;
+  if (ctas > all_bytes >> 17) ctas = all_bytes >> 17;  // at least 128 KB each
+  const bool beside = !a.accumulate && ctas > 0 && ctas * rows * 8 <= all_bytes / 2 && a.vocab <= kClearMostVocab;
+  if (beside) {
+    const ClearParams cp{(int)rows, a.vocab, sp.trow, a.tokens, (unsigned char*)a.grad, row_bytes,
+                         a.grad_ld * (int64_t)gs};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+    cfg.blockDim = dim3(kClearThreads, 1, 1);
+    cfg.dynamicSmemBytes = ((size_t)a.vocab + 31) / 32 * 4;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, clear_kernel, cp);
+    if (e != cudaSuccess) return set_error(M3_ERR_LAUNCH, std::string("m3_embed_bwd: ") + cudaGetErrorString(e));
+  }
   const SumParams p{(int)a.grad_ld,
                     a.dim,
                     chunk_of(rows, a.dim),
