@@ -1,7 +1,7 @@
 // Embedding lookup with scaling, and the table's gradient by sorted tokens.
 //   out[r] = scale * table[token r]              grad[v] = scale * sum of dy[r] over token r == v
 // The gradient's rows are summed in the order of r (fp32), so that it is the same every call:
-// (token, r) pairs are put in order by a stable radix sort (one 16-CTA cluster), the sorted list is cut
+// (token, r) pairs are put in order by a stable radix sort (one cluster of up to 16 CTAs), the sorted list is cut
 // into chunks of equal length, each summed by one group of threads, and the pieces of tokens longer
 // than that are joined.  The cuts depend on the sizes alone, so the result is the same every call.
 #include <cooperative_groups.h>
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const FwdParams p) {
 }
 
 // ---- stable radix sort of (token, r) ------------------------------------------------------
-constexpr int kSortCtas = 16, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kSortMostCtas = 16, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxBits = 9, kMaxBins = 1 << kMaxBits;
 constexpr int kSortAhead = 8;  // entries a lane has in flight
 
@@ -214,15 +214,16 @@ __global__ void __launch_bounds__(kClearThreads) clear_kernel(const ClearParams 
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Each of the cluster's 512 warps owns a contiguous piece of the input; positions are handed out
+// Each of the cluster's warps owns a contiguous piece of the input; positions are handed out
 // digit by digit, then CTA by CTA, warp by warp and lane by lane, so equal digits keep their order.
-__global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
   asm volatile("griddepcontrol.launch_dependents;");  // a clear_kernel behind this one may start
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
+  const int ctas = (int)cluster.num_blocks();
   const int bins = 1 << p.bits;
   const unsigned lt = (1u << lane) - 1u;
   int64_t n = p.rows;
@@ -230,7 +231,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
     const int shift = pass * p.bits;
     const uint2* src = p.buf[(pass + 1) & 1];
     uint2* dst = p.buf[pass & 1];
-    const int64_t piece = (n + kSortCtas * kSortWarps * 32 - 1) / (kSortCtas * kSortWarps * 32) * 32;
+    const int64_t piece = (n + ctas * kSortWarps * 32 - 1) / (ctas * kSortWarps * 32) * 32;
     int64_t i0 = (int64_t)(rank * kSortWarps + warp) * piece, i1 = i0 + piece;
     if (i0 > n) i0 = n;
     if (i1 > n) i1 = n;
@@ -276,7 +277,7 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
     cluster.sync();
     int all = 0, before = 0;
     if (tid < bins)
-      for (int r = 0; r < kSortCtas; ++r) {
+      for (int r = 0; r < ctas; ++r) {
         const int v = *cluster.map_shared_rank(&s.total[tid], r);
         before += r < rank ? v : 0;
         all += v;
@@ -373,7 +374,7 @@ __device__ __forceinline__ bool ends_by(const uint2* a, int n, int64_t b, uint32
   return b >= n || a[b].x != token;
 }
 
-constexpr int kAhead = 8;  // entries in flight
+constexpr int kAhead = 4;  // entries in flight (8, with half the warps an SM holds: 36 us instead of 30)
 
 template <typename D, typename G, int N>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const SumParams p) {
@@ -587,11 +588,11 @@ void launch_embed(const FwdParams& p, cudaStream_t s) {
   launch_embed<T, O, 1>(p, s);
 }
 
-// Entries per chunk: enough chunks for 1024 threads of 8 columns on each of 148 SMs.
+// Entries per chunk: enough chunks for 1536 threads of 8 columns on each of 148 SMs.
 constexpr int kMinChunk = 16, kMaxChunk = 256;
 
 int chunk_of(int64_t rows, int dim) {
-  int64_t c = rows * ((dim + 7) / 8) / (148 * 1024);  // not the device's: the sums' order depends on it
+  int64_t c = rows * ((dim + 7) / 8) / (148 * 1536);  // not the device's: the sums' order depends on it
   c = (c + 7) / 8 * 8;
   return (int)(c < kMinChunk ? kMinChunk : c > kMaxChunk ? kMaxChunk : c);
 }
@@ -699,27 +700,37 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   sp.buf[0] = (uint2*)(ws + 256);
   sp.buf[1] = (uint2*)(ws + 256 + align256((size_t)rows * sizeof(uint2)));
   if (const int rc = sort_setup()) return rc;
-  sort_kernel<<<kSortCtas, kSortThreads, sizeof(SortSmem), s>>>(sp);
+  // a CTA for every 2048 tokens: the cluster's barriers cost more than a few tokens a lane
+  int sort_ctas = 1;
+  while (sort_ctas < kSortMostCtas && rows > 2048 * sort_ctas) sort_ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)sort_ctas, 1, 1);
+  cfg.blockDim = dim3(kSortThreads, 1, 1);
+  cfg.dynamicSmemBytes = sizeof(SortSmem);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = sort_ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, sort_kernel, sp);
+  if (e != cudaSuccess) return set_error(M3_ERR_LAUNCH, std::string("m3_embed_bwd: ") + cudaGetErrorString(e));
   // Rows of absent tokens are cleared beside the sort by CTAs that each read all tokens; where that is
   // more to read than there is to clear, or the bitmap does not fit, the sums' launch looks them up.
   const int64_t row_bytes = (int64_t)a.dim * (int64_t)gs, all_bytes = row_bytes * a.vocab;
-  int64_t ctas = sm_count() - kSortCtas;
+  int64_t ctas = sm_count() - sort_ctas;
   if (ctas > all_bytes >> 17) ctas = all_bytes >> 17;  // at least 128 KB each
   const bool beside = !a.accumulate && ctas > 0 && ctas * rows * 8 <= all_bytes / 2 && a.vocab <= kClearMostVocab;
   if (beside) {
     const ClearParams cp{(int)rows, a.vocab, sp.trow, a.tokens, (unsigned char*)a.grad, row_bytes,
                          a.grad_ld * (int64_t)gs};
-    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas, 1, 1);
     cfg.blockDim = dim3(kClearThreads, 1, 1);
     cfg.dynamicSmemBytes = ((size_t)a.vocab + 31) / 32 * 4;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, clear_kernel, cp);
+    e = cudaLaunchKernelEx(&cfg, clear_kernel, cp);
     if (e != cudaSuccess) return set_error(M3_ERR_LAUNCH, std::string("m3_embed_bwd: ") + cudaGetErrorString(e));
   }
   const SumParams p{(int)a.grad_ld,
