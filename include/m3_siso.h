@@ -411,7 +411,7 @@ int m3_gated_act_bf16(const void *x, int64_t x_row_stride, void *out, int64_t ou
 typedef struct M3ScoreArgs {
   int32_t rows_outer, rows_inner, vocab, top;    /* top <= min(vocab, M3_MAX_TOP) */
   int32_t logits_dtype;                          /* M3_DTYPE_* */
-  float temperature;                             /* > 0 */
+  float temperature;                             /* in [1e-30, 1e30] */
   const void *logits;     int64_t ld_outer, ld_inner;
   const int64_t *targets; int64_t t_outer, t_inner;  /* NULL: no logprob */
   float *logprob, *entropy, *lse;                /* (rows) dense; logprob NULL iff targets NULL */
@@ -436,7 +436,7 @@ enum { M3_REDUCE_NONE = 0, M3_REDUCE_SUM = 1, M3_REDUCE_MEAN = 2 };
 typedef struct M3DistillArgs {
   int32_t rows_outer, rows_inner, vocab, k;      /* 1 <= k <= M3_MAX_TOP */
   int32_t logits_dtype, reduction;
-  float temperature, hard_weight, grad_scale;    /* T > 0, 0 <= hard_weight <= 1 */
+  float temperature, hard_weight, grad_scale;    /* T in [1e-30, 1e30], 0 <= hard_weight <= 1 */
   const void *logits;     int64_t ld_outer, ld_inner;
   const int64_t *ids;                            /* (rows, k) dense */
   const float *teacher;                          /* (rows, k) dense */

@@ -749,8 +749,8 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
     return set_error(M3_ERR_UNSUPPORTED, "m3_distill: logits must be f32 or bf16");
   if (a.reduction < M3_REDUCE_NONE || a.reduction > M3_REDUCE_MEAN)
     return set_error(M3_ERR_ARG, "m3_distill: reduction must be NONE, SUM or MEAN");
-  if (!(a.temperature > 0.f) || !(a.hard_weight >= 0.f && a.hard_weight <= 1.f))
-    return set_error(M3_ERR_ARG, "m3_distill: need temperature > 0 and 0 <= hard_weight <= 1");
+  if (!temperature_ok(a.temperature) || !(a.hard_weight >= 0.f && a.hard_weight <= 1.f))
+    return set_error(M3_ERR_ARG, "m3_distill: need a temperature > 0 (finite, as 1 / T) and 0 <= hard_weight <= 1");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
   if (rows > kMaxRows) return set_error(M3_ERR_SHAPE, "m3_distill: more than 2^30 rows");
   if ((rows > 0 && (!a.logits || !a.ids || !a.teacher || !a.row_loss)) ||

@@ -793,7 +793,8 @@ extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
     return set_error(M3_ERR_SHAPE, "m3_token_logprobs: need rows >= 0, 0 < vocab <= 2^30 and 0 <= top <= min(vocab, 128)");
   if (a.logits_dtype != M3_DTYPE_F32 && a.logits_dtype != M3_DTYPE_BF16)
     return set_error(M3_ERR_UNSUPPORTED, "m3_token_logprobs: logits must be f32 or bf16");
-  if (!(a.temperature > 0.f)) return set_error(M3_ERR_ARG, "m3_token_logprobs: temperature must be > 0");
+  if (!temperature_ok(a.temperature))
+    return set_error(M3_ERR_ARG, "m3_token_logprobs: temperature must be > 0, finite and not so small that 1 / T overflows");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
   if (rows == 0) return M3_OK;
   if (!a.logits || !a.entropy || !a.lse || (a.targets && !a.logprob) || (a.top > 0 && (!a.top_logprob || !a.top_ids)))

@@ -281,6 +281,8 @@ __device__ __forceinline__ float warp_max(float v) {
 constexpr float kLowRef = -1e20f;
 
 __device__ __forceinline__ float ref_of(float m, float c) { return fmaxf(ceilf(m * c), kLowRef); }
+// 1 / T and log2(e) / T are ordinary numbers.
+inline bool temperature_ok(float t) { return t >= 1e-30f && t <= 1e30f; }
 // The most that |max| c may be for a plain row; none is with c so small or large that the clamp at
 // -1e30 would not lie between kLowRef and fp32's range.
 inline float plain_most(float c) { return c >= 1e-9f && c <= 1e8f ? 1e19f : -1.f; }

@@ -214,6 +214,52 @@ def test_views_and_in_place(vocab, dtype):
 
 
 @CUDA
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,vocab,k,hard", [(60001, 256, 16, 0.0), (20003, 250, 40, 0.4), (2500, 4001, 9, 0.0),
+                                               (2500, 2000, 33, 0.4), (2400, 1500, 8, 0.4), (700, 33001, 12, 0.0),
+                                               (500, 16390, 64, 0.4)])
+def test_many_rows(rows, vocab, k, hard, dtype):
+    """Several rows per warp, a row per warp of every length, rows of one, two and more tiles of a CTA."""
+    from mamba3_b200 import distill as D
+
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn(rows, vocab, generator=g, device="cuda") * 2).to(dtype)
+    step = vocab // k
+    ids = (torch.randint(0, vocab, (rows, 1), generator=g, device="cuda") + torch.arange(k, device="cuda") * step) % vocab
+    teacher = torch.randn(rows, k, generator=g, device="cuda") * 2
+    ids[:, k // 2][torch.rand(rows, generator=g, device="cuda") < 0.3] = -1
+    ids[7], ids[rows // 2] = -1, ids[rows // 2, 0].item()  # no entry; one id k times
+    weights = (torch.rand(rows, generator=g, device="cuda") < 0.9).float()
+    weights[0] = 1.0
+    labels = torch.where(torch.rand(rows, generator=g, device="cuda") < 0.5, ids[:, 0], 3) if hard else None
+    T = 1.7
+    loss, dx = D.distill_loss_and_grad(x, ids, teacher, temperature=T, labels=labels, hard_weight=hard, weights=weights)
+    # the formulas in 64 bits, all rows at once
+    there = ids >= 0
+    t = torch.where(there, teacher.double() / T, -math.inf)
+    p = torch.nan_to_num(torch.softmax(t, 1))
+    logq = torch.log_softmax(x.double() / T, 1)
+    entries = p * (torch.log(p) - logq.gather(1, ids.clamp_min(0)))
+    rows_loss = (1 - hard) * T * T * torch.where(p > 0, entries, 0.0).sum(1)
+    soft = there.any(1).double()[:, None]
+    grad = (1 - hard) * T * soft * torch.exp(logq)
+    grad.scatter_add_(1, ids.clamp_min(0), -(1 - hard) * T * p)
+    if hard:
+        on = (labels >= 0).double()
+        logq1 = torch.log_softmax(x.double(), 1)
+        rows_loss = rows_loss - hard * on * logq1.gather(1, labels.clamp_min(0)[:, None])[:, 0]
+        hot = torch.zeros_like(grad).scatter_(1, labels.clamp_min(0)[:, None], 1.0)
+        grad = grad + hard * on[:, None] * (torch.exp(logq1) - hot)
+    w = weights.double()
+    grad = grad * (w / w.sum())[:, None]
+    assert abs(float(loss) - float((rows_loss * w).sum() / w.sum())) <= _loss_tol(T, x, 1.0)
+    _check_grad(dx, grad.cpu(), (w / w.sum() * T)[:, None].cpu(), dtype, "many")
+    again, inplace = D.distill_loss_and_grad(x, ids, teacher, temperature=T, labels=labels, hard_weight=hard,
+                                             weights=weights, out=x)
+    assert inplace is x and torch.equal(again, loss) and torch.equal(x, dx)
+
+
+@CUDA
 def test_gradient_against_differences():
     """Directional differences of the kernel's own loss (fp32, central, step h): rounding of the
     loss 1e-6 / h, truncation h^2 |d3| / 6 with third derivatives of a softmax below 1."""
@@ -280,6 +326,8 @@ def test_refusals():
     ids = torch.zeros(4, 3, dtype=torch.int64, device="cuda")
     t = torch.zeros(4, 3, device="cuda")
     lab = torch.zeros(4, dtype=torch.int64, device="cuda")
+    wide = torch.zeros(4, 24, device="cuda")
+    D.distill_loss_and_grad(wide[:, :10], ids, t, out=wide[:, 11:21])  # columns of one buffer that do not meet
     for bad in (lambda: D.distill_loss(x, ids[:3], t[:3]), lambda: D.distill_loss(x, ids, t[:, :2]),
                 lambda: D.distill_loss(x, ids.float(), t), lambda: D.distill_loss(x, ids, ids),
                 lambda: D.distill_loss(x, ids, t, temperature=0.0), lambda: D.distill_loss(x, ids, t, hard_weight=0.5),
@@ -291,7 +339,10 @@ def test_refusals():
                 lambda: D.distill_loss_and_grad(x, ids, t, reduction="none"),
                 lambda: D.distill_loss_and_grad(x, ids, t, out=torch.empty(4, 11, device="cuda")),
                 lambda: D.distill_loss_and_grad(x, ids, t, out=torch.empty(1, 10, device="cuda").expand(4, 10)),
-                lambda: D.distill_loss_and_grad(x, ids, t, out=torch.empty(10, 4, device="cuda").t())):
+                lambda: D.distill_loss_and_grad(x, ids, t, out=torch.empty(10, 4, device="cuda").t()),
+                lambda: D.distill_loss_and_grad(wide[:, :10], ids, t, out=wide[:, 3:13]),
+                lambda: D.distill_loss_and_grad(wide[:, :10], ids, t, out=wide.view(-1)[5:45].view(4, 10)),
+                lambda: D.distill_loss(x, ids, t, temperature=math.inf)):
         with pytest.raises(ValueError):
             bad()
 

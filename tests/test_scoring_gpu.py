@@ -144,6 +144,63 @@ def test_suppressed_ids(vocab, dtype):
     _check(x, torch.full((6,), vocab - 1, device="cuda"), min(vocab, 12), 1.3)
 
 
+def _vector_reference(x, t, temperature):
+    """The formulas in 64 bits over all rows at once (on the device): rows with a finite maximum."""
+    y = x.double() / temperature
+    d = y - y.amax(-1, keepdim=True)
+    z = torch.exp(d).sum(-1)
+    lp = d - torch.log(z)[:, None]
+    p = torch.exp(lp)
+    ent = -torch.where(p > 0, p * lp, 0.0).sum(-1)
+    picked = torch.where(t < 0, 0.0, lp.gather(1, t.clamp_min(0)[:, None])[:, 0])
+    return picked, ent, y.amax(-1) + torch.log(z), lp
+
+
+@CUDA
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,vocab,top", [(60001, 256, 8), (60001, 250, 3), (20003, 300, 20), (2500, 4001, 8),
+                                            (2500, 4001, 32), (2500, 2000, 0), (2400, 8100, 5), (19000, 520, 40),
+                                            (700, 33001, 12)])
+def test_many_rows(rows, vocab, top, dtype):
+    """Several rows per warp, one warp per longer row, several waves of CTAs; masks and ties among them."""
+    from mamba3_b200 import scoring as S
+
+    x = _logits((rows, vocab), dtype, rows + vocab)
+    x[:, 5] = -math.inf
+    x[rows // 3] = 0.25
+    x[rows // 2, 1::2] = -math.inf
+    x[rows - 1] = torch.arange(vocab, device="cuda").to(dtype) / 16
+    t = _targets((rows,), vocab, 3)
+    got = S.token_logprobs(x, t, top=top, temperature=1.2)
+    picked, ent, lse, lp = _vector_reference(x, t, 1.2)
+    tol = 4e-6 + 3e-7 * float(x[:, 6:].float().abs().clamp(max=1e4).max()) / 1.2
+    _close(got.lse, lse.cpu(), tol, 1e-6, "lse")
+    _close(got.entropy, ent.cpu(), 8 * tol, 1e-6, "entropy")
+    _close(got.logprob, picked.cpu(), tol, 1e-6, "logprob")
+    if top:
+        # ties to the lower index: an order of all entries that is stable in the index
+        order = torch.sort(x.float() + 0.0, dim=1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(got.top_ids, order)
+        _close(got.top_logprob, lp.gather(1, order).cpu(), tol, 1e-6, "top_logprob")
+
+
+@CUDA
+@pytest.mark.parametrize("temperature", [1e-12, 1e-6, 1e-3, 50.0, 1e6, 1e12])
+@pytest.mark.parametrize("vocab", [200, 3000])
+def test_temperatures(vocab, temperature):
+    """From a distribution on one id to a uniform one; both forms of the sums."""
+    from mamba3_b200 import scoring as S
+
+    x = _logits((6, vocab), F32, 2)
+    x[1, ::3] = -math.inf
+    got = S.token_logprobs(x, None, top=3, temperature=temperature)
+    _, ent, lse, lp = _vector_reference(x, torch.zeros(6, dtype=torch.int64, device="cuda"), temperature)
+    top = lp.topk(3, 1).values
+    _close(got.lse, lse.cpu(), 1e-5, 1e-6, "lse")
+    _close(got.entropy, ent.cpu(), 5e-5, 1e-6, "entropy")
+    _close(got.top_logprob, top.cpu(), 1e-5, 2e-6, "top_logprob")
+
+
 @CUDA
 def test_targets_outside_the_vocabulary():
     from mamba3_b200 import scoring as S
@@ -190,7 +247,8 @@ def test_refusals():
     t = torch.zeros(4, dtype=torch.int64, device="cuda")
     for bad in (lambda: S.token_logprobs(x, top=11), lambda: S.token_logprobs(x, top=-1),
                 lambda: S.token_logprobs(torch.zeros(2, 500, device="cuda"), top=129),
-                lambda: S.token_logprobs(x, temperature=0.0), lambda: S.token_logprobs(x, temperature=math.nan),
+                lambda: S.token_logprobs(x, temperature=0.0), lambda: S.token_logprobs(x, temperature=math.inf),
+                lambda: S.token_logprobs(x, temperature=1e-38), lambda: S.token_logprobs(x, temperature=math.nan),
                 lambda: S.token_logprobs(x, t[:3]), lambda: S.token_logprobs(x, t.float()),
                 lambda: S.token_logprobs(x.double()), lambda: S.token_logprobs(x, t.cpu()),
                 lambda: S.token_logprobs(torch.zeros(3, 0, device="cuda"))):
