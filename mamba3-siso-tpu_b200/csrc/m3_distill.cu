@@ -33,6 +33,10 @@ struct Params {
   float* row_loss;
 };
 
+// A mean's kernels (sum of weights, rows, sum of losses) are launched so that each may start before the
+// one in front of it has ended; what it needs of that one's results it reads behind this.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The maximum, and the sums s = sum 2^(c x - r) and, with hard labels, s1 = sum 2^(log2(e) x - r1).
 struct Part {
   float m, r, s, r1, s1;
@@ -419,6 +423,7 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   }
   const int flags = s.flags;
   float norm = p.scale;
+  after_previous();
   if (GRAD && p.weight_sum) norm /= *p.weight_sum;
   const Row r = make_row<HARD>(p, a, plain, row, flags, w, norm);
   if (warp == 0 && rank == 0) {
@@ -505,7 +510,6 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
   if (rows <= 0) return;
   const float w_all = lane < rows && p.weights ? p.weights[row0 + lane] : 1.f;
   const int64_t label_all = HARD && lane < rows ? p.labels[row0 + lane] : -1;
-  const float norm = GRAD && p.weight_sum ? p.scale / *p.weight_sum : p.scale;
   uint4 d[NV];
   int shift = 0;
   int64_t id[KE];
@@ -532,6 +536,8 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
     }
   };
   load(row0);
+  after_previous();
+  const float norm = GRAD && p.weight_sum ? p.scale / *p.weight_sum : p.scale;
   float loss_all = 0.f;
   for (int i = 0; i < rows; ++i) {
     const int row = row0 + i, at = shift;
@@ -620,11 +626,13 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
 // out = scale * (sum of n values) / (*div_by, if given), by one cluster in a fixed order.
 constexpr int kSumCtas = 8, kSumThreads = 1024;
 
-__global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads)
     sum_kernel(const float* __restrict__ v, int64_t n, const float* div_by, float scale, float* out) {
   __shared__ float sm[32], total[kSumCtas];
   const int tid = threadIdx.x, rank = cluster_rank();
+  asm volatile("griddepcontrol.launch_dependents;");
   cluster_arrive_relaxed();
+  after_previous();
   float s = 0.f;
 #pragma unroll 16
   for (int64_t i = (int64_t)rank * kSumThreads + tid; i < n; i += kSumCtas * kSumThreads) s += v[i];
@@ -651,54 +659,62 @@ int sm_count() {
   return c;
 }
 
+// `early`: the kernel may start before the one in front of it in the stream has ended.
+template <typename... P, typename... A>
+int launch_kernel(void (*kern)(P...), unsigned grid, int block, size_t smem, int cluster, bool early, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  cfg.attrs = at;
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (early) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_distill: ") + cudaGetErrorString(e));
+}
+
+// Allows a kernel its shared memory, once per device (`done`: the kernel's own).
+template <typename K>
+int allow_smem(K kern, size_t bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (bytes <= 48 * 1024 || (dev < 64 && done[dev])) return M3_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
+    return check_launch("m3_distill: cudaFuncSetAttribute");
+  if (dev < 64) done[dev] = true;
+  return M3_OK;
+}
+
 template <typename T, int TB, bool HARD, bool GRAD>
 int launch_cta(const Params& p, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.rows * p.cluster, 1, 1);
-  cfg.blockDim = dim3(TB, 1, 1);
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = p.cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  static bool done[64] = {};
   constexpr size_t kSmem = sizeof(Smem<TB, GRAD>) + (GRAD ? sizeof(uint4) * kNV * TB : 0);
-  if constexpr (kSmem > 48 * 1024) {
-    static bool done[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 64 || !done[dev]) {
-      if (cudaFuncSetAttribute(distill_kernel<T, TB, HARD, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)kSmem) != cudaSuccess)
-        return check_launch("m3_distill: cudaFuncSetAttribute");
-      if (dev < 64) done[dev] = true;
-    }
-  }
-  cfg.dynamicSmemBytes = kSmem;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, distill_kernel<T, TB, HARD, GRAD>, p);
-  return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_distill: ") + cudaGetErrorString(e));
+  auto* kern = distill_kernel<T, TB, HARD, GRAD>;
+  if (const int rc = allow_smem(kern, kSmem, done)) return rc;
+  return launch_kernel(kern, (unsigned)p.rows * p.cluster, TB, kSmem, p.cluster, p.weight_sum != nullptr, s, p);
 }
 
 template <typename T, int NV, int KE, bool HARD, bool GRAD>
 int launch_warp_k(const Params& p, cudaStream_t s) {
+  static bool done[64] = {};
   const int batch = warp_batch(p.rows, sm_count());
   const int warps = (p.rows + batch - 1) / batch;
   constexpr size_t kSmem = kWarps * sizeof(WarpSmem<T, NV, GRAD>);
-  if constexpr (kSmem > 48 * 1024) {
-    static bool done[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 64 || !done[dev]) {
-      if (cudaFuncSetAttribute(distill_warp_kernel<T, NV, KE, HARD, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)kSmem) != cudaSuccess)
-        return check_launch("m3_distill: cudaFuncSetAttribute");
-      if (dev < 64) done[dev] = true;
-    }
-  }
-  distill_warp_kernel<T, NV, KE, HARD, GRAD>
-      <<<(unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, kSmem, s>>>(p, batch);
-  return check_launch("m3_distill");
+  auto* kern = distill_warp_kernel<T, NV, KE, HARD, GRAD>;
+  if (const int rc = allow_smem(kern, kSmem, done)) return rc;
+  return launch_kernel(kern, (unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, kSmem, 1, p.weight_sum != nullptr, s,
+                       p, batch);
 }
 
 template <typename T, int NV, bool HARD, bool GRAD>
@@ -790,15 +806,17 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
   p.upstream_stride = a.upstream_stride;
   p.weight_sum = wmean ? a.weight_sum : nullptr;
   p.row_loss = a.row_loss;
-  if (wmean) sum_kernel<<<kSumCtas, kSumThreads, 0, s>>>(a.weights, rows, nullptr, 1.f, a.weight_sum);
-  if (rows > 0) {
+  auto sum = [&](const float* v, const float* div_by, float scale, float* out, bool early) {
+    return launch_kernel(sum_kernel, kSumCtas, kSumThreads, 0, kSumCtas, early, s, v, (int64_t)rows, div_by, scale, out);
+  };
+  int rc = M3_OK;
+  if (wmean) rc = sum(a.weights, nullptr, 1.f, a.weight_sum, false);
+  if (rc == M3_OK && rows > 0) {
     const int nvec = most_vectors(a.logits, a.vocab, bf ? 2 : 4, a.ld_outer, a.ld_inner);
-    const int rc = bf ? launch<__nv_bfloat16>(p, nvec, s) : launch<float>(p, nvec, s);
-    if (rc != M3_OK) return rc;
+    rc = bf ? launch<__nv_bfloat16>(p, nvec, s) : launch<float>(p, nvec, s);
   }
-  if (a.reduction != M3_REDUCE_NONE)  // the mean of no rows is 0 / 0
-    sum_kernel<<<kSumCtas, kSumThreads, 0, s>>>(a.row_loss, rows, p.weight_sum,
-                                                a.reduction == M3_REDUCE_MEAN && !a.weights ? 1.f / (float)rows : 1.f,
-                                                a.loss);
-  return check_launch("m3_distill");
+  if (rc == M3_OK && a.reduction != M3_REDUCE_NONE)  // the mean of no rows is 0 / 0
+    rc = sum(a.row_loss, p.weight_sum, a.reduction == M3_REDUCE_MEAN && !a.weights ? 1.f / (float)rows : 1.f, a.loss,
+             rows > 0);
+  return rc;
 }
