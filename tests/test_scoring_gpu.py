@@ -240,6 +240,39 @@ def test_other_streams():
 
 
 @CUDA
+def test_replayed_in_a_graph():
+    """Captured calls read their inputs anew: scoring, the distillation step and the lookup's gradient."""
+    from mamba3_b200 import distill as D
+    from mamba3_b200 import embedding as E
+    from mamba3_b200 import scoring as S
+
+    x, x2 = _logits((40, 9000), BF, 1), _logits((40, 9000), BF, 2)
+    ids = torch.randint(0, 9000, (40, 6), device="cuda")
+    teacher = torch.randn(40, 6, device="cuda")
+    w = torch.rand(40, device="cuda")
+    dy = torch.randn(40, 64, device="cuda")
+
+    def step():
+        r = S.token_logprobs(x, ids[:, 0], top=4)
+        loss, dx = D.distill_loss_and_grad(x, ids, teacher, weights=w)
+        return r.logprob, r.entropy, r.top_ids, loss, dx, E.embedding_grad(dy, ids[:, 1], 9000)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    x.copy_(x2)
+    ids.copy_(torch.randint(0, 9000, (40, 6), device="cuda"))
+    graph.replay()
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
+
+
+@CUDA
 def test_refusals():
     from mamba3_b200 import scoring as S
 
