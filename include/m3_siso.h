@@ -445,9 +445,16 @@ typedef struct M3DistillArgs {
   const float *upstream;  int64_t upstream_stride;
   float *row_loss;                               /* (rows): the rows' losses */
   float *loss;                                   /* sum or mean; NULL iff M3_REDUCE_NONE */
-  float *weight_sum;                             /* one float of scratch for a mean with weights */
+  /* With grad, both may be NULL: the gradient alone. */
+  float *weight_sum;                             /* one float for a mean with weights: their sum */
   void *grad;             int64_t g_outer, g_inner;  /* logits' dtype; may be the logits; NULL = loss only */
+  int32_t ready;                                 /* M3_READY_* of an earlier call on the same inputs */
+  int32_t reserved;
 } M3DistillArgs;
+
+/* WEIGHTS: weight_sum holds the sum of weights.  GRAD: grad holds the gradient for an upstream of 1; the
+ * kernels look at `upstream` (stride 0) and leave it alone if it is 1, and write it anew otherwise. */
+enum { M3_READY_WEIGHTS = 1, M3_READY_GRAD = 2 };
 
 int m3_distill(const M3DistillArgs *args, void *stream);
 

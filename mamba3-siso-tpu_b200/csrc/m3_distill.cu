@@ -36,11 +36,16 @@ struct Params {
   int64_t upstream_stride;
   const float* weight_sum;  // a mean's divisor, NULL = none
   float* row_loss;
+  bool ready;  // grad holds the gradient for an upstream of 1
+  bool early;  // the sum of weights is the kernel in front of this one
 };
 
 // A mean's kernels (sum of weights, rows, sum of losses) are launched so that each may start before the
 // one in front of it has ended; what it needs of that one's results it reads behind this.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The gradient is there already (the same for all threads).
+__device__ __forceinline__ bool nothing_to_do(const Params& p) { return p.ready && *p.upstream == 1.f; }
 
 // The maximum, and the sums s = sum 2^(c x - r) and, with hard labels, s1 = sum 2^(log2(e) x - r1).
 struct Part {
@@ -293,6 +298,7 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   const int cl = p.cluster, rank = cl > 1 ? cluster_rank() : 0;
   const int row = (int)blockIdx.x >> p.log2_cluster;
   const int V = p.vocab;
+  if (GRAD && nothing_to_do(p)) return;
   const T* x = reinterpret_cast<const T*>(p.logits) + p.lrow.at(row);
   const Split sp = split_row(x, V);
   const int per = (sp.full + cl - 1) >> p.log2_cluster, v0 = min(sp.full, rank * per), n = min(per, sp.full - v0);
@@ -431,7 +437,7 @@ __global__ void __launch_bounds__(TB, 1024 / TB) distill_kernel(const Params p) 
   after_previous();
   if (GRAD && p.weight_sum) norm /= *p.weight_sum;
   const Row r = make_row<HARD>(p, a, plain, row, flags, w, norm);
-  if (warp == 0 && rank == 0) {
+  if (warp == 0 && rank == 0 && p.row_loss) {
     const float loss = row_loss<HARD>(p, r, flags, w, en, xl);
     if (lane == 0) p.row_loss[row] = loss;
   }
@@ -512,7 +518,7 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
   const int lane = threadIdx.x & 31, V = p.vocab;
   const float c = p.c;
   const int row0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * batch, rows = min(batch, p.rows - row0);
-  if (rows <= 0) return;
+  if (rows <= 0 || (GRAD && nothing_to_do(p))) return;
   const float w_all = lane < rows && p.weights ? p.weights[row0 + lane] : 1.f;
   const int64_t label_all = HARD && lane < rows ? p.labels[row0 + lane] : -1;
   uint4 d[NV];
@@ -625,7 +631,7 @@ __global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params
     }
     __syncwarp();  // the row's shared memory is free again
   }
-  if (lane < rows) p.row_loss[row0 + lane] = loss_all;
+  if (lane < rows && p.row_loss) p.row_loss[row0 + lane] = loss_all;
 }
 
 // out = scale * (sum of n values) / (*div_by, if given), by one cluster in a fixed order.
@@ -707,7 +713,7 @@ int launch_cta(const Params& p, cudaStream_t s) {
   constexpr size_t kSmem = sizeof(Smem<TB, GRAD>) + (GRAD ? sizeof(uint4) * kNV * TB : 0);
   auto* kern = distill_kernel<T, TB, HARD, GRAD>;
   if (const int rc = allow_smem(kern, kSmem, done)) return rc;
-  return launch_kernel(kern, (unsigned)p.rows * p.cluster, TB, kSmem, p.cluster, p.weight_sum != nullptr, s, p);
+  return launch_kernel(kern, (unsigned)p.rows * p.cluster, TB, kSmem, p.cluster, p.early, s, p);
 }
 
 template <typename T, int NV, int KE, bool HARD, bool GRAD>
@@ -718,8 +724,7 @@ int launch_warp_k(const Params& p, cudaStream_t s) {
   constexpr size_t kSmem = kWarps * sizeof(WarpSmem<T, NV, GRAD>);
   auto* kern = distill_warp_kernel<T, NV, KE, HARD, GRAD>;
   if (const int rc = allow_smem(kern, kSmem, done)) return rc;
-  return launch_kernel(kern, (unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, kSmem, 1, p.weight_sum != nullptr, s,
-                       p, batch);
+  return launch_kernel(kern, (unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, kSmem, 1, p.early, s, p, batch);
 }
 
 template <typename T, int NV, bool HARD, bool GRAD>
@@ -747,6 +752,10 @@ int launch(Params p, int nvec, cudaStream_t s) {
   // the rows in flight of two CTAs per SM better than of four
   if (nvec <= 2 * kNV * 128 * cl) return launch_cta<T, 128, HARD, GRAD>(p, s);
   if (nvec <= 2 * kNV * 256 * cl && (int64_t)p.rows * cl > 2 * sms) return launch_cta<T, 256, HARD, GRAD>(p, s);
+  // rows too long for L2 even so, where one exponential an element leaves one CTA an SM time to spare: 394 us
+  // instead of 443 at 2048 x 128256 f32 (with 512 threads 371 instead of 400 at 4000 x 64000)
+  if constexpr (GRAD && !HARD && sizeof(T) == 4)
+    if (nvec > 5 * kNV * 512 * cl) return launch_cta<T, 1024, HARD, GRAD>(p, s);
   return launch_cta<T, 512, HARD, GRAD>(p, s);
 }
 
@@ -774,9 +783,12 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
     return set_error(M3_ERR_ARG, "m3_distill: need a temperature > 0 (finite, as 1 / T) and 0 <= hard_weight <= 1");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
   if (rows > kMaxRows) return set_error(M3_ERR_SHAPE, "m3_distill: more than 2^30 rows");
-  if ((rows > 0 && (!a.logits || !a.ids || !a.teacher || !a.row_loss)) ||
-      (a.hard_weight > 0.f && rows > 0 && !a.labels) || (a.reduction != M3_REDUCE_NONE && !a.loss))
+  const bool only_grad = a.grad && !a.row_loss && !a.loss;
+  if ((rows > 0 && (!a.logits || !a.ids || !a.teacher || (!a.row_loss && !only_grad))) ||
+      (a.hard_weight > 0.f && rows > 0 && !a.labels) || (a.reduction != M3_REDUCE_NONE && !a.loss && !only_grad))
     return set_error(M3_ERR_ARG, "m3_distill: NULL pointer");
+  if ((a.ready & M3_READY_GRAD) && (!only_grad || !a.upstream || a.upstream_stride != 0))
+    return set_error(M3_ERR_ARG, "m3_distill: a ready gradient needs one upstream value and no losses");
   const bool wmean = a.reduction == M3_REDUCE_MEAN && a.weights && rows > 0;
   if (wmean && !a.weight_sum) return set_error(M3_ERR_ARG, "m3_distill: a mean with weights needs weight_sum");
   if (a.upstream_stride < 0 || a.upstream_stride > 1)
@@ -810,17 +822,19 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
   p.upstream = a.upstream;
   p.upstream_stride = a.upstream_stride;
   p.weight_sum = wmean ? a.weight_sum : nullptr;
+  p.early = wmean && !(a.ready & M3_READY_WEIGHTS);
+  p.ready = (a.ready & M3_READY_GRAD) != 0;
   p.row_loss = a.row_loss;
   auto sum = [&](const float* v, const float* div_by, float scale, float* out, bool early) {
     return launch_kernel(sum_kernel, kSumCtas, kSumThreads, 0, kSumCtas, early, s, v, (int64_t)rows, div_by, scale, out);
   };
   int rc = M3_OK;
-  if (wmean) rc = sum(a.weights, nullptr, 1.f, a.weight_sum, false);
+  if (p.early) rc = sum(a.weights, nullptr, 1.f, a.weight_sum, false);
   if (rc == M3_OK && rows > 0) {
     const int nvec = most_vectors(a.logits, a.vocab, bf ? 2 : 4, a.ld_outer, a.ld_inner);
     rc = bf ? launch<__nv_bfloat16>(p, nvec, s) : launch<float>(p, nvec, s);
   }
-  if (rc == M3_OK && a.reduction != M3_REDUCE_NONE)  // the mean of no rows is 0 / 0
+  if (rc == M3_OK && a.loss && a.reduction != M3_REDUCE_NONE)  // the mean of no rows is 0 / 0
     rc = sum(a.row_loss, p.weight_sum, a.reduction == M3_REDUCE_MEAN && !a.weights ? 1.f / (float)rows : 1.f, a.loss,
              rows > 0);
   return rc;

@@ -159,7 +159,7 @@ class M3DistillArgs(ctypes.Structure):
         ("logits", _vp), ("ld_outer", _i64), ("ld_inner", _i64),
         ("ids", _vp), ("teacher", _vp), ("labels", _vp), ("weights", _vp), ("upstream", _vp),
         ("upstream_stride", _i64), ("row_loss", _vp), ("loss", _vp), ("weight_sum", _vp),
-        ("grad", _vp), ("g_outer", _i64), ("g_inner", _i64),
+        ("grad", _vp), ("g_outer", _i64), ("g_inner", _i64), ("ready", _i32), ("reserved", _i32),
     ]
 
 
@@ -185,6 +185,8 @@ M3_MAX_TOP = 128
 M3_REDUCE_NONE = 0
 M3_REDUCE_SUM = 1
 M3_REDUCE_MEAN = 2
+M3_READY_WEIGHTS = 1
+M3_READY_GRAD = 2
 
 EXPORTS = ("m3_siso_fwd", "m3_siso_fwd_workspace_size", "m3_siso_bwd", "m3_siso_bwd_workspace_size", "m3_siso_decode",
            "m3_last_error", "m3_version", "m3_siso_bwd_noalloc", "m3_siso_bwd_noalloc_scratch_bytes",

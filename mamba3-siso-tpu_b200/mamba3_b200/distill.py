@@ -67,48 +67,64 @@ def _check(logits, ids, teacher, labels, weights, temperature, hard_weight, redu
 
 
 def _run(logits, ids, teacher, labels, weights, temperature, hard_weight, reduction, grad=None, upstream=None,
-         grad_scale=1.0):
-    """One m3_distill call on checked inputs: the reduced loss, or the rows' losses."""
+         grad_scale=1.0, weight_sum=None, want_loss=True, ready=0):
+    """One m3_distill call on checked inputs: the reduced loss, or the rows' losses (None unless
+    wanted).  ``weight_sum``: one float that a mean with weights leaves their sum in."""
     lead, dev = logits.shape[:-1], logits.device
     nd = len(lead)
     outer, inner = T.row_counts(lead)
     logits, (ld_outer, ld_inner) = T.row_input(logits, nd)
     g_outer, g_inner = (0, 0) if grad is None else T.rows2(grad, nd)
-    loss = row_loss = None
-    if reduction == "none":
-        row_loss = torch.empty(lead, dtype=torch.float32, device=dev)
-        at = row_loss.data_ptr()
-        loss_at = scratch_at = None
-    else:  # the workspace: the sum of weights, the rows' losses
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        work = torch.empty(1 + outer * inner, dtype=torch.float32, device=dev)
-        loss_at, scratch_at = loss.data_ptr(), work.data_ptr()
-        at = scratch_at + 4
+    result = rows_at = loss_at = None
+    sum_at = T.ptr(weight_sum)
+    if want_loss and reduction == "none":
+        result = torch.empty(lead, dtype=torch.float32, device=dev)
+        rows_at = result.data_ptr()
+    elif want_loss:
+        result = torch.empty((), dtype=torch.float32, device=dev)
+        work = torch.empty(1 + outer * inner, dtype=torch.float32, device=dev)  # sum of weights, rows' losses
+        loss_at, rows_at = result.data_ptr(), work.data_ptr() + 4
+        sum_at = sum_at or work.data_ptr()
     stride = 0 if upstream is None or upstream.dim() == 0 or upstream.numel() == 1 else 1
     a = C.M3DistillArgs(outer, inner, logits.shape[-1], ids.shape[-1], T.io_dtype(logits.dtype), _REDUCE[reduction],
                         temperature, hard_weight, grad_scale, logits.data_ptr(), ld_outer, ld_inner, ids.data_ptr(),
-                        teacher.data_ptr(), T.ptr(labels), T.ptr(weights), T.ptr(upstream), stride, at, loss_at,
-                        scratch_at, T.ptr(grad), g_outer, g_inner)
+                        teacher.data_ptr(), T.ptr(labels), T.ptr(weights), T.ptr(upstream), stride, rows_at, loss_at,
+                        sum_at, T.ptr(grad), g_outer, g_inner, ready, 0)
     T.call(C.lib().m3_distill, a, dev)
-    return row_loss if loss is None else loss
+    return result
 
 
 class _DistillFn(torch.autograd.Function):
-    """The forward reads the logits once; the backward reads them once more and writes their
-    gradient, the softmax recomputed in the same pass (nothing but the inputs is saved)."""
+    """A reduced loss comes with its gradient from one read of the logits: the backward, whose
+    upstream gradient is 1 in a plain ``loss.backward()``, then only looks at that and returns it; with
+    another upstream (or a second backward) it reads the logits again.  The rows' losses have one upstream
+    each, so theirs is always written in the backward."""
 
     @staticmethod
     def forward(ctx, logits, ids, teacher, labels, weights, temperature, hard_weight, reduction):
         ctx.save_for_backward(logits, ids, teacher, labels, weights)
         ctx.opts = (temperature, hard_weight, reduction)
-        return _run(logits, ids, teacher, labels, weights, temperature, hard_weight, reduction)
+        ctx.grad = ctx.weight_sum = None
+        if reduction != "none":
+            ctx.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            if weights is not None:
+                ctx.weight_sum = torch.empty(1, dtype=torch.float32, device=logits.device)
+        return _run(logits, ids, teacher, labels, weights, *ctx.opts, grad=ctx.grad, weight_sum=ctx.weight_sum)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        logits = ctx.saved_tensors[0]
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _run(*ctx.saved_tensors, *ctx.opts, grad=grad, upstream=dloss.float().contiguous())
+        saved = ctx.saved_tensors
+        logits, weights = saved[0], saved[4]
+        grad, ctx.grad = ctx.grad, None  # handed out once: its next owner may write to it
+        ready = 0 if grad is None else C.M3_READY_GRAD
+        if grad is None:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        total = ctx.weight_sum
+        if total is not None:
+            ready |= C.M3_READY_WEIGHTS
+        _run(*saved, *ctx.opts, grad=grad, upstream=dloss.float().contiguous(), weight_sum=total, want_loss=False,
+             ready=ready)
         return (grad,) + (None,) * 7
 
 

@@ -307,6 +307,35 @@ def test_backward_twice_and_grad_scale():
 
 
 @CUDA
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("vocab", [300, 5000])
+def test_upstream_of_one_and_others(vocab, weighted, reduction):
+    """The gradient that came with the loss, and the ones written in the backward, whatever was done to
+    the first in between."""
+    from mamba3_b200 import distill as D
+
+    x, ids, teacher, labels, weights = _cuda(*_case(9, vocab, 6, BF, 2, 0.3, weighted=weighted))
+    args = dict(labels=labels, hard_weight=0.3, weights=weights, temperature=1.5)
+    leaf = x.clone().requires_grad_(True)
+    loss = D.distill_loss(leaf, ids, teacher, reduction=reduction, **args)
+    one = torch.ones_like(loss)
+    first, = torch.autograd.grad(loss, leaf, one, retain_graph=True)
+    keep = first.clone()
+    first.fill_(5.0)
+    again, = torch.autograd.grad(loss, leaf, one, retain_graph=True)
+    twice, = torch.autograd.grad(loss, leaf, 2.0 * one, retain_graph=True)
+    zero, = torch.autograd.grad(loss, leaf, 0.0 * one)
+    assert torch.equal(again, keep) and torch.equal(twice, 2.0 * keep) and not zero.any()
+    fresh = x.clone().requires_grad_(True)
+    other, = torch.autograd.grad(D.distill_loss(fresh, ids, teacher, reduction=reduction, **args), fresh, 2.0 * one)
+    assert torch.equal(other, 2.0 * keep)
+    if reduction != "none":
+        l2, dx = D.distill_loss_and_grad(x, ids, teacher, reduction=reduction, **args)
+        assert torch.equal(dx, keep) and torch.equal(l2, loss.detach())
+
+
+@CUDA
 def test_no_rows():
     from mamba3_b200 import distill as D
 
@@ -366,3 +395,7 @@ def test_entry_point_checks_its_arguments():
     assert f(a, None) == C.M3_ERR_ARG
     a.reduction, a.logits, a.ids, a.teacher, a.row_loss, a.hard_weight = 0, 16, 16, 16, 16, 0.5
     assert f(a, None) == C.M3_ERR_ARG  # no labels
+    a.hard_weight, a.ready = 0.0, C.M3_READY_GRAD
+    assert f(a, None) == C.M3_ERR_ARG  # a ready gradient without a gradient
+    a.ready, a.row_loss = 0, None
+    assert f(a, None) == C.M3_ERR_ARG  # neither losses nor a gradient
