@@ -40,10 +40,6 @@ struct Params {
   bool early;  // the sum of weights is the kernel in front of this one
 };
 
-// A mean's kernels (sum of weights, rows, sum of losses) are launched so that each may start before the
-// one in front of it has ended; what it needs of that one's results it reads behind this.
-__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // The gradient is there already (the same for all threads).
 __device__ __forceinline__ bool nothing_to_do(const Params& p) { return p.ready && *p.upstream == 1.f; }
 
@@ -641,7 +637,7 @@ __global__ void __launch_bounds__(kSumThreads)
     sum_kernel(const float* __restrict__ v, int64_t n, const float* div_by, float scale, float* out) {
   __shared__ float sm[32], total[kSumCtas];
   const int tid = threadIdx.x, rank = cluster_rank();
-  asm volatile("griddepcontrol.launch_dependents;");
+  next_may_start();
   cluster_arrive_relaxed();
   after_previous();
   float s = 0.f;
@@ -670,31 +666,6 @@ int sm_count() {
   return c;
 }
 
-// `early`: the kernel may start before the one in front of it in the stream has ended.
-template <typename... P, typename... A>
-int launch_kernel(void (*kern)(P...), unsigned grid, int block, size_t smem, int cluster, bool early, cudaStream_t s, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(block, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[2];
-  cfg.attrs = at;
-  if (cluster > 1) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    at[cfg.numAttrs].val.clusterDim.x = cluster;
-    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
-    ++cfg.numAttrs;
-  }
-  if (early) {
-    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_distill: ") + cudaGetErrorString(e));
-}
-
 // Allows a kernel its shared memory, once per device (`done`: the kernel's own).
 template <typename K>
 int allow_smem(K kern, size_t bytes, bool (&done)[64]) {
@@ -713,7 +684,7 @@ int launch_cta(const Params& p, cudaStream_t s) {
   constexpr size_t kSmem = sizeof(Smem<TB, GRAD>) + (GRAD ? sizeof(uint4) * kNV * TB : 0);
   auto* kern = distill_kernel<T, TB, HARD, GRAD>;
   if (const int rc = allow_smem(kern, kSmem, done)) return rc;
-  return launch_kernel(kern, (unsigned)p.rows * p.cluster, TB, kSmem, p.cluster, p.early, s, p);
+  return launch_ex("m3_distill", kern, (unsigned)p.rows * p.cluster, TB, kSmem, p.cluster, p.early, s, p);
 }
 
 template <typename T, int NV, int KE, bool HARD, bool GRAD>
@@ -724,7 +695,7 @@ int launch_warp_k(const Params& p, cudaStream_t s) {
   constexpr size_t kSmem = kWarps * sizeof(WarpSmem<T, NV, GRAD>);
   auto* kern = distill_warp_kernel<T, NV, KE, HARD, GRAD>;
   if (const int rc = allow_smem(kern, kSmem, done)) return rc;
-  return launch_kernel(kern, (unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, kSmem, 1, p.early, s, p, batch);
+  return launch_ex("m3_distill", kern, (unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, kSmem, 1, p.early, s, p, batch);
 }
 
 template <typename T, int NV, bool HARD, bool GRAD>
@@ -826,7 +797,7 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
   p.ready = (a.ready & M3_READY_GRAD) != 0;
   p.row_loss = a.row_loss;
   auto sum = [&](const float* v, const float* div_by, float scale, float* out, bool early) {
-    return launch_kernel(sum_kernel, kSumCtas, kSumThreads, 0, kSumCtas, early, s, v, (int64_t)rows, div_by, scale, out);
+    return launch_ex("m3_distill", sum_kernel, kSumCtas, kSumThreads, 0, kSumCtas, early, s, v, (int64_t)rows, div_by, scale, out);
   };
   int rc = M3_OK;
   if (p.early) rc = sum(a.weights, nullptr, 1.f, a.weight_sum, false);

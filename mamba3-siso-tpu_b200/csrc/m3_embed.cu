@@ -15,7 +15,7 @@
 namespace m3 {
 namespace {
 
-using vocab::Rows;
+using namespace vocab;
 
 constexpr int kThreads = 256;
 constexpr int64_t kMaxLd = 1 << 30;  // elements between rows of a table
@@ -213,8 +213,7 @@ __global__ void __launch_bounds__(kClearThreads) clear_kernel(const ClearParams 
       for (int64_t b = lane * 2; b < p.row_bytes; b += 64) *reinterpret_cast<uint16_t*>(g + b) = 0;
     }
   }
-  // the kernel behind this one reads what the sort writes
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_previous();  // the kernel behind this one reads what the sort writes
 }
 
 // Each of the cluster's warps owns a contiguous piece of the input; positions are handed out
@@ -224,7 +223,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SortSmem& s = *reinterpret_cast<SortSmem*>(smem_raw);
-  asm volatile("griddepcontrol.launch_dependents;");  // a clear_kernel behind this one may start
+  next_may_start();  // the clear needs nothing of this kernel; the sums wait in place
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank();
   const int ctas = (int)cluster.num_blocks();
   const int bins = 1 << p.bits;
@@ -381,6 +380,7 @@ constexpr int kAhead = 4;  // entries in flight (8, with half the warps an SM ho
 
 template <typename D, typename G, int N>
 __global__ void __launch_bounds__(kThreads) sum_kernel(const SumParams p) {
+  after_previous();
   const int n = *p.count;
   if ((int)blockIdx.x >= p.sum_ctas) {
     // the rows of tokens that do not occur: a warp looks 32 of them up and clears those
@@ -474,6 +474,7 @@ constexpr int kJoinWidth = 8, kJoinChunks = 16, kJoinAhead = 4;
 template <typename G, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(const SumParams p) {
   constexpr int kGroups = kThreads / kJoinWidth;
+  after_previous();
   __shared__ float sums[kThreads / 32][kJoinWidth * N];
   const int n = *p.count, lane = threadIdx.x & 31;
   const int64_t k = (int64_t)blockIdx.x * kJoinChunks + lane, b1 = (k + 1) * p.chunk;
@@ -601,27 +602,31 @@ int chunk_of(int64_t rows, int dim) {
 }
 
 template <typename D, typename G, int N>
-void launch_sum(SumParams p, int64_t rows, cudaStream_t s) {
+int launch_sum(SumParams p, int64_t rows, cudaStream_t s) {
   p.cols = columns(p.dim, N);
   const int y = slabs(p.dim, N, p.cols);
   const int64_t chunks = (rows + p.chunk - 1) / p.chunk;
   p.sum_ctas = (int)((chunks + p.cols.groups - 1) / p.cols.groups);
   const int64_t want = (p.vocab + 32 * (kThreads / 32) - 1) / (32 * (kThreads / 32)), most = (int64_t)sm_count() * 8;
   const int64_t clear = !p.clear ? 0 : want < most ? want : most;
-  if (p.sum_ctas + clear > 0) sum_kernel<D, G, N><<<dim3((unsigned)(p.sum_ctas + clear), y), kThreads, 0, s>>>(p);
-  if (chunks > 1)
-    join_kernel<G, N><<<dim3((unsigned)((chunks + kJoinChunks - 2) / kJoinChunks), (p.dim + N * kJoinWidth - 1) / (N * kJoinWidth)), kThreads,
-                        0, s>>>(p);
+  int rc = M3_OK;
+  if (p.sum_ctas + clear > 0)
+    rc = launch_ex("m3_embed_bwd", sum_kernel<D, G, N>, dim3((unsigned)(p.sum_ctas + clear), y), kThreads, 0, 1, true, s, p);
+  if (rc == M3_OK && chunks > 1)
+    rc = launch_ex("m3_embed_bwd", join_kernel<G, N>,
+                   dim3((unsigned)((chunks + kJoinChunks - 2) / kJoinChunks), (p.dim + N * kJoinWidth - 1) / (N * kJoinWidth)),
+                   kThreads, 0, 1, true, s, p);
+  return rc;
 }
 
 template <typename D, typename G>
-void launch_sum(const SumParams& p, int64_t rows, int64_t dy_outer, int64_t dy_inner, cudaStream_t s) {
+int launch_sum(const SumParams& p, int64_t rows, int64_t dy_outer, int64_t dy_inner, cudaStream_t s) {
   auto fits = [&](int n) {
     return whole(p.dy, sizeof(D), n, p.dim, dy_outer, dy_inner) && whole(p.grad, sizeof(G), n, p.dim, p.grad_ld, 0);
   };
   if (fits(8)) return launch_sum<D, G, 8>(p, rows, s);
   if (fits(2)) return launch_sum<D, G, 2>(p, rows, s);
-  launch_sum<D, G, 1>(p, rows, s);
+  return launch_sum<D, G, 1>(p, rows, s);
 }
 
 }  // namespace
@@ -706,19 +711,9 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   // a CTA for every 2048 tokens: the cluster's barriers cost more than a few tokens a lane
   int sort_ctas = 1;
   while (sort_ctas < kSortMostCtas && rows > 2048 * sort_ctas) sort_ctas *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)sort_ctas, 1, 1);
-  cfg.blockDim = dim3(kSortThreads, 1, 1);
-  cfg.dynamicSmemBytes = sizeof(SortSmem);
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = sort_ctas;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, sort_kernel, sp);
-  if (e != cudaSuccess) return set_error(M3_ERR_LAUNCH, std::string("m3_embed_bwd: ") + cudaGetErrorString(e));
+  if (const int rc = launch_ex("m3_embed_bwd", sort_kernel, (unsigned)sort_ctas, kSortThreads, sizeof(SortSmem), sort_ctas,
+                               false, s, sp))
+    return rc;
   // Rows of absent tokens are cleared beside the sort by CTAs that each read all tokens; where that is
   // more to read than there is to clear, or the bitmap does not fit, the sums' launch looks them up.
   const int64_t row_bytes = (int64_t)a.dim * (int64_t)gs, all_bytes = row_bytes * a.vocab;
@@ -728,13 +723,9 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   if (beside) {
     const ClearParams cp{(int)rows, a.vocab, sp.trow, a.tokens, (unsigned char*)a.grad, row_bytes,
                          a.grad_ld * (int64_t)gs};
-    cfg.gridDim = dim3((unsigned)ctas, 1, 1);
-    cfg.blockDim = dim3(kClearThreads, 1, 1);
-    cfg.dynamicSmemBytes = ((size_t)a.vocab + 31) / 32 * 4;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    e = cudaLaunchKernelEx(&cfg, clear_kernel, cp);
-    if (e != cudaSuccess) return set_error(M3_ERR_LAUNCH, std::string("m3_embed_bwd: ") + cudaGetErrorString(e));
+    if (const int rc = launch_ex("m3_embed_bwd", clear_kernel, (unsigned)ctas, kClearThreads, ((size_t)a.vocab + 31) / 32 * 4,
+                                 1, true, s, cp))
+      return rc;
   }
   const SumParams p{(int)a.grad_ld,
                     a.dim,
@@ -754,8 +745,8 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   using bf16 = __nv_bfloat16;
   const bool gb = a.grad_dtype == M3_DTYPE_BF16;
   if (a.dy_dtype == M3_DTYPE_BF16)
-    gb ? launch_sum<bf16, bf16>(p, rows, a.dy_outer, a.dy_inner, s) : launch_sum<bf16, float>(p, rows, a.dy_outer, a.dy_inner, s);
-  else
-    gb ? launch_sum<float, bf16>(p, rows, a.dy_outer, a.dy_inner, s) : launch_sum<float, float>(p, rows, a.dy_outer, a.dy_inner, s);
-  return check_launch("m3_embed_bwd");
+    return gb ? launch_sum<bf16, bf16>(p, rows, a.dy_outer, a.dy_inner, s)
+              : launch_sum<bf16, float>(p, rows, a.dy_outer, a.dy_inner, s);
+  return gb ? launch_sum<float, bf16>(p, rows, a.dy_outer, a.dy_inner, s)
+            : launch_sum<float, float>(p, rows, a.dy_outer, a.dy_inner, s);
 }

@@ -733,18 +733,8 @@ int sm_count() {
 
 template <typename T, int TB, bool TOP>
 int launch_cta(const Params& p, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.rows * p.cluster, 1, 1);
-  cfg.blockDim = dim3(TB, 1, 1);
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = p.cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, score_kernel<T, TB, TOP>, p);
-  return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string("m3_token_logprobs: ") + cudaGetErrorString(e));
+  return launch_ex("m3_token_logprobs", score_kernel<T, TB, TOP>, (unsigned)p.rows * p.cluster, TB, 0, p.cluster, false, s,
+                   p);
 }
 
 template <typename T, int NV, bool TOP>

@@ -2,7 +2,10 @@
 // strides, the order of logits, and the running (max, sum) of a softmax.
 #pragma once
 
+#include <string>
+
 #include "m3_common.cuh"
+#include "m3_internal.h"
 
 namespace m3 {
 namespace vocab {
@@ -319,6 +322,38 @@ __device__ __forceinline__ P* peer(P* p, int rank) {
   uint64_t a;
   asm volatile("mapa.u64 %0, %1, %2;" : "=l"(a) : "l"((uint64_t)p), "r"(rank));
   return reinterpret_cast<P*>(a);
+}
+
+// ---- launches that overlap -------------------------------------------------------------------
+// A kernel launched `early` may start before the one in front of it in the stream has ended (from that
+// one's next_may_start on, or as its CTAs end); what it needs of that one's results it reads behind
+// after_previous().
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+template <typename... P, typename... A>
+int launch_ex(const char* what, void (*kern)(P...), dim3 grid, int block, size_t smem, int cluster, bool early,
+              cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  cfg.attrs = at;
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (early) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 }  // namespace vocab
