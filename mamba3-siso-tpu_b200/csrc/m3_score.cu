@@ -581,6 +581,11 @@ __global__ void __launch_bounds__(kWarpThreads) score_warp_kernel(const Params p
 // soon for a CTA's.  BEST: 0 without alternatives; else the bound is the top-th largest of every lane's BEST
 // largest vector maxima (1 for up to 8 alternatives; 2 for up to 32, where the lanes' maxima alone would
 // let a hundred candidates through and overflow the lists).
+// NV: vectors a lane loads at a time, no more than the row has, and registers bounded so that 3 to 5 CTAs are
+// resident; the selection hides its latency behind other warps, and a few spilled registers cost it less than
+// a CTA.  Measured, with tiles of 8 without a bound against these: 262144 x 1024 bf16 without alternatives
+// 141 -> 112 us, with 8 413 -> 258; 131072 x 2048 f32 with 8 302 -> 237; 38400 x 256 f32 with 1 46 -> 28.
+// Tiles of 4 for the longer rows too: with 8 alternatives 237 -> 266 us, as their bound rises more often.
 constexpr int kRowVecCap = 96, kRowCandCap = 128, kRowMostTop = 32;
 
 struct RowSmem {
@@ -590,8 +595,9 @@ struct RowSmem {
   int n_cand;
 };
 
-template <typename T, int BEST>
-__global__ void __launch_bounds__(kWarpThreads) score_rows_kernel(const Params p, int batch) {
+template <typename T, int NV, int BEST>
+__global__ void __launch_bounds__(kWarpThreads, NV == 2 ? 5 : NV == 4 || BEST ? 4 : 3) score_rows_kernel(
+    const Params p, int batch) {
   constexpr int E = kVec<T>;
   constexpr bool TOP = BEST > 0;
   __shared__ RowSmem smem[TOP ? kWarps : 1];
@@ -619,12 +625,12 @@ __global__ void __launch_bounds__(kWarpThreads) score_rows_kernel(const Params p
         ref = r;
       }
     };
-    walk<T, kNV, 32>(v, n, lane, Keep::kNo, [&](const uint4(&d)[kNV], int base, auto full) {
-      VecMax<T> vm[kNV];
-      const float mt = vecs_max<T, kNV>(d, vm, [&](int j) { return full.value || base + j * 32 < n; });
+    walk<T, NV, 32>(v, n, lane, Keep::kNo, [&](const uint4(&d)[NV], int base, auto full) {
+      VecMax<T> vm[NV];
+      const float mt = vecs_max<T, NV>(d, vm, [&](int j) { return full.value || base + j * 32 < n; });
       raise(warp_max(mt));
 #pragma unroll
-      for (int j = 0; j < kNV; ++j)
+      for (int j = 0; j < NV; ++j)
         if (full.value || base + j * 32 < n) add_vec<T>(d[j], ref, c, s2, u2);
       if constexpr (TOP) {
         bool higher;  // a change of the top-th largest
@@ -634,7 +640,7 @@ __global__ void __launch_bounds__(kWarpThreads) score_rows_kernel(const Params p
         } else {
           const float before = best[1];
 #pragma unroll
-          for (int j = 0; j < kNV; ++j)
+          for (int j = 0; j < NV; ++j)
             if (full.value || base + j * 32 < n) {
               const float f = vm[j].value();
               best[1] = fmaxf(best[1], fminf(best[0], f));
@@ -655,7 +661,7 @@ __global__ void __launch_bounds__(kWarpThreads) score_rows_kernel(const Params p
         }
         if (__any_sync(0xffffffffu, mt >= bound)) {
 #pragma unroll
-          for (int j = 0; j < kNV; ++j) {
+          for (int j = 0; j < NV; ++j) {
             if (!full.value && base + j * 32 >= n) break;
             const bool put = (full.value || base + j * 32 + lane < n) && vm[j].reaches(bound);
             const unsigned who = __ballot_sync(0xffffffffu, put);
@@ -745,12 +751,20 @@ int launch_warp(const Params& p, cudaStream_t s) {
   return check_launch("m3_token_logprobs");
 }
 
-template <typename T, int BEST>
-int launch_rows(const Params& p, cudaStream_t s) {
+template <typename T, int NV, int BEST>
+int launch_rows_n(const Params& p, cudaStream_t s) {
   const int batch = warp_batch(p.rows, sm_count());
   const int warps = (p.rows + batch - 1) / batch;
-  score_rows_kernel<T, BEST><<<(unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, 0, s>>>(p, batch);
+  score_rows_kernel<T, NV, BEST><<<(unsigned)((warps + kWarps - 1) / kWarps), kWarpThreads, 0, s>>>(p, batch);
   return check_launch("m3_token_logprobs");
+}
+
+// Tiles no larger than the row: fewer registers, more warps.
+template <typename T, int BEST>
+int launch_rows(const Params& p, int nvec, cudaStream_t s) {
+  if (nvec <= 64) return launch_rows_n<T, 2, BEST>(p, s);
+  if (nvec <= 128) return launch_rows_n<T, 4, BEST>(p, s);
+  return launch_rows_n<T, 8, BEST>(p, s);
 }
 
 // A row goes to a warp while its vectors fit the lanes' registers (one each; with many alternatives two, which
@@ -761,8 +775,8 @@ int launch(Params p, int nvec, cudaStream_t s) {
   if (nvec <= 32) return launch_warp<T, 1, TOP>(p, s);
   const bool few = !TOP || p.top <= kRowMostTop;
   if (few && (nvec <= 32 * kNV || (nvec <= 4 * 32 * kNV && p.rows >= 16 * sm_count()))) {
-    if constexpr (!TOP) return launch_rows<T, 0>(p, s);
-    return p.top <= 8 ? launch_rows<T, 1>(p, s) : launch_rows<T, 2>(p, s);
+    if constexpr (!TOP) return launch_rows<T, 0>(p, nvec, s);
+    return p.top <= 8 ? launch_rows<T, 1>(p, nvec, s) : launch_rows<T, 2>(p, nvec, s);
   }
   if constexpr (TOP)
     if (nvec <= 64) return launch_warp<T, 2, TOP>(p, s);
