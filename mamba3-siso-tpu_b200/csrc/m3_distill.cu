@@ -505,9 +505,19 @@ struct alignas(16) WarpSmem {
   uint32_t seen[GRAD ? NV * kVec<T> : 1];  // a bit per element
 };
 
+// CTAs that have to fit an SM, which bounds the registers.  Measured, without a bound against this one: 65536 x 4096
+// bf16 with gradient 355 -> 272 us, 131072 x 2048 bf16 260 -> 241, with 64 entries for 1024 181 -> 165, with
+// hard labels for 1024 212 -> 181; one CTA more for each spills and is slower (1024, 64 entries: 185).
+template <int NV, int KE, bool HARD>
+constexpr int kWarpCtas = NV == 1   ? 0  // the compiler's own choice
+                          : NV == 2 ? 4
+                          : NV == 4 ? (KE > 1 ? 3 : HARD ? 4 : 0)
+                          : NV == 8 ? (KE > 1 ? 2 : 3)
+                                    : 2;
+
 // KE: 1 for up to 32 entries, which are most lists, else kEnt.
 template <typename T, int NV, int KE, bool HARD, bool GRAD>
-__global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Params p, int batch) {
+__global__ void __launch_bounds__(kWarpThreads, kWarpCtas<NV, KE, HARD>) distill_warp_kernel(const Params p, int batch) {
   constexpr int E = kVec<T>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   WarpSmem<T, NV, GRAD>& s = reinterpret_cast<WarpSmem<T, NV, GRAD>*>(smem_raw)[threadIdx.x >> 5];
