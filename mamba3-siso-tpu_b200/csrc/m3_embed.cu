@@ -6,7 +6,8 @@
 // than that are joined.  The cuts depend on the sizes alone, so the result is the same every call.
 // Floor: the rows once in, the gradient once out.  Measured, lookup and gradient together: 16384 positions
 // over 128256 x 2048 fp32 232 us (5.7 TB/s: the clear runs beside the sort at the rate of writes), 131072
-// positions over 256 x 512 98 us (2.8 TB/s: lookup 29, sort 17, chunk sums 30, join 15 by themselves).
+// positions over 256 x 512 94 us (2.9 TB/s: lookup 29, sort 17, chunk sums 30, join 15 by themselves; the
+// gradient's launches overlap, without that 98).
 #include <cooperative_groups.h>
 
 #include "m3_internal.h"

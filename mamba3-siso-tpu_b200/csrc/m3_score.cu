@@ -3,7 +3,7 @@
 // One read of the logits, which is the floor: about 6 instructions an element (load, unpack, maximum,
 // multiply-add, exponential, two sums) against 0.3 ns an element that memory gives an SM in bf16, so the
 // loops have to stay lean.  Measured at 4096 x 128256 bf16: 157 us without alternatives (6.7 TB/s), 235 with
-// 32; 4092 x 50257 f32: 126 us (6.5 TB/s); 131072 x 256 bf16 with 8: 57 us (1.4 TB/s), bound by instructions.
+// 32; 4092 x 50257 f32: 124 us (6.5 TB/s); 131072 x 256 bf16 with 8: 57 us (1.4 TB/s), bound by instructions.
 //
 // Rows go to threads by their length (see launch): a warp that holds a short row in registers, a warp that
 // walks a row of some thousand entries, or a CTA that walks a long one.  Each warp walks its share with a

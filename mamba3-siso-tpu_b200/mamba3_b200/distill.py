@@ -139,7 +139,11 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     row of weight 0, or with neither entries nor label, contributes exactly 0 to the loss and
     the gradient whatever its logits are.  An id or label at or past V makes its row NaN.
     ``reduction``: "mean" over the weights' sum (or the row count), "sum", or "none" for the
-    rows' losses."""
+    rows' losses.
+
+    With gradients enabled a "mean" or "sum" forms the gradient together with the loss, in memory of
+    the logits' size that the backward hands on; a backward whose upstream gradient is not 1 (a
+    scaled loss) reads the logits again, where `distill_loss_and_grad`'s ``grad_scale`` does not."""
     side = _check(logits, teacher_ids, teacher_logits, labels, weights, temperature, hard_weight, reduction)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillFn.apply(logits, *side, float(temperature), float(hard_weight), reduction)
