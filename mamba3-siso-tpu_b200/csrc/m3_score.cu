@@ -807,6 +807,7 @@ extern "C" int m3_token_logprobs(const M3ScoreArgs* args, void* stream) {
   if (!temperature_ok(a.temperature))
     return set_error(M3_ERR_ARG, "m3_token_logprobs: temperature must be > 0, finite and not so small that 1 / T overflows");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
+  if (rows > kMaxRows) return set_error(M3_ERR_SHAPE, "m3_token_logprobs: more than 2^30 rows");
   if (rows == 0) return M3_OK;
   if (!a.logits || !a.entropy || !a.lse || (a.targets && !a.logprob) || (a.top > 0 && (!a.top_logprob || !a.top_ids)))
     return set_error(M3_ERR_ARG, "m3_token_logprobs: NULL pointer");
