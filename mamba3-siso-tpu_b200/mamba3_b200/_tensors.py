@@ -157,3 +157,8 @@ def call(fn, args, device):
         rc = fn(args, _raw_stream(device.index) if _raw_stream else stream_handle(device))
     if rc:
         C.check(rc)
+
+
+def written(t):
+    """Tells autograd that a kernel wrote to the caller's ``t``, so that a backward that saved its old values raises."""
+    torch.autograd.graph.increment_version(t)

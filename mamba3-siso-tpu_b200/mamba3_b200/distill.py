@@ -156,12 +156,14 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
                           out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """`distill_loss` ("mean" or "sum") and ``grad_scale`` times its gradient with respect to the
     logits, in the logits' dtype, from one read of them.  ``out`` takes the gradient; it may be
-    ``logits`` itself, which are then overwritten."""
+    ``logits`` itself, which are then overwritten: as after any in-place operation, a backward
+    that saved them raises."""
     if reduction == "none":
         raise ValueError("reduction must be 'mean' or 'sum'")
     side = _check(logits, teacher_ids, teacher_logits, labels, weights, temperature, hard_weight, reduction)
     nd = logits.dim() - 1
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     elif out.requires_grad and out.is_leaf and torch.is_grad_enabled():
         raise ValueError("out must not be a leaf that requires grad")
@@ -172,6 +174,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
     elif not _apart_or_same(out, logits):
         raise ValueError("out must be the logits themselves or share no memory with them")
     loss = _run(logits, *side, temperature, hard_weight, reduction, grad=out, grad_scale=grad_scale)
+    if given:
+        T.written(out)
     return loss, out
 
 

@@ -97,4 +97,6 @@ def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: fl
                          tokens.data_ptr(), t_outer, t_inner, dy.data_ptr(), dy_outer, dy_inner, out.data_ptr(),
                          out.stride(0), ws.data_ptr(), size)
     T.call(lib.m3_embed_bwd, a, dev)
+    if add:
+        T.written(out)
     return out

@@ -1,0 +1,50 @@
+"""The vocabulary-end operators as torch calls: what autograd is told of writes, and what is refused."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _lists(rows, vocab, k=5, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, vocab, (rows, k), generator=g).cuda()
+    return torch.randn(rows, vocab, generator=g).cuda(), ids, torch.randn(rows, k, generator=g).cuda()
+
+
+@pytest.mark.parametrize("vocab", [300, 9000])
+def test_overwritten_logits_are_not_differentiated(vocab):
+    """Another loss saved the logits that ``out=`` then overwrites: its backward must not run on the gradient."""
+    from mamba3_b200 import distill as D
+
+    x, ids, teacher = _lists(6, vocab)
+    leaf = x.clone().requires_grad_(True)
+    for other in (lambda t: torch.logsumexp(t, -1).square().sum(), lambda t: D.distill_loss(t, ids, teacher)):
+        logits = leaf * 1.0
+        loss, view = other(logits), logits.detach()
+        before = logits._version
+        D.distill_loss_and_grad(view, ids, teacher, out=view)
+        assert logits._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    # memory of its own: the other loss goes on
+    logits = leaf * 1.0
+    loss = torch.logsumexp(logits, -1).square().sum()
+    D.distill_loss_and_grad(logits.detach(), ids, teacher, out=torch.empty_like(x))
+    loss.backward()
+    with torch.inference_mode():  # tensors without a version
+        y = x.clone()
+        _, dx = D.distill_loss_and_grad(y, ids, teacher, out=y)
+    assert torch.equal(dx, D.distill_loss_and_grad(x, ids, teacher)[1])
+
+
+def test_table_added_to_is_not_differentiated():
+    from mamba3_b200 import embedding as E
+
+    leaf = torch.randn(20, 8, device="cuda").requires_grad_(True)
+    held = leaf * 1.0
+    loss = held.square().sum()
+    tokens, dy = torch.arange(5, device="cuda"), torch.ones(5, 8, device="cuda")
+    E.embedding_grad(dy, tokens, 20, out=held.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
