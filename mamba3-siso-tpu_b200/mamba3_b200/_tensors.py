@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import math
 import weakref
 
 import torch
@@ -162,3 +163,20 @@ def call(fn, args, device):
 def written(t):
     """Tells autograd that a kernel wrote to the caller's ``t``, so that a backward that saved its old values raises."""
     torch.autograd.graph.increment_version(t)
+
+
+def _span(t):
+    """Bytes from a tensor's first element to past its last."""
+    return t.element_size() * (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+
+
+def apart(a, b) -> bool:
+    """Two tensors with contiguous last axes have no byte in common (certainly: apart in memory, or column
+    ranges of rows whose distances have a common divisor)."""
+    if not a.numel() or not b.numel():
+        return True
+    d = b.data_ptr() - a.data_ptr()
+    if d >= _span(a) or -d >= _span(b):
+        return True
+    pitch = math.gcd(*(st * t.element_size() for t in (a, b) for n, st in zip(t.shape[:-1], t.stride()) if n > 1))
+    return pitch > 0 and a.shape[-1] * a.element_size() <= d % pitch <= pitch - b.shape[-1] * b.element_size()

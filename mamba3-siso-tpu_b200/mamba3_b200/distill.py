@@ -171,32 +171,12 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_ids: torch.Tensor, teach
         raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype} on {logits.device}")
     elif not _writable_rows(out, nd):
         raise ValueError("out must have a contiguous vocabulary axis and rows that do not overlap")
-    elif not _apart_or_same(out, logits):
+    elif not (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()) and not T.apart(out, logits):
         raise ValueError("out must be the logits themselves or share no memory with them")
     loss = _run(logits, *side, temperature, hard_weight, reduction, grad=out, grad_scale=grad_scale)
     if given:
         T.written(out)
     return loss, out
-
-
-def _span(t):
-    """Elements from a tensor's first to past its last."""
-    return 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else 0
-
-
-def _apart_or_same(a, b) -> bool:
-    """Two tensors of one shape and dtype are the same view, or have no element in common (certainly:
-    apart in memory, or column ranges of rows of one pitch)."""
-    d = (b.data_ptr() - a.data_ptr()) / a.element_size()
-    if d == 0 and a.stride() == b.stride():
-        return True
-    if d >= _span(a) or -d >= _span(b):
-        return True
-    pitches = [st for n, st in zip(a.shape[:-1], a.stride()) if n > 1]
-    if a.stride() != b.stride() or not pitches:
-        return False
-    pitch, width = min(pitches), a.shape[-1]
-    return all(st % pitch == 0 for st in pitches) and width <= d % pitch <= pitch - width
 
 
 def _writable_rows(t, nd) -> bool:

@@ -74,7 +74,7 @@ def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: fl
     """The gradient of `embed_tokens` with respect to its table: ``dy (..., D)`` -> ``(vocab, D)``
     in ``dtype``.  With ``out`` it is added to that ``(vocab, D)`` tensor instead (only the rows
     of tokens that occur are touched; each sum is rounded once), e.g. the gradient a tied head
-    has left there."""
+    has left there.  It shares no memory with ``dy``, and its version is raised."""
     if dy.dim() != tokens.dim() + 1 or dy.shape[:-1] != tokens.shape or dy.shape[-1] < 1:
         raise ValueError(f"dy must be {tuple(tokens.shape)} + (dim,), got {tuple(dy.shape)}")
     if vocab < 1:
@@ -90,6 +90,8 @@ def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: fl
     outer, inner = T.row_counts(lead)
     tokens, (t_outer, t_inner) = T.row_input(tokens, nd)
     dy, (dy_outer, dy_inner) = T.row_input(dy, nd)
+    if add and not T.apart(dy, out):
+        raise ValueError("out must share no memory with dy")
     lib = C.lib()
     size = lib.m3_embed_bwd_workspace_size(outer * inner, dim)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)

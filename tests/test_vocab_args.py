@@ -1,6 +1,9 @@
-"""What the C entries of the vocabulary-end operators refuse before anything is launched (no GPU needed)."""
+"""What the vocabulary-end operators refuse before anything is launched (no GPU needed)."""
+
+import torch
 
 from mamba3_b200 import _capi as C
+from mamba3_b200 import _tensors as T
 
 
 def test_scoring_refuses_more_rows_than_its_indices_hold():
@@ -14,3 +17,27 @@ def test_scoring_refuses_more_rows_than_its_indices_hold():
     assert C.lib().m3_token_logprobs(a, None) == C.M3_ERR_SHAPE
     a.rows_outer = 0
     assert C.lib().m3_token_logprobs(a, None) == C.M3_OK
+
+
+def test_memory_apart():
+    """Every pair of views of one buffer: certain to be apart only if no byte is in both, and found to be where
+    the views are column ranges of one pitch."""
+    buf = torch.zeros(6, 24)
+    flat = buf.view(-1)
+    views = [buf[:, lo:lo + w] for lo in (0, 3, 8, 16) for w in (1, 5, 8)]
+    views += [flat[lo:lo + 40].view(5, 8) for lo in (0, 20, 41, 80)] + [flat[24:48], buf[2], buf[::2, 8:16], buf[:0]]
+    views += [buf.view(torch.bfloat16)[:, lo:lo + 8] for lo in (0, 6, 16, 40)] + [buf.view(3, 2, 24)[:, :, 4:6]]
+
+    def held(t):
+        at = torch.zeros(6 * 24 * 4, dtype=torch.bool)
+        idx = torch.arange(6 * 24 * 4 // t.element_size()).as_strided(t.shape, t.stride(), t.storage_offset())
+        for i in idx.reshape(-1).tolist():
+            at[i * t.element_size():(i + 1) * t.element_size()] = True
+        return at
+
+    for a in views:
+        for b in views:
+            meet = bool((held(a) & held(b)).any())
+            assert not (meet and T.apart(a, b))
+            if a.dim() == b.dim() == 2 and a.stride(0) == b.stride(0) == 24:
+                assert T.apart(a, b) == (not meet)

@@ -48,3 +48,22 @@ def test_table_added_to_is_not_differentiated():
     E.embedding_grad(dy, tokens, 20, out=held.detach())
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_gradient_is_not_added_to_the_memory_it_is_read_from():
+    from mamba3_b200 import embedding as E
+
+    tokens = torch.tensor([1, 0, 1, 3], device="cuda")
+    buf = torch.ones(4, 24, device="cuda")
+    flat = buf.view(-1)
+    for dy, out in ((buf[:, :8], buf[:, :8]), (buf[:, :8], buf[:, 4:12]), (flat[:32].view(4, 8), flat[16:48].view(4, 8)),
+                    (flat[:32].view(4, 8), buf[:, :8]),
+                    (buf.view(torch.bfloat16)[:, 8:16], buf[:, :8])):  # half the bytes an element
+        with pytest.raises(ValueError, match="share no memory"):
+            E.embedding_grad(dy, tokens, 4, out=out)
+    assert (buf == 1).all()
+    # columns of one buffer that do not meet, and memory apart
+    E.embedding_grad(buf[:, :8], tokens, 4, out=buf[:, 8:16])
+    want = torch.tensor([2.0, 3.0, 1.0, 2.0], device="cuda")[:, None].expand(4, 8)
+    assert torch.equal(buf[:, 8:16], want) and (buf[:, :8] == 1).all() and (buf[:, 16:] == 1).all()
+    E.embedding_grad(flat[:32].view(4, 8), tokens, 4, out=flat[64:96].view(4, 8))
