@@ -86,6 +86,8 @@ def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: fl
         out = torch.empty((vocab, dim), dtype=dtype, device=dev)
     elif out.shape != (vocab, dim) or out.device != dev or (dim > 1 and out.stride(1) != 1) or out.stride(0) < dim:
         raise ValueError(f"out must be ({vocab}, {dim}) on {dev} with contiguous rows")
+    elif out.requires_grad and out.is_leaf and torch.is_grad_enabled():
+        raise ValueError("out must not be a leaf that requires grad")
     nd = len(lead)
     outer, inner = T.row_counts(lead)
     tokens, (t_outer, t_inner) = T.row_input(tokens, nd)

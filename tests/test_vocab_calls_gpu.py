@@ -67,3 +67,16 @@ def test_gradient_is_not_added_to_the_memory_it_is_read_from():
     want = torch.tensor([2.0, 3.0, 1.0, 2.0], device="cuda")[:, None].expand(4, 8)
     assert torch.equal(buf[:, 8:16], want) and (buf[:, :8] == 1).all() and (buf[:, 16:] == 1).all()
     E.embedding_grad(flat[:32].view(4, 8), tokens, 4, out=flat[64:96].view(4, 8))
+
+
+def test_gradient_is_not_added_to_a_leaf():
+    from mamba3_b200 import embedding as E
+
+    tokens, dy = torch.arange(3, device="cuda"), torch.ones(3, 8, device="cuda")
+    leaf = torch.zeros(4, 8, device="cuda").requires_grad_(True)
+    with pytest.raises(ValueError, match="leaf"):
+        E.embedding_grad(dy, tokens, 4, out=leaf)
+    assert not leaf.any()
+    with torch.no_grad():  # as torch's own in-place operations
+        E.embedding_grad(dy, tokens, 4, out=leaf)
+    assert (leaf[:3] == 1).all() and not leaf[3].any()
