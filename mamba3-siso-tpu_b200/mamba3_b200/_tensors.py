@@ -6,6 +6,7 @@ import math
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi as C
 
@@ -158,6 +159,13 @@ def call(fn, args, device):
         rc = fn(args, _raw_stream(device.index) if _raw_stream else stream_handle(device))
     if rc:
         C.check(rc)
+
+
+def no_tangent(name, t):
+    """Refuses a dual tensor: `torch.autograd.forward_ad` marks it neither by requires_grad nor by its memory,
+    and a kernel's result would come without the tangent."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def written(t):

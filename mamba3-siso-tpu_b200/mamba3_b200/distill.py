@@ -132,7 +132,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
                  temperature: float = 1.0, labels: Optional[torch.Tensor] = None, hard_weight: float = 0.0,
                  weights: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
     """The loss of ``logits (..., V)`` (bf16 or f32) against ``teacher_ids`` / ``teacher_logits``
-    ``(..., k)``, k <= 128; differentiable in ``logits`` alone.
+    ``(..., k)``, k <= 128; differentiable in ``logits`` alone, once and in reverse mode.
 
     A negative id is an absent entry, a negative label an absent label; the teacher's logits
     may be shifted by any constant (log probabilities do).  ``weights (...)`` weigh the rows; a
@@ -144,6 +144,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     With gradients enabled a "mean" or "sum" forms the gradient together with the loss, in memory of
     the logits' size that the backward hands on; a backward whose upstream gradient is not 1 (a
     scaled loss) reads the logits again, where `distill_loss_and_grad`'s ``grad_scale`` does not."""
+    T.no_tangent("distill_loss", logits)
     side = _check(logits, teacher_ids, teacher_logits, labels, weights, temperature, hard_weight, reduction)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _DistillFn.apply(logits, *side, float(temperature), float(hard_weight), reduction)

@@ -59,9 +59,11 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
                  dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``table (V, D)`` bf16 or f32, ``tokens (...)`` int -> ``(..., D)`` in ``dtype`` (the table's
     by default).  A negative token is padding: a zero row without gradient; one at or past V
-    gives a NaN row.  Differentiable in ``table`` (a dense gradient in its dtype)."""
+    gives a NaN row.  Differentiable in ``table``, once and in reverse mode (a dense gradient in its
+    dtype)."""
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"table must be (vocab, dim), got {tuple(table.shape)}")
+    T.no_tangent("embed_tokens", table)
     tokens = _check_tokens(tokens, table)
     dtype = table.dtype if dtype is None else dtype
     if table.requires_grad and torch.is_grad_enabled():

@@ -80,3 +80,24 @@ def test_gradient_is_not_added_to_a_leaf():
     with torch.no_grad():  # as torch's own in-place operations
         E.embedding_grad(dy, tokens, 4, out=leaf)
     assert (leaf[:3] == 1).all() and not leaf[3].any()
+
+
+def test_forward_mode_is_refused():
+    """There is no forward-mode derivative; a result without its tangent would be a derivative of 0."""
+    import torch.autograd.forward_ad as fw
+    from mamba3_b200 import distill as D
+    from mamba3_b200 import embedding as E
+
+    x, ids, teacher = _lists(4, 50)
+    tokens = ids[:, 0]
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for mode in (torch.enable_grad(), torch.no_grad()):
+            with mode:
+                for reduction in ("mean", "sum", "none"):
+                    with pytest.raises(NotImplementedError):
+                        D.distill_loss(dual, ids, teacher, reduction=reduction)
+                with pytest.raises(NotImplementedError):
+                    E.embed_tokens(dual, tokens % 4)
+                D.distill_loss(x, ids, teacher)  # tensors without a tangent go on
+                E.embed_tokens(x, tokens % 4)
