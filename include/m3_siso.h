@@ -429,6 +429,7 @@ int m3_token_logprobs(const M3ScoreArgs *args, void *stream);
  *   g w [ (1 - hard_weight) T (softmax(x / T) - p) + hard_weight (softmax(x) - onehot(label)) ]
  * times grad_scale and, for M3_REDUCE_MEAN, over sum(w); g is `upstream` (element r *
  * upstream_stride; NULL = 1).  An id that occurs twice counts with both probabilities.
+ * KL is a difference of fp32 logarithms: the loss holds T^2 times their rounding (some 1e-7).
  * label < 0: no CE term; no id >= 0: no KL term; a row with neither or with w == 0 has loss 0
  * and gradient 0 whatever its logits are.  An id or label >= vocab makes the row NaN. */
 enum { M3_REDUCE_NONE = 0, M3_REDUCE_SUM = 1, M3_REDUCE_MEAN = 2 };
@@ -436,7 +437,7 @@ enum { M3_REDUCE_NONE = 0, M3_REDUCE_SUM = 1, M3_REDUCE_MEAN = 2 };
 typedef struct M3DistillArgs {
   int32_t rows_outer, rows_inner, vocab, k;      /* 1 <= k <= M3_MAX_TOP */
   int32_t logits_dtype, reduction;
-  float temperature, hard_weight, grad_scale;    /* T in [1e-30, 1e30], 0 <= hard_weight <= 1 */
+  float temperature, hard_weight, grad_scale;    /* T in [1e-30, 1e18], 0 <= hard_weight <= 1 */
   const void *logits;     int64_t ld_outer, ld_inner;
   const int64_t *ids;                            /* (rows, k) dense */
   const float *teacher;                          /* (rows, k) dense */

@@ -24,6 +24,7 @@ using namespace vocab;
 constexpr int kNV = 8;          // vectors a thread loads at a time
 constexpr int kMaxCluster = 8;  // CTAs per row (portable size)
 constexpr int kEnt = M3_MAX_TOP / 32;  // entries a lane holds at most
+constexpr float kMostTemperature = 1e18f;  // T * T is a finite factor of the loss
 
 struct Params {
   int rows, vocab, k, cluster, log2_cluster;
@@ -199,7 +200,8 @@ __device__ __forceinline__ float row_loss(const Params& p, const Row& r, int fla
   for (int e = 0; e < KE; ++e)  // an entry of probability 0 has no term
     if (en.p[e] != 0.f) kl = fmaf(en.p[e], en.lp[e] - r.q.ln(en.x[e], p.inv_t), kl);
   kl = warp_sum(kl);
-  float loss = flags & kSoft ? (1.f - p.hard) * p.temperature * p.temperature * kl : 0.f;
+  // KL grows as 1 / T where T is small: T * T would leave fp32's range before T * (T * KL) does
+  float loss = flags & kSoft ? (1.f - p.hard) * (p.temperature * (p.temperature * kl)) : 0.f;
   if (HARD && (flags & kHard)) loss -= p.hard * r.q1.ln(xl, 1.f);
   return w * loss;
 }
@@ -760,8 +762,8 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
     return set_error(M3_ERR_UNSUPPORTED, "m3_distill: logits must be f32 or bf16");
   if (a.reduction < M3_REDUCE_NONE || a.reduction > M3_REDUCE_MEAN)
     return set_error(M3_ERR_ARG, "m3_distill: reduction must be NONE, SUM or MEAN");
-  if (!temperature_ok(a.temperature) || !(a.hard_weight >= 0.f && a.hard_weight <= 1.f))
-    return set_error(M3_ERR_ARG, "m3_distill: need a temperature > 0 (finite, as 1 / T) and 0 <= hard_weight <= 1");
+  if (!temperature_ok(a.temperature) || a.temperature > kMostTemperature || !(a.hard_weight >= 0.f && a.hard_weight <= 1.f))
+    return set_error(M3_ERR_ARG, "m3_distill: need a temperature in [1e-30, 1e18] and 0 <= hard_weight <= 1");
   const int64_t rows = (int64_t)a.rows_outer * a.rows_inner;
   if (rows > kMaxRows) return set_error(M3_ERR_SHAPE, "m3_distill: more than 2^30 rows");
   const bool only_grad = a.grad && !a.row_loss && !a.loss;

@@ -140,6 +140,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     the gradient whatever its logits are.  An id or label at or past V makes its row NaN.
     ``reduction``: "mean" over the weights' sum (or the row count), "sum", or "none" for the
     rows' losses.
+    ``temperature``: 1e-30 to 1e18; the loss holds T^2 times the rounding of fp32 logarithms (some
+    1e-7), the gradient T times that of fp32 probabilities.
 
     With gradients enabled a "mean" or "sum" forms the gradient together with the loss, in memory of
     the logits' size that the backward hands on; a backward whose upstream gradient is not 1 (a

@@ -41,3 +41,12 @@ def test_memory_apart():
             assert not (meet and T.apart(a, b))
             if a.dim() == b.dim() == 2 and a.stride(0) == b.stride(0) == 24:
                 assert T.apart(a, b) == (not meet)
+
+
+def test_distillation_refuses_temperatures_whose_square_is_no_number():
+    a = C.M3DistillArgs()
+    a.rows_outer, a.rows_inner, a.vocab, a.k = 1, 1, 10, 3
+    a.logits, a.ids, a.teacher, a.row_loss = 16, 16, 16, 16
+    for t in (1e19, 1e30):
+        a.temperature = t
+        assert C.lib().m3_distill(a, None) == C.M3_ERR_ARG

@@ -1,0 +1,52 @@
+"""The vocabulary-end operators at the ends of their ranges: temperatures, rows without weight,
+distributions on one entry."""
+
+import math
+
+import pytest
+import torch
+
+from tests import vocab_ref as R
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("vocab", [200, 3000, 40000])
+@pytest.mark.parametrize("temperature", [2.0 ** -99, 2.0 ** -66, 2.0 ** -40, 2.0 ** -10])
+def test_distillation_at_low_temperatures(vocab, temperature):
+    """T^2 KL where T^2 is not an fp32 number.  Both distributions are on one entry (logits apart by more than
+    2^-10 * 100), so that KL = (x_max - x_id) / T and the loss T (x_max - x_id), to a few roundings (1e-5)."""
+    from mamba3_b200 import distill as D
+
+    g = torch.Generator().manual_seed(vocab)
+    rows, k = 5, 7
+    x = torch.stack([torch.randperm(vocab, generator=g) for _ in range(rows)]).float() / 8
+    ids = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(rows)])
+    teacher = torch.stack([torch.randperm(k, generator=g) for _ in range(rows)]).float()
+    xd = x.double().requires_grad_(True)
+    want = R.distill_rows(xd, ids, teacher, None, None, temperature, 0.0)
+    grad, = torch.autograd.grad(want.sum(), xd)
+    args = (x.cuda(), ids.cuda(), teacher.cuda())
+    got = D.distill_loss(*args, temperature=temperature, reduction="none").double().cpu()
+    assert (want > 0).all()
+    assert ((got - want).abs() <= 1e-5 * want.abs()).all()
+    loss, dx = D.distill_loss_and_grad(*args, temperature=temperature, reduction="sum")
+    assert abs(float(loss) - float(want.sum())) <= 1e-5 * float(want.sum())
+    assert ((dx.double().cpu() - grad).abs() <= 1e-5 * grad.abs() + 1e-40).all()  # 1e-40: below fp32
+
+
+@pytest.mark.parametrize("vocab", [200, 40000])
+def test_distillation_at_high_temperatures(vocab):
+    from mamba3_b200 import distill as D
+
+    g = torch.Generator().manual_seed(vocab)
+    x, teacher = torch.randn(4, vocab, generator=g).cuda(), torch.randn(4, 6, generator=g).cuda()
+    ids = torch.randint(0, vocab, (4, 6), generator=g).cuda()
+    for t in (1e19, 1e30):  # T^2 is past fp32
+        with pytest.raises(ValueError):
+            D.distill_loss(x, ids, teacher, temperature=t)
+        with pytest.raises(ValueError):
+            D.distill_loss_and_grad(x, ids, teacher, temperature=t)
+    loss, dx = D.distill_loss_and_grad(x, ids, teacher, temperature=1e18)
+    assert torch.isfinite(loss) and torch.isfinite(dx).all()
