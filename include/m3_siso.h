@@ -429,6 +429,7 @@ int m3_token_logprobs(const M3ScoreArgs *args, void *stream);
  *   g w [ (1 - hard_weight) T (softmax(x / T) - p) + hard_weight (softmax(x) - onehot(label)) ]
  * times grad_scale and, for M3_REDUCE_MEAN, over sum(w); g is `upstream` (element r *
  * upstream_stride; NULL = 1).  An id that occurs twice counts with both probabilities.
+ * A mean over weights that are all 0 is 0.
  * KL is a difference of fp32 logarithms: the loss holds T^2 times their rounding (some 1e-7).
  * label < 0: no CE term; no id >= 0: no KL term; a row with neither or with w == 0 has loss 0
  * and gradient 0 whatever its logits are.  An id or label >= vocab makes the row NaN. */

@@ -667,7 +667,8 @@ __global__ void __launch_bounds__(kSumThreads)
   if (rank == 0 && tid == 0) {
     s = 0.f;
     for (int r = 0; r < kSumCtas; ++r) s += total[r];
-    *out = s * scale / (div_by ? *div_by : 1.f);
+    const float by = div_by ? *div_by : 1.f;
+    *out = s == 0.f && by == 0.f ? 0.f : s * scale / by;  // no row has a weight: 0, as the gradient
   }
 }
 

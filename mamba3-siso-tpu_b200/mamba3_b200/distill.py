@@ -139,7 +139,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     row of weight 0, or with neither entries nor label, contributes exactly 0 to the loss and
     the gradient whatever its logits are.  An id or label at or past V makes its row NaN.
     ``reduction``: "mean" over the weights' sum (or the row count), "sum", or "none" for the
-    rows' losses.
+    rows' losses.  A mean over weights that are all 0 is 0 (a rank's shard of padding).
     ``temperature``: 1e-30 to 1e18; the loss holds T^2 times the rounding of fp32 logarithms (some
     1e-7), the gradient T times that of fp32 probabilities.
 

@@ -50,3 +50,31 @@ def test_distillation_at_high_temperatures(vocab):
             D.distill_loss_and_grad(x, ids, teacher, temperature=t)
     loss, dx = D.distill_loss_and_grad(x, ids, teacher, temperature=1e18)
     assert torch.isfinite(loss) and torch.isfinite(dx).all()
+
+
+@pytest.mark.parametrize("vocab", [256, 3001, 40000])
+@pytest.mark.parametrize("hard", [0.0, 0.5])
+def test_mean_over_rows_without_weight(vocab, hard):
+    """No row contributes: loss and gradient are 0, as for a single row of weight 0."""
+    from mamba3_b200 import distill as D
+
+    x = torch.randn(6, vocab, device="cuda")
+    x[1] = math.nan
+    ids = torch.randint(0, vocab, (6, 4), device="cuda")
+    teacher, weights = torch.randn(6, 4, device="cuda"), torch.zeros(6, device="cuda")
+    args = dict(weights=weights, hard_weight=hard, labels=ids[:, 1] if hard else None)
+    for reduction in ("mean", "sum"):
+        loss, dx = D.distill_loss_and_grad(x, ids, teacher, reduction=reduction, **args)
+        assert float(loss) == 0.0 and not dx.any()
+        leaf = x.clone().requires_grad_(True)
+        loss = D.distill_loss(leaf, ids, teacher, reduction=reduction, **args)
+        (2.0 * loss).backward()
+        assert float(loss) == 0.0 and not leaf.grad.any()
+        with torch.no_grad():
+            assert float(D.distill_loss(x, ids, teacher, reduction=reduction, **args)) == 0.0
+    weights[2] = 0.5  # a mean over one row
+    loss, _ = D.distill_loss_and_grad(x, ids, teacher, **args)
+    rows = D.distill_loss(x, ids, teacher, reduction="none", **args)
+    assert float(loss) == float(rows[2]) * 2.0
+    x[2, 0] = math.nan
+    assert torch.isnan(D.distill_loss_and_grad(x, ids, teacher, **args)[0])
