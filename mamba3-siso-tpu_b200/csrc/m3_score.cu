@@ -85,7 +85,8 @@ __device__ __forceinline__ Log2P distribution(const Part& a, bool plain, float c
 }
 __device__ __forceinline__ void write_row(const Params& p, const Part& a, const Log2P& q, int row) {
   p.lse[row] = q.lse(p.inv_t);
-  p.entropy[row] = (q.l2 - a.u / a.s) * kLn2;
+  const float h = (q.l2 - a.u / a.s) * kLn2;
+  p.entropy[row] = h < 0.f ? 0.f : h;  // below 0 by rounding; NaN stays
 }
 __device__ __forceinline__ void write_target(const Params& p, const Log2P& q, int row, int64_t t, float xt) {
   p.logprob[row] = t < 0 ? 0.f : t >= p.vocab ? NAN : q.ln(xt, p.inv_t);

@@ -301,8 +301,8 @@ struct Log2P {
   __device__ __forceinline__ float ln(float x, float inv_t) const {
     const float d = exponent(x);
     // log2(e) x may overflow where x does not
-    if (fabsf(d) == INFINITY && fabsf(x) != INFINITY) return fmaf(x, inv_t, -lse(inv_t));
-    return (d - l2) * kLn2;
+    const float r = fabsf(d) == INFINITY && fabsf(x) != INFINITY ? fmaf(x, inv_t, -lse(inv_t)) : (d - l2) * kLn2;
+    return r > 0.f ? 0.f : r;  // above 0 by rounding; NaN stays
   }
 };
 

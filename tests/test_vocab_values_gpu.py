@@ -78,3 +78,31 @@ def test_mean_over_rows_without_weight(vocab, hard):
     assert float(loss) == float(rows[2]) * 2.0
     x[2, 0] = math.nan
     assert torch.isnan(D.distill_loss_and_grad(x, ids, teacher, **args)[0])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("vocab", [1, 2, 200, 700, 5000, 40000, 300000])
+def test_probabilities_of_at_most_one(vocab, dtype):
+    """Rows on one entry: a log probability is never above 0 nor an entropy below it, and both are within
+    the rounding of a sum (|logit| 2^-22) of 0."""
+    from mamba3_b200 import scoring as S
+
+    g = torch.Generator().manual_seed(vocab)
+    rows, top = 40, min(vocab, 3)
+    at = torch.randint(0, vocab, (rows,), generator=g)
+    x = torch.full((rows, vocab), -math.inf)
+    x[::2] = torch.randn(rows // 2, vocab, generator=g) - 300  # the rest: 2^-300 and less
+    x[torch.arange(rows), at] = torch.randn(rows, generator=g) * 20
+    x = x.to(dtype)
+    x, at = x.cuda(), at.cuda()
+    for temperature in (1.0, 0.7, 1.9):
+        for k in (0, top):
+            r = S.token_logprobs(x, at, top=k, temperature=temperature)
+            tol = float(x.max()) / temperature * 2.0 ** -22 + 1e-6
+            assert float(r.entropy.min()) >= 0.0 and float(r.entropy.max()) <= tol
+            assert float(r.logprob.max()) <= 0.0 and float(r.logprob.min()) >= -tol
+            if k:
+                assert float(r.top_logprob.max()) <= 0.0 and torch.equal(r.top_ids[:, 0], at)
+    x[3, 0] = math.nan
+    r = S.token_logprobs(x, at, top=top)
+    assert torch.isnan(r.entropy[3]) and torch.isnan(r.logprob[3]) and torch.isfinite(r.entropy[:3]).all()
