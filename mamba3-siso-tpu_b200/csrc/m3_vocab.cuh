@@ -353,7 +353,9 @@ int launch_ex(const char* what, void (*kern)(P...), dim3 grid, int block, size_t
     ++cfg.numAttrs;
   }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  return e == cudaSuccess ? M3_OK : set_error(M3_ERR_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
+  if (e == cudaSuccess) return M3_OK;
+  cudaGetLastError();  // else the next call's check would report it again
+  return set_error(M3_ERR_LAUNCH, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 }  // namespace vocab

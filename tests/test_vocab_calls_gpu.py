@@ -101,3 +101,15 @@ def test_forward_mode_is_refused():
                     E.embed_tokens(dual, tokens % 4)
                 D.distill_loss(x, ids, teacher)  # tensors without a tangent go on
                 E.embed_tokens(x, tokens % 4)
+
+
+def test_a_failed_call_does_not_fail_the_next():
+    """Rows too wide for the gradient's launches are refused; the call after it is not blamed for that."""
+    from mamba3_b200 import embedding as E
+
+    dim = 600001  # odd: one column a thread
+    tokens, dy = torch.arange(40, device="cuda") % 4, torch.ones(40, dim, device="cuda")
+    with pytest.raises(ValueError):
+        E.embedding_grad(dy, tokens, 4)
+    out = E.embed_tokens(torch.ones(4, 8, device="cuda"), tokens, scale=3.0)
+    assert (out == 3).all()
