@@ -621,13 +621,21 @@ int launch_sum(SumParams p, int64_t rows, cudaStream_t s) {
 }
 
 template <typename D, typename G>
-int launch_sum(const SumParams& p, int64_t rows, int64_t dy_outer, int64_t dy_inner, cudaStream_t s) {
-  auto fits = [&](int n) {
-    return whole(p.dy, sizeof(D), n, p.dim, dy_outer, dy_inner) && whole(p.grad, sizeof(G), n, p.dim, p.grad_ld, 0);
-  };
-  if (fits(8)) return launch_sum<D, G, 8>(p, rows, s);
-  if (fits(2)) return launch_sum<D, G, 2>(p, rows, s);
+int launch_sum(const SumParams& p, int n, int64_t rows, cudaStream_t s) {
+  if (n == 8) return launch_sum<D, G, 8>(p, rows, s);
+  if (n == 2) return launch_sum<D, G, 2>(p, rows, s);
   return launch_sum<D, G, 1>(p, rows, s);
+}
+
+// Columns a thread takes of the gradient's rows: what the alignment of both allows.
+int sum_columns(const M3EmbedBwdArgs& a, int dy_size, int grad_size) {
+  for (int n : {8, 2})
+    if (whole(a.dy, dy_size, n, a.dim, a.dy_outer, a.dy_inner) && whole(a.grad, grad_size, n, a.dim, a.grad_ld, 0)) return n;
+  return 1;
+}
+// Whether the grids of launch_sum's kernels reach all columns.
+bool grids_reach(int dim, int n, bool join) {
+  return slabs(dim, n, columns(dim, n)) <= 65535 && (!join || (dim + n * kJoinWidth - 1) / (n * kJoinWidth) <= 65535);
 }
 
 }  // namespace
@@ -690,6 +698,9 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   const size_t ds = a.dy_dtype == M3_DTYPE_BF16 ? 2 : 4, gs = a.grad_dtype == M3_DTYPE_BF16 ? 2 : 4;
   if (((uintptr_t)a.dy) % ds || ((uintptr_t)a.grad) % gs)
     return set_error(M3_ERR_ARG, "m3_embed_bwd: dy and grad must be aligned to their types");
+  const int columns_at_once = sum_columns(a, (int)ds, (int)gs);
+  if (!grids_reach(a.dim, columns_at_once, rows > chunk_of(rows, a.dim)))
+    return set_error(M3_ERR_SHAPE, "m3_embed_bwd: dim is too large");
   const size_t need = m3_embed_bwd_workspace_size(rows, a.dim);
   if (!a.workspace || a.workspace_bytes < need || ((uintptr_t)a.workspace) % 256)
     return set_error(M3_ERR_WORKSPACE, "m3_embed_bwd: 256-byte aligned workspace of " + std::to_string(need) +
@@ -746,8 +757,6 @@ extern "C" int m3_embed_bwd(const M3EmbedBwdArgs* args, void* stream) {
   using bf16 = __nv_bfloat16;
   const bool gb = a.grad_dtype == M3_DTYPE_BF16;
   if (a.dy_dtype == M3_DTYPE_BF16)
-    return gb ? launch_sum<bf16, bf16>(p, rows, a.dy_outer, a.dy_inner, s)
-              : launch_sum<bf16, float>(p, rows, a.dy_outer, a.dy_inner, s);
-  return gb ? launch_sum<float, bf16>(p, rows, a.dy_outer, a.dy_inner, s)
-            : launch_sum<float, float>(p, rows, a.dy_outer, a.dy_inner, s);
+    return gb ? launch_sum<bf16, bf16>(p, columns_at_once, rows, s) : launch_sum<bf16, float>(p, columns_at_once, rows, s);
+  return gb ? launch_sum<float, bf16>(p, columns_at_once, rows, s) : launch_sum<float, float>(p, columns_at_once, rows, s);
 }

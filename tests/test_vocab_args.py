@@ -50,3 +50,14 @@ def test_distillation_refuses_temperatures_whose_square_is_no_number():
     for t in (1e19, 1e30):
         a.temperature = t
         assert C.lib().m3_distill(a, None) == C.M3_ERR_ARG
+
+
+def test_embedding_gradient_refuses_widths_before_it_writes():
+    """The widest rows that the launches' grids reach: 65535 times 8 threads' columns, 1, 2 or 8 a thread."""
+    a = C.M3EmbedBwdArgs()
+    a.rows_outer, a.rows_inner, a.vocab, a.scale = 1, 1000, 4, 1.0  # more than one chunk of rows
+    a.tokens, a.grad, a.workspace, a.workspace_bytes = 16, 256, 256, 1 << 40
+    for dim, dy in ((65535 * 8 + 1, 256), (65535 * 16 + 2, 256), (65535 * 64 + 8, 256), (65535 * 8 + 8, 260)):
+        a.dim = a.grad_ld = a.dy_inner = a.dy_outer = dim
+        a.dy = dy
+        assert C.lib().m3_embed_bwd(a, None) == C.M3_ERR_SHAPE
