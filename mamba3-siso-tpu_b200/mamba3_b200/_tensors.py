@@ -137,6 +137,13 @@ def row_counts(lead):
     return (outer, inner) if inner else (0, 1)
 
 
+def vocab_of(n, most):
+    """A vocabulary that the kernels' ints hold (a wider one would be cut to 32 bits on its way to them)."""
+    if not 1 <= n <= most:
+        raise ValueError(f"a vocabulary of {n}: from 1 to {most} are supported")
+    return n
+
+
 def require_here(device, *ts):
     """Every given tensor is on the CUDA device ``device``."""
     if device.type != "cuda":

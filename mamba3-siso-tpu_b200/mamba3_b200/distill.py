@@ -45,6 +45,7 @@ def _check(logits, ids, teacher, labels, weights, temperature, hard_weight, redu
     shape = logits.shape
     if not shape or shape[-1] < 1:
         raise ValueError(f"logits must be (..., vocab), got {tuple(shape)}")
+    T.vocab_of(shape[-1], 1 << 30)
     T.require_here(logits.device, ids, teacher, labels, weights)
     lead = shape[:-1]
     k = ids.shape[-1] if ids.dim() else 0

@@ -14,6 +14,8 @@ import torch
 from . import _capi as C
 from . import _tensors as T
 
+_MOST_VOCAB = 2 ** 31 - 1
+
 
 def _check_tokens(tokens, ref):
     """The tokens as the kernels read them (int64)."""
@@ -63,6 +65,7 @@ def embed_tokens(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0,
     dtype)."""
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"table must be (vocab, dim), got {tuple(table.shape)}")
+    T.vocab_of(table.shape[0], _MOST_VOCAB)
     T.no_tangent("embed_tokens", table)
     tokens = _check_tokens(tokens, table)
     dtype = table.dtype if dtype is None else dtype
@@ -79,8 +82,7 @@ def embedding_grad(dy: torch.Tensor, tokens: torch.Tensor, vocab: int, scale: fl
     has left there.  It shares no memory with ``dy``, and its version is raised."""
     if dy.dim() != tokens.dim() + 1 or dy.shape[:-1] != tokens.shape or dy.shape[-1] < 1:
         raise ValueError(f"dy must be {tuple(tokens.shape)} + (dim,), got {tuple(dy.shape)}")
-    if vocab < 1:
-        raise ValueError(f"vocab must be >= 1, got {vocab}")
+    T.vocab_of(vocab, _MOST_VOCAB)
     tokens = _check_tokens(tokens, dy)
     lead, dim, dev = tokens.shape, dy.shape[-1], dy.device
     add = out is not None

@@ -37,7 +37,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     shape, dev = logits.shape, logits.device
     if not shape or shape[-1] < 1:
         raise ValueError(f"logits must be (..., vocab), got {tuple(shape)}")
-    lead, vocab = shape[:-1], shape[-1]
+    lead, vocab = shape[:-1], T.vocab_of(shape[-1], 1 << 30)
     T.require_here(dev, targets)
     if not 0 <= top <= min(vocab, C.M3_MAX_TOP):
         raise ValueError(f"top must be in [0, {min(vocab, C.M3_MAX_TOP)}], got {top}")

@@ -113,3 +113,20 @@ def test_a_failed_call_does_not_fail_the_next():
         E.embedding_grad(dy, tokens, 4)
     out = E.embed_tokens(torch.ones(4, 8, device="cuda"), tokens, scale=3.0)
     assert (out == 3).all()
+
+
+def test_sizes_past_32_bits_are_refused():
+    """A vocabulary of 2^32 + 256 is not one of 256."""
+    from mamba3_b200 import distill as D
+    from mamba3_b200 import embedding as E
+    from mamba3_b200 import scoring as S
+
+    one = torch.zeros(1, dtype=torch.bfloat16, device="cuda")
+    logits = one.expand(2 ** 32 + 256)  # no memory of that size
+    ids, teacher = torch.zeros(3, dtype=torch.int64, device="cuda"), torch.zeros(3, device="cuda")
+    for call in (lambda: S.token_logprobs(logits), lambda: D.distill_loss(logits, ids, teacher),
+                 lambda: D.distill_loss_and_grad(logits, ids, teacher),
+                 lambda: E.embed_tokens(one[:, None].expand(2 ** 32 + 8, 1), ids),
+                 lambda: E.embedding_grad(torch.zeros(3, 1, device="cuda"), ids, 2 ** 32 + 8)):
+        with pytest.raises(ValueError, match="vocab"):
+            call()
