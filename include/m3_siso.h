@@ -398,8 +398,8 @@ int m3_gated_act_bf16(const void *x, int64_t x_row_stride, void *out, int64_t ou
  * The vocabulary end of the language model.  No counterparts in the reference, which leaves
  * these to XLA (embed[tokens], log_softmax, its gradient).  Rows are addressed by two levels
  * of element strides, row r at (r / rows_inner) * outer + (r % rows_inner) * inner, so that
- * logits[:, :-1] and tokens[:, 1:] need no copy; the vocabulary axis is contiguous.  All
- * arithmetic is fp32.  Results are the same every call (no floating-point atomics).
+ * logits[:, :-1] and tokens[:, 1:] need no copy; the vocabulary axis is contiguous.  At most
+ * 2^30 rows.  All arithmetic is fp32.  Results are the same every call (no floating-point atomics).
  * ------------------------------------------------------------------------------- */
 #define M3_MAX_TOP 128
 

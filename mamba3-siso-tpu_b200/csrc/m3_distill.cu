@@ -8,11 +8,13 @@
 // rest from L2 (so that the rows in flight have to fit there), and its gradient written.  One warp holds
 // the teacher's entries.  The dense gradient k_s q is stored first; then each entry's place is stored
 // again as k_s q - p, from the same fp32 values, so that every element is rounded once.
-// Floor: one read and one write.  Measured with the gradient: 4096 x 128256 bf16 401 us (5.2 TB/s of the 6.4
-// that a copy reaches; exponentials take the SFU 230 us of it, and the rows of two CTAs an SM pass through
-// the phases at the same time), 32768 x 8192 f32 329 us (6.5 TB/s), 131072 x 256 bf16 with weights 72 us
-// (2.2 TB/s, bound by about 430 instructions a row).  Reading the whole row again from L2 took 535 us at the
-// first size with four rows an SM in flight (150 MB, more than L2), 430 with two.
+// Floor: one read and one write.  Measured with the gradient: 4096 x 128256 bf16 397 to 420 us (5.0 to 5.3 TB/s of
+// the 6.4 that a copy reaches; the SFU is busy 62 % of the time with the exponentials and the issue slots 39 %, so
+// that it is how the phases of two CTAs an SM overlap that decides), 32768 x 8192 f32 332 us (6.5 TB/s), 131072 x 256
+// bf16 with weights 72 us (2.2 TB/s, bound by about 440 instructions a row).  Reading the whole row again from L2
+// took 535 us at the first size with four rows an SM in flight (150 MB, more than L2), 430 with two.
+// The loss alone: 168 us at the first size; with hard labels 427, as the 64 registers of a thread then hold a bf16
+// tile only with 488 bytes of them spilled (f32, 4095 x 50257: 136 and 146).
 #include "m3_internal.h"
 #include "m3_vocab.cuh"
 
