@@ -645,10 +645,12 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpCtas<NV, KE, HARD>) distill
 }
 
 // out = scale * (sum of n values) / (*div_by, if given), by one cluster in a fixed order.
+// v is not __restrict__: the kernel in front may still be writing it when this one starts, and a load through
+// the read-only path, which __restrict__ allows, need not stay behind after_previous().
 constexpr int kSumCtas = 8, kSumThreads = 1024;
 
 __global__ void __launch_bounds__(kSumThreads)
-    sum_kernel(const float* __restrict__ v, int64_t n, const float* div_by, float scale, float* out) {
+    sum_kernel(const float* v, int64_t n, const float* div_by, float scale, float* out) {
   __shared__ float sm[32], total[kSumCtas];
   const int tid = threadIdx.x, rank = cluster_rank();
   next_may_start();

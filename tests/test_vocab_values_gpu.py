@@ -106,3 +106,25 @@ def test_probabilities_of_at_most_one(vocab, dtype):
     x[3, 0] = math.nan
     r = S.token_logprobs(x, at, top=top)
     assert torch.isnan(r.entropy[3]) and torch.isnan(r.logprob[3]) and torch.isfinite(r.entropy[:3]).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(5000, 64), (9, 40000), (700, 3000)])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_losses_of_calls_in_a_row(rows, vocab, weighted):
+    """The sum of the rows' losses starts before they are all written and waits for them: calls one behind the
+    other, whose workspaces are the same memory, each give their own.  A sum of positive terms in a tree of
+    fewer than 40 levels: 40 * 2^-24 relative, and as much for the weights' sum."""
+    from mamba3_b200 import distill as D
+
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    ids = torch.randint(0, vocab, (rows, 4), generator=g, device="cuda")
+    teacher = torch.randn(rows, 4, generator=g, device="cuda")
+    xs = [torch.randn(rows, vocab, generator=g, device="cuda") * (1 + i) for i in range(4)]
+    ws = [torch.rand(rows, generator=g, device="cuda") + 0.1 if weighted else None for _ in xs]
+    losses = [D.distill_loss(xs[i % 4], ids, teacher, weights=ws[i % 4]) for i in range(60)]
+    steps = [D.distill_loss_and_grad(xs[i % 4], ids, teacher, weights=ws[i % 4])[0] for i in range(8)]
+    for i in range(4):
+        per_row = D.distill_loss(xs[i], ids, teacher, weights=ws[i], reduction="none").double()
+        want = float(per_row.sum() / (rows if ws[i] is None else ws[i].double().sum()))
+        for got in losses[i::4] + steps[i::4]:
+            assert abs(float(got) - want) <= 80 * 2.0 ** -24 * want
