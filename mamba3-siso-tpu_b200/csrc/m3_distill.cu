@@ -40,7 +40,7 @@ struct Params {
   const float* weight_sum;  // a mean's divisor, NULL = none
   float* row_loss;
   bool ready;  // grad holds the gradient for an upstream of 1
-  bool early;  // the sum of weights is the kernel in front of this one
+  bool early;  // the sum of weights is the kernel in front of this one, which may start before that has ended
 };
 
 // The gradient is there already (the same for all threads).
@@ -810,14 +810,15 @@ extern "C" int m3_distill(const M3DistillArgs* args, void* stream) {
   p.upstream = a.upstream;
   p.upstream_stride = a.upstream_stride;
   p.weight_sum = wmean ? a.weight_sum : nullptr;
-  p.early = wmean && !(a.ready & M3_READY_WEIGHTS);
   p.ready = (a.ready & M3_READY_GRAD) != 0;
+  const bool sum_weights = wmean && !(a.ready & M3_READY_WEIGHTS);
+  p.early = sum_weights && !p.ready;  // with nothing to do it would end without waiting for the sum
   p.row_loss = a.row_loss;
   auto sum = [&](const float* v, const float* div_by, float scale, float* out, bool early) {
     return launch_ex("m3_distill", sum_kernel, kSumCtas, kSumThreads, 0, kSumCtas, early, s, v, (int64_t)rows, div_by, scale, out);
   };
   int rc = M3_OK;
-  if (p.early) rc = sum(a.weights, nullptr, 1.f, a.weight_sum, false);
+  if (sum_weights) rc = sum(a.weights, nullptr, 1.f, a.weight_sum, false);
   if (rc == M3_OK && rows > 0) {
     const int nvec = most_vectors(a.logits, a.vocab, bf ? 2 : 4, a.ld_outer, a.ld_inner);
     rc = bf ? launch<__nv_bfloat16>(p, nvec, s) : launch<float>(p, nvec, s);

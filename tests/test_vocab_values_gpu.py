@@ -128,3 +128,25 @@ def test_losses_of_calls_in_a_row(rows, vocab, weighted):
         want = float(per_row.sum() / (rows if ws[i] is None else ws[i].double().sum()))
         for got in losses[i::4] + steps[i::4]:
             assert abs(float(got) - want) <= 80 * 2.0 ** -24 * want
+
+
+@pytest.mark.parametrize("upstream", [1.0, 2.0])
+@pytest.mark.parametrize("vocab", [64, 3000, 40000])
+def test_ready_gradient_without_ready_weights(vocab, upstream):
+    """The C entry with a gradient that is there and a weight sum that is not: left alone or written anew."""
+    from mamba3_b200 import _capi as C
+    from mamba3_b200 import _tensors as T
+    from mamba3_b200 import distill as D
+
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x, teacher = torch.randn(50, vocab, generator=g, device="cuda"), torch.randn(50, 4, generator=g, device="cuda")
+    ids, w = torch.randint(0, vocab, (50, 4), generator=g, device="cuda"), torch.rand(50, generator=g, device="cuda") + 0.1
+    _, want = D.distill_loss_and_grad(x, ids, teacher, weights=w, grad_scale=upstream)
+    grad, up, total = torch.full_like(x, 7.0), torch.full((1,), upstream, device="cuda"), torch.zeros(1, device="cuda")
+    a = C.M3DistillArgs(1, 50, vocab, 4, T.io_dtype(x.dtype), C.M3_REDUCE_MEAN, 1.0, 0.0, 1.0, x.data_ptr(), 0, vocab,
+                        ids.data_ptr(), teacher.data_ptr(), None, w.data_ptr(), up.data_ptr(), 0, None, None,
+                        total.data_ptr(), grad.data_ptr(), 0, vocab, C.M3_READY_GRAD, 0)
+    T.call(C.lib().m3_distill, a, x.device)
+    after = total.clone()  # behind the call in the stream: behind the sum of weights too
+    assert abs(float(after) - float(w.double().sum())) <= 1e-5 * 50
+    assert (grad == 7).all() if upstream == 1 else torch.equal(grad, want)
